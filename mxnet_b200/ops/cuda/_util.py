@@ -1,4 +1,6 @@
 """Helpers shared by the kernel wrappers."""
+import contextlib
+
 import torch
 
 from . import lib, ptr, stream_ptr, count_launch, check
@@ -45,3 +47,14 @@ def job_wide(choice):
     flag = torch.tensor([1 if choice else 0], dtype=torch.int32, device='cuda')
     dist.broadcast_(flag, 0)
     return bool(int(flag.item()))
+
+
+def on_device(t):
+    """Context in which the device of ``t`` is the current one (the raw launchers start their kernels there); the caller's
+    current device is put back on exit."""
+    if t.device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(t.device)
+
+
+_HERE = contextlib.nullcontext()

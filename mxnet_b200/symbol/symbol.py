@@ -119,7 +119,7 @@ def _parse_attr(s):
 # is meant to save), the ones with running state, and the sources of randomness.
 _NO_MIRROR = frozenset(['Convolution', 'Deconvolution', 'FullyConnected', 'Concat', 'SoftmaxOutput', 'BatchNorm', 'SyncBatchNorm',
                         '_contrib_SyncBatchNorm', 'Dropout', 'RNN', 'Custom', 'dot', 'batch_dot', 'Embedding', '_FusedOp',
-                        '_contrib_fused_self_attention', '_contrib_interleaved_matmul_selfatt_qk',
+                        '_contrib_fused_self_attention', '_contrib_sldwin_attention', '_contrib_interleaved_matmul_selfatt_qk',
                         '_contrib_interleaved_matmul_selfatt_valatt', '_contrib_interleaved_matmul_encdec_qk',
                         '_contrib_interleaved_matmul_encdec_valatt', '_npi_matmul', '_npi_dot', '_npi_tensordot', '_npi_einsum',
                         '_foreach', '_while_loop', '_cond', 'CTCLoss', 'Correlation', '_contrib_DeformableConvolution'])
@@ -1031,6 +1031,8 @@ def _op_frontend(op):
                         pass
                     else:
                         continue
+                if nm == 'valid_length' and op.name in ('_contrib_sldwin_attention', '_contrib_sldwin_cache_fill'):
+                    continue
                 # a missing data input becomes the free variable ``<name>_data`` that composition fills later
                 # (``net(fc3_data=other)``), as every missing input does in the reference
                 s = var('%s_%s' % (name, nm))

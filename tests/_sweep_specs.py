@@ -166,6 +166,14 @@ simple('_contrib_sldwin_atten_score', lambda g: [f(g, 2, 6, 2, 4), f(g, 2, 6, 2,
        symmetric=True)
 simple('_contrib_sldwin_atten_mask_like',
        lambda g: [f(g, 2, 6, 2, 5), torch.ones(2, dtype=torch.int32), torch.tensor([6, 4], dtype=torch.int32)], w=2, symmetric=True)
+simple('_contrib_rotary_embedding', lambda g: [f(g, 2, 5, 3, 8), torch.arange(5) * 3, f(g, 3)], interleaved=True, scale=1.5)
+simple('_npx_rotary_inv_freq', lambda g: [], dim=8, scaling='yarn', factor=4.0, original_length=64)
+simple('_contrib_sldwin_attention', lambda g: [f(g, 2, 9, 4, 8), f(g, 2, 9, 2, 8), f(g, 2, 9, 2, 8), torch.tensor([9, 5])], window=3, sinks=1)
+simple('_contrib_sldwin_cache_fill', lambda g: [f(g, 2, 9, 2, 8), f(g, 2, 9, 2, 8), f(g, 2, 6, 2, 8), f(g, 2, 6, 2, 8), torch.tensor([9, 5])],
+       sinks=1)
+simple('_contrib_sldwin_attention_step',
+       lambda g: [f(g, 2, 4, 8), f(g, 2, 2, 8), f(g, 2, 2, 8), f(g, 2, 6, 2, 8), f(g, 2, 6, 2, 8), torch.tensor([9, 2])], window=3, sinks=1)
+simple('_contrib_token_log_probs', lambda g: [f(g, 3, 4, 11), i(g, 0, 11, 3, 4)], topk=3)
 simple('_contrib_sldwin_atten_context', lambda g: [f(g, 2, 6, 2, 5), f(g, 2, 6, 2, 4), torch.ones(2, dtype=torch.int32)], w=2,
        symmetric=True)
 
@@ -274,6 +282,7 @@ NO_GRADCHECK = {k: v for k, v in NO_GRADCHECK.items() if v}
 GRAD_INPUTS = {
     'ROIPooling': (0,), 'ROIAlign': (0,), 'RROIAlign': (0,), 'PSROIPooling': (0,), 'DeformablePSROIPooling': (0,),
     'MultiBoxDetection': (), 'Proposal': (), 'MultiProposal': (), 'CTCLoss': (0,),
+    '_contrib_rotary_embedding': (0,), '_contrib_sldwin_attention': (0, 1, 2), '_contrib_token_log_probs': (0,),
     '_contrib_sldwin_atten_score': (0, 1), '_contrib_sldwin_atten_context': (0, 1), '_contrib_sldwin_atten_mask_like': (0,),
 }
 
