@@ -235,6 +235,8 @@ static bool sw_shape_ok(const SwParams& p) {
          p.window <= p.T && p.sinks >= 0 && p.sinks <= p.T && p.T <= (1 << 30) && (int64_t)p.B * p.Hq <= 0x7fffffff;
 }
 
+#include "sldwin_tc.inl"
+
 }  // namespace mxb
 
 using namespace mxb;
@@ -244,7 +246,7 @@ MXB_EXPORT int mxb_sldwin_max_dim(void) { return kSwMaxD; }
 // dims: B, T, Hq, Hk, D, window (1 .. T), sinks (0 .. T).  strides: batch, position and head of q, k, v (and dO), in elements;
 // channels are adjacent.  lse: [B, Hq, T] floats (forward: may be null when no backward pass follows).
 MXB_EXPORT int mxb_sldwin_forward(int dtype, const void* q, const void* k, const void* v, const int* valid, void* out, float* lse,
-                                  const int* dims, const int64_t* strides, float scale, void* stream) {
+                                  const int* dims, const int64_t* strides, float scale, int* error_flag, void* stream) {
   SwParams p{};
   p.q = q; p.k = k; p.v = v; p.valid = valid; p.out = out; p.lse = lse;
   p.B = dims[0]; p.T = dims[1]; p.Hq = dims[2]; p.Hk = dims[3]; p.D = dims[4]; p.window = dims[5]; p.sinks = dims[6];
@@ -254,6 +256,10 @@ MXB_EXPORT int mxb_sldwin_forward(int dtype, const void* q, const void* k, const
   p.scale = scale;
   if (!sw_shape_ok(p)) return -2;
   cudaStream_t st = (cudaStream_t)stream;
+  if (tc_takes(p, dtype)) {
+    if (dtype == kF16) return p.D == 64 ? tc_forward<__half, 64>(p, 0, error_flag, st) : tc_forward<__half, 128>(p, 0, error_flag, st);
+    return p.D == 64 ? tc_forward<__nv_bfloat16, 64>(p, 1, error_flag, st) : tc_forward<__nv_bfloat16, 128>(p, 1, error_flag, st);
+  }
   if (dtype == kF32) return sw_general<float>(p, 0, st);
   if (dtype == kF16) return sw_general<__half>(p, 0, st);
   if (dtype == kBF16) return sw_general<__nv_bfloat16>(p, 0, st);
@@ -263,7 +269,7 @@ MXB_EXPORT int mxb_sldwin_forward(int dtype, const void* q, const void* k, const
 // dq: [B, T, Hq, D], dk and dv: [B, T, Hk, D], contiguous; delta: [B, Hq, T] floats of workspace.
 MXB_EXPORT int mxb_sldwin_backward(int dtype, const void* q, const void* k, const void* v, const int* valid, const void* o,
                                    const void* dout, const float* lse, float* delta, void* dq, void* dk, void* dv, const int* dims,
-                                   const int64_t* strides, float scale, void* stream) {
+                                   const int64_t* strides, float scale, int* error_flag, void* stream) {
   SwParams p{};
   p.q = q; p.k = k; p.v = v; p.valid = valid; p.o = o; p.dout = dout; p.lse = const_cast<float*>(lse); p.delta = delta;
   p.dq = dq; p.dk = dk; p.dv = dv;

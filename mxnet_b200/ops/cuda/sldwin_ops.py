@@ -13,12 +13,32 @@ _DIMS7, _DIMS6 = C.c_int * 7, C.c_int * 6
 _S6, _S12 = C.c_int64 * 6, C.c_int64 * 12
 
 
+_report = []          # a word of pinned host memory that the kernels set when a wait inside them ran out, and its reader
+
+
+def _error_word():
+    if not _report:
+        if torch.cuda.is_current_stream_capturing():
+            return C.c_void_p(0)                                  # a capture allows no allocation of host memory
+        word = torch.zeros(1, dtype=torch.int32).pin_memory()
+        _report.extend((word, C.c_void_p(word.data_ptr()), C.c_int.from_address(word.data_ptr())))
+    elif _report[2].value:
+        _report[2].value = 0
+        raise RuntimeError('an earlier call reported a barrier time-out inside its kernel: its results are not valid')
+    return _report[1]
+
+
 def _rows(t):
-    """``t`` with adjacent channels and no two elements in one place (an expanded axis is written out)."""
-    s = t.stride()
-    if s[3] == 1 and all(s[i] > 0 or t.shape[i] == 1 for i in range(3)):
-        return t
-    return t.contiguous()
+    """``t`` as the kernels read it: adjacent channels, no two elements in one place (an expanded axis is written out), and
+    where the rows are whole 16-byte units every row on a 16-byte boundary."""
+    s0, s1, s2, s3 = t.stride()
+    n0, n1, n2, n3 = t.shape
+    unit = 16 // t.element_size()
+    if s3 == 1 and (s0 > 0 or n0 == 1) and (s1 > 0 or n1 == 1) and (s2 > 0 or n2 == 1):
+        if n3 % unit or (t.data_ptr() % 16 == 0 and (s0 % unit == 0 or n0 == 1) and (s1 % unit == 0 or n1 == 1) and
+                         (s2 % unit == 0 or n2 == 1)):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _forward(q, k, v, valid, window, sinks, scale, keep):
@@ -29,7 +49,7 @@ def _forward(q, k, v, valid, window, sinks, scale, keep):
     strides = _S12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
     with on_device(q):
         check(lib().mxb_sldwin_forward(dt(q), ptr(q), ptr(k), ptr(v), ptr(valid), ptr(out), ptr(lse), dims, strides, scale,
-                                       stream_ptr(q.device)), 'sldwin_attention')
+                                       _error_word(), stream_ptr(q.device)), 'sldwin_attention')
     count_launch(1)
     return out, lse
 
@@ -58,7 +78,8 @@ class _SldwinAttention(torch.autograd.Function):
         strides = _S12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *dout.stride()[:3])
         with on_device(q):
             check(lib().mxb_sldwin_backward(dt(q), ptr(q), ptr(k), ptr(v), ptr(valid), ptr(out), ptr(dout), ptr(lse), ptr(delta), ptr(dq),
-                                            ptr(dk), ptr(dv), dims, strides, scale, stream_ptr(q.device)), 'sldwin_attention backward')
+                                            ptr(dk), ptr(dv), dims, strides, scale, _error_word(), stream_ptr(q.device)),
+                  'sldwin_attention backward')
         count_launch(2)
         return dq, dk, dv, None, None, None, None
 

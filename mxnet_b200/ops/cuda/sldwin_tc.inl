@@ -1,0 +1,459 @@
+// Sliding-window attention on the tcgen05 tensor cores, head sizes 64 and 128, fp16 and bf16 (included by
+// sldwin_attention.cu inside namespace mxb).
+//
+// Products with both operands in shared memory make scores in TMEM (S = Q K^T and the like); row threads turn them into
+// probabilities (or their gradients), written back to TMEM in the operand type over the scores they came from; products
+// with the first operand in TMEM accumulate the outputs there.  Nothing of a score passes through shared memory.
+// Tiles come by TMA out of strided [B, T, H, D] tensors (4-D maps, 128-byte swizzle, rows behind T read as zeros).
+// Every wait is bounded; on expiry the CTA reports through an error word, waits for its copies, frees its TMEM and ends.
+
+constexpr int kTcRows = 128;
+constexpr uint32_t kTcHalf = kTcRows * 64 * 2;           // 16 KB: 128 rows x 64 channels, one swizzled box
+
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct TcParams {
+  const int* valid;
+  const void* o;                         // backward: forward output, contiguous [B, T, Hq, D]
+  const void* dout;
+  SwStride sdo;
+  void *out, *dq, *dk, *dv;              // contiguous
+  float* lse;                            // [B, Hq, T]
+  float* delta;
+  int B, T, Hq, Hk, window, sinks;
+  int qpair;                             // 1: the two tiles of a CTA are two query heads, 0: two consecutive query tiles
+  int items;                             // (sample, head or head pair) combinations
+  float scale;
+  int* error_flag;
+};
+
+__device__ __forceinline__ int tc_valid(const TcParams& p, int b) {
+  int n = p.valid ? p.valid[b] : p.T;
+  return n < 0 ? 0 : (n > p.T ? p.T : n);
+}
+
+// Key tiles that queries [q0, q0 + 128) of a sequence of n tokens see: the first `ns` tiles (sinks) and tiles [lo, hi].
+struct KeyRange {
+  int ns, lo, hi;
+  __device__ __forceinline__ KeyRange(int q0, int n, int window, int sinks) {
+    const int last = min(q0 + kTcRows, n) - 1;           // last query that is there
+    if (last < q0) { ns = 0; lo = 0; hi = -1; return; }
+    hi = last / kTcRows;
+    const int64_t first = (int64_t)q0 - window + 1;
+    lo = first <= 0 ? 0 : (int)(first / kTcRows);
+    ns = min((min(sinks, last + 1) + kTcRows - 1) / kTcRows, lo);
+  }
+  __device__ __forceinline__ bool has(int kt) const { return kt <= hi && (kt >= lo || kt < ns); }
+  __device__ __forceinline__ int count() const { return hi < lo ? 0 : ns + hi - lo + 1; }
+};
+
+// One [128 x D] tile: D / 64 boxes on one barrier.
+template <int D>
+__device__ __forceinline__ void tc_load_tile(uint8_t* dst, const CUtensorMap* map, int h, int t, int b, uint64_t* bar) {
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) tma_load_4d(dst + c * kTcHalf, map, c * 64, h, t, b, bar);
+}
+// Rows [from, 128) of a tile become zeros (a whole warp): what lies behind a sequence must not reach a sum, not even times 0.
+template <int D>
+__device__ __forceinline__ void tc_clear_rows(uint8_t* tile, int from) {
+  const int lane = threadIdx.x & 31;
+  for (int c = 0; c < D / 64; ++c)
+    for (uint32_t o = (uint32_t)from * 128u + lane * 16u; o < kTcHalf; o += 512u)
+      *reinterpret_cast<uint4*>(tile + c * kTcHalf + o) = make_uint4(0, 0, 0, 0);
+  fence_async_smem();
+  __syncwarp();
+}
+// S[128, 128] = A B^T over D channels, both tiles row by row in shared memory.
+template <int D>
+__device__ __forceinline__ void tc_scores(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc) {
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) {
+    const uint32_t o = (uint32_t)(k >> 2) * kTcHalf;
+    umma(tmem_d, make_desc(a + o) + 2 * (k & 3), make_desc(b + o) + 2 * (k & 3), idesc, k > 0 ? 1u : 0u);
+  }
+}
+// O[128, D] (+)= P[128, 128] V[128, D], P in TMEM (two values to a column), V row by row in shared memory.
+__device__ __forceinline__ void tc_accumulate(uint32_t tmem_d, uint32_t tmem_p, uint32_t v, uint32_t idesc, uint32_t carry) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    umma_ts(tmem_d, tmem_p + 8 * k, make_desc_mn(v + (uint32_t)k * 2048u, kTcHalf), idesc, k > 0 ? 1u : carry);
+}
+
+__device__ __forceinline__ void tc_finish(uint32_t tmem_base, uint32_t cols, int warp, int alloc_warp, volatile int* abort_flag, int* error_flag) {
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag && error_flag) {
+    *static_cast<volatile int*>(error_flag) = 1;         // host memory
+    __threadfence_system();
+  }
+  if (warp == alloc_warp) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(cols) : "memory");
+  }
+}
+__device__ __forceinline__ uint32_t tc_alloc(uint32_t* slot, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  return 0;
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+// Warps 0-3 and 4-7: the softmax of query tiles 0 and 1, one thread for each row; warp 8: MMA issue and TMEM; warp 9: TMA.
+// The two tiles take turns: while one's scores are in the hands of its row threads, the tensor cores work for the other.
+// TMEM columns: S0 | S1 (128 each; P over the first 64 of its S), O0 | O1 (D each).
+constexpr int kFwdThreads = 320;
+constexpr int kFwdStages = 2;
+template <int D> struct FwdSmem {
+  static constexpr uint32_t tile = (D / 64) * kTcHalf;
+  static constexpr uint32_t q = 0, k = 2 * tile, v = k + kFwdStages * tile, bars = v + kFwdStages * tile;
+  static constexpr uint32_t total = bars + 256 + 1024;
+};
+// P is kept 2^6 times its value, so that in fp16 a weight keeps its digits down to 2^-20 of the row's largest; the running
+// maximum may lag behind by 8 (2^14 in all, far from the type's largest) before the output is rescaled.
+constexpr float kPShift = 6.f, kMaxLag = 8.f;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                 const __grid_constant__ CUtensorMap map_v, const TcParams p, int bf16) {
+  typedef FwdSmem<D> L;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
+  uint64_t *q_full = bars, *k_full = bars + 2, *k_empty = bars + 4, *v_full = bars + 6, *v_empty = bars + 8, *s_full = bars + 10,
+           *p_full = bars + 12, *o_full = bars + 14, *patch = bars + 15, *drain = bars + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // the last tiles of causal attention are the longest: they start first
+  const int tiles = p.T / kTcRows + (p.T % kTcRows ? 1 : 0);
+  const int qblocks = p.qpair ? tiles : (tiles + 1) / 2;
+  const int qb = qblocks - 1 - (int)(blockIdx.x / p.items), item = blockIdx.x % p.items;
+  const int hcount = p.qpair ? p.Hq / 2 : p.Hq;
+  const int b = item / hcount, h0 = (item % hcount) * (p.qpair ? 2 : 1), hk = h0 / (p.Hq / p.Hk);
+  const int n = tc_valid(p, b);
+  const int qa = p.qpair ? qb * kTcRows : qb * 2 * kTcRows;
+  const int qstep = p.qpair ? 0 : kTcRows, hstep = p.qpair ? 1 : 0;
+  const KeyRange r0(qa, n, p.window, p.sinks), r1(qa + qstep, n, p.window, p.sinks);
+  // the union of both: sinks, then [lo of the first, hi of the second]
+  const int hi = max(r0.hi, r1.hi), lo = r0.lo, ns = max(r0.ns, min(r1.ns, lo));
+  const int ntiles = hi < lo ? 0 : ns + hi - lo + 1;
+  auto key_tile = [&](int j) { return j < ns ? j : lo + (j - ns); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 1); mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1);
+      mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4);
+    }
+    mbar_init(o_full, 1); mbar_init(patch, 1); mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) tc_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 9) {
+    // ---------------------------------------------------------------- loads
+    if (ntiles > 0) {
+      if (lane == 0) {
+        for (int s = 0; s < 2; ++s) {
+          if ((s ? r1 : r0).count() == 0) continue;
+          mbar_expect_tx(&q_full[s], L::tile);
+          tc_load_tile<D>(smem + L::q + s * L::tile, &map_q, h0 + s * hstep, qa + s * qstep, b, &q_full[s]);
+        }
+      }
+      bool ok = true;
+      int nk = 0, nv = 0;                                         // tiles asked for
+      for (int j = 0; j < ntiles; ++j) {
+        const int st = j % kFwdStages, kt = key_tile(j);
+        const uint32_t ph = (uint32_t)(j / kFwdStages + 1) & 1u;
+        if (j >= kFwdStages && !(ok = mbar_wait_warp(&k_empty[st], ph))) break;
+        if (lane == 0) {
+          mbar_expect_tx(&k_full[st], L::tile);
+          tc_load_tile<D>(smem + L::k + st * L::tile, &map_k, hk, kt * kTcRows, b, &k_full[st]);
+        }
+        nk = j + 1;
+        if (j >= kFwdStages && !(ok = mbar_wait_warp(&v_empty[st], ph))) break;
+        const bool ends = (kt + 1) * kTcRows > n && n < p.T;      // the sequence ends inside this tile
+        uint8_t* tile = smem + L::v + st * L::tile;
+        if (lane == 0) {
+          uint64_t* bar = ends ? patch : &v_full[st];
+          mbar_expect_tx(bar, L::tile);
+          tc_load_tile<D>(tile, &map_v, hk, kt * kTcRows, b, bar);
+        }
+        nv = ends ? j : j + 1;
+        if (ends) {                                               // the last tile of the sequence: at most once
+          if (!(ok = mbar_wait_warp(patch, 0))) break;
+          tc_clear_rows<D>(tile, n - kt * kTcRows);
+          if (lane == 0) mbar_arrive(&v_full[st]);
+        }
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        if (lane == 0) {
+          // no copy may still be under way when the CTA's shared memory is given back
+          for (int s = 0; s < 2; ++s) {
+            if ((s ? r1 : r0).count()) mbar_wait(&q_full[s], 0);
+            if (nk > s) mbar_wait(&k_full[s], (uint32_t)((nk - 1 - s) / kFwdStages) & 1u);
+            if (nv > s) mbar_wait(&v_full[s], (uint32_t)((nv - 1 - s) / kFwdStages) & 1u);
+          }
+        }
+      }
+    }
+  } else if (warp == 8) {
+    // ---------------------------------------------------------------- products
+    if (lane == 0 && ntiles > 0) {
+      const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
+      const uint32_t sq = smem_u32(smem + L::q), sk = smem_u32(smem + L::k), sv = smem_u32(smem + L::v);
+      bool ok = true;
+      uint32_t pphase[2] = {0, 0}, started[2] = {0, 0};
+      for (int s = 0; s < 2 && ok; ++s) {
+        const KeyRange& r = s ? r1 : r0;
+        if (r.count() == 0) continue;
+        ok = mbar_wait(&q_full[s], 0);
+        if (ok && r.has(key_tile(0))) {
+          ok = mbar_wait(&k_full[0], 0);
+          tc_fence_after();
+          if (ok) { tc_scores<D>(tmem + 128 * s, sq + s * L::tile, sk, id_s); umma_commit(&s_full[s]); }
+        }
+      }
+      umma_commit(&k_empty[0]);
+      for (int j = 0; j < ntiles && ok; ++j) {
+        const int kt = key_tile(j), next = j + 1 < ntiles ? key_tile(j + 1) : -1;
+        const int st = j % kFwdStages, sn = (j + 1) % kFwdStages;
+        const uint32_t ph = (uint32_t)(j / kFwdStages) & 1u, pn = (uint32_t)((j + 1) / kFwdStages) & 1u;
+        for (int s = 0; s < 2 && ok; ++s) {
+          const KeyRange& r = s ? r1 : r0;
+          if (r.has(kt)) {
+            ok = mbar_wait(&v_full[st], ph) && mbar_wait(&p_full[s], pphase[s]);
+            if (!ok) break;
+            pphase[s] ^= 1u;
+            tc_fence_after();
+            tc_accumulate(tmem + 256 + D * s, tmem + 128 * s, sv + st * L::tile, id_o, started[s]);
+            started[s] = 1u;
+          }
+          if (next >= 0 && r.has(next)) {
+            ok = mbar_wait(&k_full[sn], pn);
+            if (!ok) break;
+            tc_fence_after();
+            tc_scores<D>(tmem + 128 * s, sq + s * L::tile, sk + sn * L::tile, id_s);
+            umma_commit(&s_full[s]);                              // complete only after P V of this tile, issued before it
+          }
+        }
+        if (ok) {
+          umma_commit(&v_empty[st]);
+          if (next >= 0) umma_commit(&k_empty[sn]);
+        }
+      }
+      if (ok) umma_commit(o_full);
+      else { *abort_flag = 1; umma_commit(drain); mbar_wait(drain, 0); }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const int s = warp >> 2, quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const int q0 = qa + s * qstep, i = q0 + row, h = h0 + s * hstep;
+    const KeyRange r = s ? r1 : r0;
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const uint32_t ts = tmem + 128 * s + lane_off, to = tmem + 256 + D * s + lane_off;
+    const float sc = p.scale * kSwLog2e;
+    float m = -INFINITY, l = 0.f;
+    uint32_t phase = 0;
+    bool ok = true, first = true;
+    for (int j = 0; j < ntiles; ++j) {
+      const int kt = key_tile(j);
+      if (!r.has(kt)) continue;
+      ok = mbar_wait_warp(&s_full[s], phase);
+      if (!ok) break;
+      phase ^= 1u;
+      tc_fence_after();
+      uint32_t x[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, x + 32 * c);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_wait_ld32(x + 32 * c);
+      const int k0 = kt * kTcRows;
+      const bool whole = k0 + kTcRows - 1 <= q0 && (q0 + kTcRows - 1 - k0 < p.window || k0 + kTcRows <= p.sinks);
+      if (!whole) {
+        const int c_hi = i - k0, c_sink = p.sinks - k0;
+        const int c_lo = i - k0 >= p.window ? i - k0 - p.window + 1 : 0;
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          if (c > c_hi || (c < c_lo && c >= c_sink)) x[c] = 0xff800000u;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(x[c]));
+      const float mt = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc);
+      const bool move = mt > m + kMaxLag || m == -INFINITY;
+      if (__any_sync(0xffffffffu, move)) {
+        const float to_m = move ? mt : m;
+        const float alpha = move ? (to_m == -INFINITY ? 0.f : ex2(m - to_m)) : 1.f;
+        m = to_m;
+        l *= alpha;
+        if (!first) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(to + c, o);
+            tmem_wait_ld32(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(to + c, o);
+          }
+        }
+      }
+      first = false;
+      const float off = kPShift - (m == -INFINITY ? 0.f : m);
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += 32) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          const float e0 = ex2(fmaf(__uint_as_float(x[c0 + c]), sc, off));
+          const float e1 = ex2(fmaf(__uint_as_float(x[c0 + c + 1]), sc, off));
+          part[c & 2] += e0;
+          part[(c & 2) + 1] += e1;
+          pk[c >> 1] = pack2<T>(e0, e1);
+        }
+        tmem_st16(ts + (c0 >> 1), pk);
+      }
+      l += (part[0] + part[1]) + (part[2] + part[3]);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[s]);
+    }
+    if (ok && ntiles > 0) ok = mbar_wait_warp(o_full, 0);
+    if (!ok) *abort_flag = 1;
+    tc_fence_after();
+    if (ok) {
+      const bool live = i < n && r.count() > 0;
+      const float inv = live ? (l > 0.f || l != l ? 1.f / l : 0.f) : 0.f;
+      T* orow = static_cast<T*>(p.out) + (((int64_t)b * p.T + i) * p.Hq + h) * D;
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t o[32];
+        if (r.count() > 0) { tmem_ld32(to + c0, o); tmem_wait_ld32(o); }
+        if (i < p.T) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (live) {
+              w.x = pack2<T>(__uint_as_float(o[v * 8]) * inv, __uint_as_float(o[v * 8 + 1]) * inv);
+              w.y = pack2<T>(__uint_as_float(o[v * 8 + 2]) * inv, __uint_as_float(o[v * 8 + 3]) * inv);
+              w.z = pack2<T>(__uint_as_float(o[v * 8 + 4]) * inv, __uint_as_float(o[v * 8 + 5]) * inv);
+              w.w = pack2<T>(__uint_as_float(o[v * 8 + 6]) * inv, __uint_as_float(o[v * 8 + 7]) * inv);
+            }
+            *reinterpret_cast<uint4*>(orow + c0 + v * 8) = w;
+          }
+        }
+      }
+      if (i < p.T && p.lse) p.lse[((int64_t)b * p.Hq + h) * p.T + i] = live && (l > 0.f || l != l) ? m + log2f(l) - kPShift : INFINITY;
+    }
+  }
+  tc_finish(tmem, 512, warp, 8, abort_flag, p.error_flag);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+// 4-D tensor map over [B, T, H, D] with element strides; box = 64 channels x 1 head x 128 positions.
+static int tc_map(CUtensorMap* map, const void* base, int bf16, int B, int T, int H, int D, SwStride s) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return -10;
+  auto bytes = [&](int64_t stride, int size) { return size == 1 ? (cuuint64_t)D * 2 : (cuuint64_t)stride * 2; };   // an axis of one entry is never walked
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T, (cuuint64_t)B};
+  cuuint64_t strides[3] = {bytes(s.h, H), bytes(s.t, T), bytes(s.b, B)};
+  cuuint32_t box[4] = {64, 1, (cuuint32_t)kTcRows, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult rc = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
+                         dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? 0 : -(1000 + (int)rc);
+}
+
+// TMA reads from 16-byte boundaries with strides of whole 16 bytes (below 2^40 bytes).
+static bool tc_layout_ok(const void* base, const SwStride& s, int B, int T, int H) {
+  auto ok = [](int64_t st, int size) { return size == 1 || (st > 0 && st % 8 == 0 && st < (1ll << 38)); };
+  return (uintptr_t)base % 16 == 0 && ok(s.b, B) && ok(s.t, T) && ok(s.h, H);
+}
+
+// The tensor cores take half types, head sizes 64 and 128 and a positive scale (the running maximum is taken of the unscaled
+// scores).  What they do not take runs on the general kernels.
+static bool tc_takes(const SwParams& p, int dtype) {
+  return (dtype == kF16 || dtype == kBF16) && (p.D == 64 || p.D == 128) && p.scale > 0.f && p.scale < 1e30f &&
+         tc_layout_ok(p.q, p.sq, p.B, p.T, p.Hq) && tc_layout_ok(p.k, p.sk, p.B, p.T, p.Hk) && tc_layout_ok(p.v, p.sv, p.B, p.T, p.Hk);
+}
+
+static TcParams tc_params(const SwParams& p, int* error_flag) {
+  TcParams t{};
+  t.valid = p.valid; t.o = p.o; t.dout = p.dout; t.sdo = p.sdo; t.out = p.out; t.dq = p.dq; t.dk = p.dk; t.dv = p.dv;
+  t.lse = p.lse; t.delta = p.delta;
+  t.B = p.B; t.T = p.T; t.Hq = p.Hq; t.Hk = p.Hk; t.window = p.window; t.sinks = p.sinks; t.scale = p.scale; t.error_flag = error_flag;
+  return t;
+}
+
+template <typename T, int D>
+static int tc_forward(const SwParams& p, int bf16, int* error_flag, cudaStream_t st) {
+  CUtensorMap mq, mk, mv;
+  int rc = tc_map(&mq, p.q, bf16, p.B, p.T, p.Hq, D, p.sq);
+  if (!rc) rc = tc_map(&mk, p.k, bf16, p.B, p.T, p.Hk, D, p.sk);
+  if (!rc) rc = tc_map(&mv, p.v, bf16, p.B, p.T, p.Hk, D, p.sv);
+  if (rc) return rc;
+  TcParams t = tc_params(p, error_flag);
+  t.qpair = (p.Hq / p.Hk) % 2 == 0;      // two heads over the same keys and the same rows, where heads come in pairs
+  t.items = p.B * (t.qpair ? p.Hq / 2 : p.Hq);
+  const int64_t tiles = (p.T + kTcRows - 1) / kTcRows;
+  const int64_t grid = (t.qpair ? tiles : (tiles + 1) / 2) * t.items;
+  if (grid > 0x7fffffff) return -2;
+  static unsigned long long seen = 0;
+  if (first_on_device(&seen)) cudaFuncSetAttribute(sw_fwd_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdSmem<D>::total);
+  sw_fwd_tc_kernel<T, D><<<(unsigned)grid, kFwdThreads, FwdSmem<D>::total, st>>>(mq, mk, mv, t, bf16);
+  return (int)cudaGetLastError();
+}
