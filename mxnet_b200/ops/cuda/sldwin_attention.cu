@@ -235,7 +235,18 @@ static bool sw_shape_ok(const SwParams& p) {
          p.window <= p.T && p.sinks >= 0 && p.sinks <= p.T && p.T <= (1 << 30) && (int64_t)p.B * p.Hq <= 0x7fffffff;
 }
 
+static SwParams sw_params(const int* dims, const int64_t* strides, float scale) {
+  SwParams p{};
+  p.B = dims[0]; p.T = dims[1]; p.Hq = dims[2]; p.Hk = dims[3]; p.D = dims[4]; p.window = dims[5]; p.sinks = dims[6];
+  p.sq = {strides[0], strides[1], strides[2]};
+  p.sk = {strides[3], strides[4], strides[5]};
+  p.sv = {strides[6], strides[7], strides[8]};
+  p.scale = scale;
+  return p;
+}
+
 #include "sldwin_tc.inl"
+#include "sldwin_tc_bwd.inl"
 
 }  // namespace mxb
 
@@ -247,13 +258,8 @@ MXB_EXPORT int mxb_sldwin_max_dim(void) { return kSwMaxD; }
 // channels are adjacent.  lse: [B, Hq, T] floats (forward: may be null when no backward pass follows).
 MXB_EXPORT int mxb_sldwin_forward(int dtype, const void* q, const void* k, const void* v, const int* valid, void* out, float* lse,
                                   const int* dims, const int64_t* strides, float scale, int* error_flag, void* stream) {
-  SwParams p{};
+  SwParams p = sw_params(dims, strides, scale);
   p.q = q; p.k = k; p.v = v; p.valid = valid; p.out = out; p.lse = lse;
-  p.B = dims[0]; p.T = dims[1]; p.Hq = dims[2]; p.Hk = dims[3]; p.D = dims[4]; p.window = dims[5]; p.sinks = dims[6];
-  p.sq = {strides[0], strides[1], strides[2]};
-  p.sk = {strides[3], strides[4], strides[5]};
-  p.sv = {strides[6], strides[7], strides[8]};
-  p.scale = scale;
   if (!sw_shape_ok(p)) return -2;
   cudaStream_t st = (cudaStream_t)stream;
   if (tc_takes(p, dtype)) {
@@ -266,23 +272,31 @@ MXB_EXPORT int mxb_sldwin_forward(int dtype, const void* q, const void* k, const
   return -1;
 }
 
-// dq: [B, T, Hq, D], dk and dv: [B, T, Hk, D], contiguous; delta: [B, Hq, T] floats of workspace.
+// dq: [B, T, Hq, D], dk and dv: [B, T, Hk, D], contiguous; delta: [B, Hq, T + ceil(T / 128)] floats of workspace; parts:
+// mxb_sldwin_backward_parts floats of workspace (may be null when that is 0).
 MXB_EXPORT int mxb_sldwin_backward(int dtype, const void* q, const void* k, const void* v, const int* valid, const void* o,
-                                   const void* dout, const float* lse, float* delta, void* dq, void* dk, void* dv, const int* dims,
-                                   const int64_t* strides, float scale, int* error_flag, void* stream) {
-  SwParams p{};
+                                   const void* dout, const float* lse, float* delta, float* parts, void* dq, void* dk, void* dv,
+                                   const int* dims, const int64_t* strides, float scale, int* error_flag, void* stream) {
+  SwParams p = sw_params(dims, strides, scale);
   p.q = q; p.k = k; p.v = v; p.valid = valid; p.o = o; p.dout = dout; p.lse = const_cast<float*>(lse); p.delta = delta;
   p.dq = dq; p.dk = dk; p.dv = dv;
-  p.B = dims[0]; p.T = dims[1]; p.Hq = dims[2]; p.Hk = dims[3]; p.D = dims[4]; p.window = dims[5]; p.sinks = dims[6];
-  p.sq = {strides[0], strides[1], strides[2]};
-  p.sk = {strides[3], strides[4], strides[5]};
-  p.sv = {strides[6], strides[7], strides[8]};
   p.sdo = {strides[9], strides[10], strides[11]};
-  p.scale = scale;
   if (!sw_shape_ok(p)) return -2;
   cudaStream_t st = (cudaStream_t)stream;
+  if (tc_takes(p, dtype) && tc_layout_ok(dout, p.sdo, p.B, p.T, p.Hq)) {
+    if (dtype == kF16) return p.D == 64 ? tc_backward<__half, 64>(p, parts, 0, error_flag, st) : tc_backward<__half, 128>(p, parts, 0, error_flag, st);
+    return p.D == 64 ? tc_backward<__nv_bfloat16, 64>(p, parts, 1, error_flag, st) : tc_backward<__nv_bfloat16, 128>(p, parts, 1, error_flag, st);
+  }
   if (dtype == kF32) return sw_general<float>(p, 1, st);
   if (dtype == kF16) return sw_general<__half>(p, 1, st);
   if (dtype == kBF16) return sw_general<__nv_bfloat16>(p, 1, st);
   return -1;
+}
+
+// Floats of workspace for sums that come in parts (0 for shapes that only the general kernels take).
+MXB_EXPORT int64_t mxb_sldwin_backward_parts(int dtype, const int* dims) {
+  const int64_t none[12] = {0};
+  const SwParams p = sw_params(dims, none, 1.f);
+  if (!sw_shape_ok(p) || (p.D != 64 && p.D != 128) || (dtype != kF16 && dtype != kBF16)) return 0;
+  return dkv_part_floats(p);
 }

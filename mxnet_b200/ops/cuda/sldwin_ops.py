@@ -73,14 +73,16 @@ class _SldwinAttention(torch.autograd.Function):
         dq = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
         dk = torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device)
         dv = torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device)
-        delta = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device)
+        delta = torch.empty(B * Hq * (T + (T + 127) // 128), dtype=torch.float32, device=q.device)
         dims = _DIMS7(B, T, Hq, Hk, D, window, sinks)
         strides = _S12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *dout.stride()[:3])
+        words = lib().mxb_sldwin_backward_parts(dt(q), dims)      # key gradients that several blocks sum up
+        parts = torch.empty(words, dtype=torch.float32, device=q.device) if words else None
         with on_device(q):
-            check(lib().mxb_sldwin_backward(dt(q), ptr(q), ptr(k), ptr(v), ptr(valid), ptr(out), ptr(dout), ptr(lse), ptr(delta), ptr(dq),
-                                            ptr(dk), ptr(dv), dims, strides, scale, _error_word(), stream_ptr(q.device)),
+            check(lib().mxb_sldwin_backward(dt(q), ptr(q), ptr(k), ptr(v), ptr(valid), ptr(out), ptr(dout), ptr(lse), ptr(delta), ptr(parts),
+                                            ptr(dq), ptr(dk), ptr(dv), dims, strides, scale, _error_word(), stream_ptr(q.device)),
                   'sldwin_attention backward')
-        count_launch(2)
+        count_launch(3 if words else 2)
         return dq, dk, dv, None, None, None, None
 
 

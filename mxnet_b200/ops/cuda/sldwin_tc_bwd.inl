@@ -1,0 +1,660 @@
+// Backward pass of the tensor-core sliding-window attention (included by sldwin_attention.cu inside namespace mxb).
+//
+// Two kernels, each the owner of what it accumulates, so that no result depends on the order of anything: dQ by query tiles
+// (S, dP and dS K: three products per pair of tiles) and dK, dV by key tiles (S^T, dP^T, P^T dO, dS^T Q: four).  The scores
+// are formed twice; sharing them would need sums of dQ across CTAs in memory.  In both, two warpgroups share each tile of
+// scores (64 columns each), so that their exponentials take less time than the products and the tensor cores set the pace.
+
+//
+// Range in fp16: probabilities enter the dV product 2^14 times their value (at most 2^14, digits kept down to 2^-28), and dS is
+// formed from dO scaled by the power of two that brings the largest dO of the CTA's tiles into [8, 16): neither small
+// gradients nor a loss scale push it out of the type's range.  Both factors leave with the fp32 sums.  bf16 needs neither.
+template <typename T> struct BwdRange { static constexpr bool scaled = false; static constexpr float shift = 0.f, unshift = 1.f; };
+template <> struct BwdRange<__half> { static constexpr bool scaled = true; static constexpr float shift = 14.f, unshift = 1.f / 16384.f; };
+__device__ __forceinline__ float bwd_factor(float amax) {          // 2^(3 - e) for amax in [2^e, 2^(e + 1))
+  const int e = (int)((__float_as_uint(amax) >> 23) & 255u) - 127;
+  return e < -30 || e > 16 ? 1.f : __uint_as_float((uint32_t)(127 + 3 - e) << 23);
+}
+
+// ------------------------------------------------------------------------------------------------ dQ
+// Warps 0-3: columns 0..63 of the scores, warps 4-7: columns 64..127; warp 8: MMA and TMEM; warp 9: TMA.
+// TMEM columns: S of even tiles | S of odd tiles | dP (128 each) | dQ (D).  dS lies over the S it comes from: each half of the
+// columns over its own part.
+template <int D> struct DqSmem {
+  static constexpr uint32_t tile = (D / 64) * kTcHalf;
+  static constexpr int kst = 3, vst = 2;
+  static constexpr uint32_t q = 0, g = tile, k = 2 * tile, v = k + kst * tile, delta = v + vst * tile, bars = delta + 1088;
+  static constexpr uint32_t total = bars + 192 + 1024;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g, const TcParams p, int bf16) {
+  typedef DqSmem<D> L;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  float* s_delta = reinterpret_cast<float*>(smem + L::delta);      // [2][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
+  uint64_t *qg_full = bars, *k_full = bars + 1, *k_empty = bars + 4, *v_full = bars + 7, *v_empty = bars + 9, *sd_full = bars + 11,
+           *dp_empty = bars + 12, *ds_full = bars + 13, *done = bars + 14, *patch = bars + 15, *drain = bars + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const int tiles = p.T / kTcRows + (p.T % kTcRows ? 1 : 0);
+  const int qt = tiles - 1 - (int)(blockIdx.x / p.items), item = blockIdx.x % p.items;
+  const int b = item / p.Hq, h = item % p.Hq, hk = h / (p.Hq / p.Hk);
+  const int n = tc_valid(p, b);
+  const int q0 = qt * kTcRows;
+  const KeyRange r(q0, n, p.window, p.sinks);
+  const int ntiles = r.count();
+  auto key_tile = [&](int j) { return j < r.ns ? j : r.lo + (j - r.ns); };
+
+  if (threadIdx.x == 0) {
+    mbar_init(qg_full, 1);
+    for (int s = 0; s < L::kst; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
+    for (int s = 0; s < L::vst; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+    mbar_init(sd_full, 1); mbar_init(dp_empty, 8); mbar_init(ds_full, 8); mbar_init(done, 1); mbar_init(patch, 1); mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) tc_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t kDp = 256, kDq = 384;
+
+  if (warp == 9) {
+    if (ntiles > 0) {
+      if (lane == 0) {
+        mbar_expect_tx(qg_full, 2 * L::tile);
+        tc_load_tile<D>(smem + L::q, &map_q, h, q0, b, qg_full);
+        tc_load_tile<D>(smem + L::g, &map_g, h, q0, b, qg_full);
+      }
+      bool ok = true;
+      int nk = 0, nv = 0;
+      for (int j = 0; j < ntiles; ++j) {
+        const int sk = j % L::kst, sv = j % L::vst, kt = key_tile(j);
+        if (j >= L::kst && !(ok = mbar_wait_warp(&k_empty[sk], (uint32_t)(j / L::kst + 1) & 1u))) break;
+        const bool ends = (kt + 1) * kTcRows > n && n < p.T;      // the sequence ends inside this tile: dS K must not meet what follows
+        uint8_t* tile = smem + L::k + sk * L::tile;
+        if (lane == 0) {
+          uint64_t* bar = ends ? patch : &k_full[sk];
+          mbar_expect_tx(bar, L::tile);
+          tc_load_tile<D>(tile, &map_k, hk, kt * kTcRows, b, bar);
+        }
+        nk = ends ? j : j + 1;
+        if (ends) {
+          if (!(ok = mbar_wait_warp(patch, 0))) break;
+          tc_clear_rows<D>(tile, n - kt * kTcRows);
+          if (lane == 0) mbar_arrive(&k_full[sk]);
+        }
+        if (j >= L::vst && !(ok = mbar_wait_warp(&v_empty[sv], (uint32_t)(j / L::vst + 1) & 1u))) break;
+        if (lane == 0) {
+          mbar_expect_tx(&v_full[sv], L::tile);
+          tc_load_tile<D>(smem + L::v + sv * L::tile, &map_v, hk, kt * kTcRows, b, &v_full[sv]);
+        }
+        nv = j + 1;
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        if (lane == 0) {                                          // no copy may still be under way at the end
+          mbar_wait(qg_full, 0);
+          for (int s = 0; s < L::kst; ++s) if (nk > s) mbar_wait(&k_full[s], (uint32_t)((nk - 1 - s) / L::kst) & 1u);
+          for (int s = 0; s < L::vst; ++s) if (nv > s) mbar_wait(&v_full[s], (uint32_t)((nv - 1 - s) / L::vst) & 1u);
+        }
+      }
+    }
+  } else if (warp == 8) {
+    if (lane == 0 && ntiles > 0) {
+      const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
+      const uint32_t sq = smem_u32(smem + L::q), sg = smem_u32(smem + L::g), sk = smem_u32(smem + L::k), sv = smem_u32(smem + L::v);
+      bool ok = mbar_wait(qg_full, 0);
+      auto scores = [&](int j) {
+        ok = mbar_wait(&k_full[j % L::kst], (uint32_t)(j / L::kst) & 1u);
+        tc_fence_after();
+        if (ok) tc_scores<D>(tmem + 128 * (j & 1), sq, sk + (j % L::kst) * L::tile, id_s);
+      };
+      auto dprobs = [&](int j) {
+        ok = mbar_wait(&v_full[j % L::vst], (uint32_t)(j / L::vst) & 1u);
+        tc_fence_after();
+        if (ok) { tc_scores<D>(tmem + kDp, sg, sv + (j % L::vst) * L::tile, id_s); umma_commit(sd_full); umma_commit(&v_empty[j % L::vst]); }
+      };
+      if (ok) scores(0);
+      if (ok) dprobs(0);
+      if (ok && ntiles > 1) scores(1);
+      for (int j = 0; j < ntiles && ok; ++j) {
+        if (j + 1 < ntiles) {
+          ok = mbar_wait(dp_empty, (uint32_t)j & 1u);             // dP of this tile is in registers
+          if (ok) dprobs(j + 1);
+          if (!ok) break;
+        }
+        ok = mbar_wait(ds_full, (uint32_t)j & 1u);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t ds = tmem + 128 * (j & 1), kt = sk + (j % L::kst) * L::tile;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          umma_ts(tmem + kDq, ds + (k < 4 ? 8 * k : 64 + 8 * (k - 4)), make_desc_mn(kt + (uint32_t)k * 2048u, kTcHalf), id_o, (j > 0 || k > 0) ? 1u : 0u);
+        umma_commit(&k_empty[j % L::kst]);
+        if (j + 2 < ntiles) scores(j + 2);                        // over S and dS of this tile, read by the product before it
+      }
+      if (ok) umma_commit(done);
+      else { *abort_flag = 1; umma_commit(drain); mbar_wait(drain, 0); }
+    }
+  } else {
+    const int half = warp >> 2, quad = warp & 3;
+    const int row = quad * 32 + lane, i = q0 + row;
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const bool live = i < n;
+    // delta = rowsum(dO * O), half of the channels in each warpgroup, while the first products run
+    float part = 0.f, lse = INFINITY, big = 0.f;
+    if (live) {
+      const T* orow = static_cast<const T*>(p.o) + (((int64_t)b * p.T + i) * p.Hq + h) * D + half * (D / 2);
+      const T* grow = static_cast<const T*>(p.dout) + b * p.sdo.b + i * p.sdo.t + h * p.sdo.h + half * (D / 2);
+#pragma unroll
+      for (int v = 0; v < D / 16; ++v) {
+        const Vec16<T> a = ld16(orow + v * 8), g = ld16(grow + v * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float ge = Cvt<T>::to_f(g.v[e]);
+          part += Cvt<T>::to_f(a.v[e]) * ge;
+          if (BwdRange<T>::scaled) big = fmaxf(big, fabsf(ge));
+        }
+      }
+      lse = p.lse[((int64_t)b * p.Hq + h) * p.T + i];
+    }
+    s_delta[half * 128 + row] = part;
+    if (BwdRange<T>::scaled) {
+      big = warp_max(big);
+      if (lane == 0) s_delta[256 + warp] = big;
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    // Rows whose keys are all in one tile get delta from the sum of P dP instead of from the rounded output: with few keys the
+    // output's rounding is not small beside dP - delta.
+    const bool one_tile = ntiles == 1;
+    float delta = one_tile ? 0.f : s_delta[row] + s_delta[128 + row];
+    float f = 1.f;
+    if (BwdRange<T>::scaled) {
+#pragma unroll
+      for (int w = 0; w < 8; ++w) big = fmaxf(big, s_delta[256 + w]);
+      if (threadIdx.x == 0) p.gmax[((int64_t)b * p.Hq + h) * tiles + qt] = big;
+      f = bwd_factor(big);
+    }
+    if (half == 0 && i < p.T && !one_tile) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = delta;
+    delta *= f;
+    const float out_scale = p.scale / f;
+    const float sc = p.scale * kSwLog2e;
+    bool ok = true;
+    for (int j = 0; j < ntiles; ++j) {
+      const int kt = key_tile(j);
+      ok = mbar_wait_warp(sd_full, (uint32_t)j & 1u);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t ts = tmem + 128 * (j & 1) + 64 * half + lane_off, td = tmem + kDp + 64 * half + lane_off;
+      uint32_t x[64], y[64];
+      tmem_ld32(ts, x);
+      tmem_ld32(ts + 32, x + 32);
+      tmem_ld32(td, y);
+      tmem_ld32(td + 32, y + 32);
+      tmem_wait_ld32(x);
+      tmem_wait_ld32(x + 32);
+      tmem_wait_ld32(y);
+      tmem_wait_ld32(y + 32);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dp_empty);
+      const int k0 = kt * kTcRows;
+      const bool whole = k0 + kTcRows - 1 <= q0 && (q0 + kTcRows - 1 - k0 < p.window || k0 + kTcRows <= p.sinks);
+      if (one_tile) {
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (k0 + 64 * half + c <= i && (i - (k0 + 64 * half + c) < p.window || k0 + 64 * half + c < p.sinks))
+            sum += ex2(fmaf(__uint_as_float(x[c]), sc, -lse)) * __uint_as_float(y[c]);
+        s_delta[half * 128 + row] = sum;                          // nobody reads the first sums in this case
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        sum = s_delta[row] + s_delta[128 + row];
+        if (half == 0 && i < p.T) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = live ? sum : 0.f;
+        delta = sum * f;
+      }
+#pragma unroll
+      for (int c = 0; c < 64; ++c) {
+        const float pr = ex2(fmaf(__uint_as_float(x[c]), sc, -lse));
+        x[c] = __float_as_uint(pr * (BwdRange<T>::scaled ? fmaf(__uint_as_float(y[c]), f, -delta) : __uint_as_float(y[c]) - delta));
+      }
+      if (!whole) {
+        const int base = k0 + 64 * half;
+        const int c_hi = i - base, c_sink = p.sinks - base;
+        const int c_lo = i - k0 >= p.window ? i - base - p.window + 1 : -64;
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c > c_hi || (c < c_lo && c >= c_sink)) x[c] = 0u;
+      }
+      uint32_t pk[32];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) pk[c] = pack2<T>(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1]));
+      tmem_st32(ts, pk);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_full);
+    }
+    if (ok && ntiles > 0) ok = mbar_wait_warp(done, 0);
+    if (!ok) *abort_flag = 1;
+    tc_fence_after();
+    if (ok) {
+      T* dst = static_cast<T*>(p.dq) + (((int64_t)b * p.T + i) * p.Hq + h) * D + half * (D / 2);
+#pragma unroll 1
+      for (int c0 = 0; c0 < D / 2; c0 += 32) {
+        uint32_t o[32];
+        if (ntiles > 0) { tmem_ld32(tmem + kDq + half * (D / 2) + c0 + lane_off, o); tmem_wait_ld32(o); }
+        if (i < p.T) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (live) {
+              w.x = pack2<T>(__uint_as_float(o[v * 8]) * out_scale, __uint_as_float(o[v * 8 + 1]) * out_scale);
+              w.y = pack2<T>(__uint_as_float(o[v * 8 + 2]) * out_scale, __uint_as_float(o[v * 8 + 3]) * out_scale);
+              w.z = pack2<T>(__uint_as_float(o[v * 8 + 4]) * out_scale, __uint_as_float(o[v * 8 + 5]) * out_scale);
+              w.w = pack2<T>(__uint_as_float(o[v * 8 + 6]) * out_scale, __uint_as_float(o[v * 8 + 7]) * out_scale);
+            }
+            *reinterpret_cast<uint4*>(dst + c0 + v * 8) = w;
+          }
+        }
+      }
+    }
+  }
+  tc_finish(tmem, 512, warp, 8, abort_flag, p.error_flag);
+}
+
+// ------------------------------------------------------------------------------------------------ dK, dV
+// A CTA owns 128 keys of one key head and walks (query head, query tile): the heads of its part of the group, the tiles whose
+// windows reach its keys.  A key tile that holds sinks is seen by all later queries as well: those far tiles go to CTAs of
+// their own in chunks as long as a window, and where keys are few the heads of a group are split over CTAs; such parts are
+// written in fp32 and added in a fixed order by a last small kernel.
+// TMEM columns: S^T | dP^T (128 each) | dV | dK (D each); P^T over S^T, dS^T over dP^T, each half of the columns over its own part.
+struct DkvSplit {
+  int tiles, near_span;                  // query tiles kt .. kt + near_span reach a key tile by their windows
+  int sink_tiles, far_chunks;            // far CTAs: sink_tiles x far_chunks of near_span + 1 query tiles
+  int hsplit;                            // parts of a head group
+  int part_tiles;                        // key tiles whose sums come in parts: the first part_tiles
+  int items;                             // B * Hk * hsplit
+  float* parts;                          // near: [hsplit][B * Hk][part_tiles], far: [hsplit][far_chunks][B * Hk][sink_tiles], each 2 x 128 x D
+};
+__device__ __forceinline__ float* dkv_near_part(const DkvSplit& s, int64_t bh_all, int hs, int bh, int kt, int D) {
+  return s.parts + ((((int64_t)hs * bh_all + bh) * s.part_tiles + kt) * 2) * kTcRows * D;
+}
+__device__ __forceinline__ float* dkv_far_part(const DkvSplit& s, int64_t bh_all, int hs, int chunk, int bh, int kt, int D) {
+  const int64_t near = (int64_t)s.hsplit * bh_all * s.part_tiles;
+  return s.parts + ((near + (((int64_t)hs * s.far_chunks + chunk) * bh_all + bh) * s.sink_tiles + kt) * 2) * kTcRows * D;
+}
+
+template <int D> struct DkvSmem {
+  static constexpr uint32_t tile = (D / 64) * kTcHalf;
+  static constexpr int qst = 3, gst = 2;
+  static constexpr uint32_t k = 0, v = tile, q = 2 * tile, g = q + qst * tile, stat = g + gst * tile, bars = stat + 2048;
+  static constexpr uint32_t total = bars + 256;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g, const TcParams p,
+                 const DkvSplit sp, int bf16) {
+  typedef DkvSmem<D> L;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  float* s_stat = reinterpret_cast<float*>(smem + L::stat);        // [2 stages][lse 128 | delta 128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
+  uint64_t *kv_full = bars, *q_full = bars + 1, *q_empty = bars + 4, *g_full = bars + 7, *g_empty = bars + 9, *st_full = bars + 11,
+           *st_empty = bars + 13, *s_full = bars + 15, *dp_full = bars + 16, *p_ready = bars + 17, *ds_ready = bars + 18, *done = bars + 19,
+           *patch = bars + 20, *drain = bars + 21;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* s_factor = reinterpret_cast<float*>(tmem_slot + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (smem_u32(smem) & 1023u) {                                    // swizzled tiles lie on 1024-byte boundaries
+    if (threadIdx.x == 0 && p.error_flag) *static_cast<volatile int*>(p.error_flag) = 1;
+    return;
+  }
+  const int unit = blockIdx.x / sp.items, item = blockIdx.x % sp.items;
+  const int hs = item % sp.hsplit, bh = item / sp.hsplit, b = bh / p.Hk, hk = bh % p.Hk;
+  const int group = p.Hq / p.Hk, heads = group / sp.hsplit, h_first = hk * group + hs * heads;
+  const bool far = unit >= sp.tiles;
+  const int kt = far ? (unit - sp.tiles) % sp.sink_tiles : unit;
+  const int chunk = far ? (unit - sp.tiles) / sp.sink_tiles : 0;
+  const int n = tc_valid(p, b);
+  const int k0 = kt * kTcRows;
+  const int last_tile = n > 0 ? (n - 1) / kTcRows : -1;
+  const int qlo = far ? kt + sp.near_span + 1 + chunk * (sp.near_span + 1) : kt;
+  const int qhi = min(last_tile, qlo + sp.near_span);
+  const int per_head = max(0, qhi - qlo + 1);
+  const int nit = k0 < n ? per_head * heads : 0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    for (int s = 0; s < L::qst; ++s) { mbar_init(&q_full[s], 1); mbar_init(&q_empty[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&g_full[s], 1); mbar_init(&g_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], 8); }
+    mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_ready, 8); mbar_init(ds_ready, 8); mbar_init(done, 1); mbar_init(patch, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) tc_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t kDp = 128, kDv = 256, kDk = 256 + D;
+
+  if (warp == 9) {
+    if (nit > 0) {
+      if (lane == 0) {
+        mbar_expect_tx(kv_full, 2 * L::tile);
+        tc_load_tile<D>(smem + L::k, &map_k, hk, k0, b, kv_full);
+        tc_load_tile<D>(smem + L::v, &map_v, hk, k0, b, kv_full);
+      }
+      bool ok = true;
+      int nq = 0, ng = 0;
+      uint32_t patched = 0;
+      float f = BwdRange<T>::unshift;
+      if (BwdRange<T>::scaled) {
+        float big = 0.f;
+        for (int e = lane; e < nit; e += 32)
+          big = fmaxf(big, p.gmax[((int64_t)b * p.Hq + h_first + e / per_head) * sp.tiles + qlo + e % per_head]);
+        const float up = bwd_factor(warp_max(big));
+        f *= up;
+        if (lane == 0) s_factor[0] = up;
+      }
+      for (int it = 0; it < nit && ok; ++it) {
+        const int h = h_first + it / per_head, q0 = (qlo + it % per_head) * kTcRows;
+        const int sq = it % L::qst, sg = it % L::gst;
+        const bool ends = q0 + kTcRows > n && n < p.T;            // the sequence ends inside this tile
+        uint8_t *tq = smem + L::q + sq * L::tile, *tg = smem + L::g + sg * L::tile;
+        if (it >= L::qst && !(ok = mbar_wait_warp(&q_empty[sq], (uint32_t)(it / L::qst + 1) & 1u))) break;
+        if (lane == 0) {
+          uint64_t* bar = ends ? patch : &q_full[sq];
+          mbar_expect_tx(bar, L::tile);
+          tc_load_tile<D>(tq, &map_q, h, q0, b, bar);
+        }
+        nq = ends ? it : it + 1;
+        if (ends) {
+          if (!(ok = mbar_wait_warp(patch, patched++ & 1u))) break;
+          tc_clear_rows<D>(tq, n - q0);
+          if (lane == 0) mbar_arrive(&q_full[sq]);
+        }
+        if (it >= L::gst && !(ok = mbar_wait_warp(&g_empty[sg], (uint32_t)(it / L::gst + 1) & 1u))) break;
+        if (lane == 0) {
+          uint64_t* bar = ends ? patch : &g_full[sg];
+          mbar_expect_tx(bar, L::tile);
+          tc_load_tile<D>(tg, &map_g, h, q0, b, bar);
+        }
+        ng = ends ? it : it + 1;
+        if (ends) {
+          if (!(ok = mbar_wait_warp(patch, patched++ & 1u))) break;
+          tc_clear_rows<D>(tg, n - q0);
+          if (lane == 0) mbar_arrive(&g_full[sg]);
+        }
+        // log-sum-exp and delta of the tile's rows; a row that is not there gets +inf: probability 0
+        if (it >= 2 && !(ok = mbar_wait_warp(&st_empty[it & 1], (uint32_t)(it / 2 + 1) & 1u))) break;
+        const int64_t at = ((int64_t)b * p.Hq + h) * p.T + q0;
+        float* st = s_stat + (it & 1) * 256;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = lane + 32 * e;
+          st[c] = q0 + c < n ? p.lse[at + c] - BwdRange<T>::shift : INFINITY;
+          st[128 + c] = q0 + c < n ? p.delta[at + c] * f : 0.f;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&st_full[it & 1]);
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        if (lane == 0) {                                          // no copy may still be under way at the end
+          mbar_wait(kv_full, 0);
+          for (int s = 0; s < L::qst; ++s) if (nq > s) mbar_wait(&q_full[s], (uint32_t)((nq - 1 - s) / L::qst) & 1u);
+          for (int s = 0; s < L::gst; ++s) if (ng > s) mbar_wait(&g_full[s], (uint32_t)((ng - 1 - s) / L::gst) & 1u);
+        }
+      }
+    }
+  } else if (warp == 8) {
+    if (lane == 0 && nit > 0) {
+      const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
+      const uint32_t sk = smem_u32(smem + L::k), sv = smem_u32(smem + L::v), sq = smem_u32(smem + L::q), sg = smem_u32(smem + L::g);
+      bool ok = mbar_wait(kv_full, 0);
+      auto scores = [&](int it) {
+        ok = mbar_wait(&q_full[it % L::qst], (uint32_t)(it / L::qst) & 1u);
+        tc_fence_after();
+        if (ok) { tc_scores<D>(tmem, sk, sq + (it % L::qst) * L::tile, id_s); umma_commit(s_full); }
+      };
+      auto dprobs = [&](int it) {
+        ok = mbar_wait(&g_full[it % L::gst], (uint32_t)(it / L::gst) & 1u);
+        tc_fence_after();
+        if (ok) { tc_scores<D>(tmem + kDp, sv, sg + (it % L::gst) * L::tile, id_s); umma_commit(dp_full); }
+      };
+      auto add = [&](uint32_t acc, uint32_t a, uint32_t tile, bool carry) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          umma_ts(tmem + acc, a + (k < 4 ? 8 * k : 64 + 8 * (k - 4)), make_desc_mn(tile + (uint32_t)k * 2048u, kTcHalf), id_o, (carry || k > 0) ? 1u : 0u);
+      };
+      if (ok) scores(0);
+      if (ok) dprobs(0);
+      for (int it = 0; it < nit && ok; ++it) {
+        ok = mbar_wait(p_ready, (uint32_t)it & 1u);
+        if (!ok) break;
+        tc_fence_after();
+        add(kDv, tmem, sg + (it % L::gst) * L::tile, it > 0);
+        umma_commit(&g_empty[it % L::gst]);                       // dP of this tile was issued before: dO is done with
+        if (it + 1 < nit) scores(it + 1);
+        if (!ok) break;
+        ok = mbar_wait(ds_ready, (uint32_t)it & 1u);
+        if (!ok) break;
+        tc_fence_after();
+        add(kDk, tmem + kDp, sq + (it % L::qst) * L::tile, it > 0);
+        umma_commit(&q_empty[it % L::qst]);
+        if (it + 1 < nit) dprobs(it + 1);
+      }
+      if (ok) umma_commit(done);
+      else { *abort_flag = 1; umma_commit(drain); mbar_wait(drain, 0); }
+    }
+  } else {
+    const int half = warp >> 2, quad = warp & 3;
+    const int row = quad * 32 + lane, j = k0 + row;
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const uint32_t ts = tmem + 64 * half + lane_off, td = tmem + kDp + 64 * half + lane_off;
+    const float sc = p.scale * kSwLog2e;
+    float f = 1.f;                                                // of dO in dS
+    bool ok = true;
+    for (int it = 0; it < nit; ++it) {
+      const int q0 = (qlo + it % per_head) * kTcRows;
+      const float* st = s_stat + (it & 1) * 256 + 64 * half;
+      ok = mbar_wait_warp(&st_full[it & 1], (uint32_t)(it / 2) & 1u) && mbar_wait_warp(s_full, (uint32_t)it & 1u);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t x[64], y[64];
+      tmem_ld32(ts, x);
+      tmem_ld32(ts + 32, x + 32);
+      tmem_wait_ld32(x);
+      tmem_wait_ld32(x + 32);
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        const float4 l4 = *reinterpret_cast<const float4*>(st + c);
+        x[c] = __float_as_uint(ex2(fmaf(__uint_as_float(x[c]), sc, -l4.x)));
+        x[c + 1] = __float_as_uint(ex2(fmaf(__uint_as_float(x[c + 1]), sc, -l4.y)));
+        x[c + 2] = __float_as_uint(ex2(fmaf(__uint_as_float(x[c + 2]), sc, -l4.z)));
+        x[c + 3] = __float_as_uint(ex2(fmaf(__uint_as_float(x[c + 3]), sc, -l4.w)));
+      }
+      const bool whole = k0 + kTcRows - 1 <= q0 && (q0 + kTcRows - 1 - k0 < p.window || k0 + kTcRows <= p.sinks);
+      if (!whole) {
+        // query i = base + c sees key j when c >= j - base, and c < j - base + window or j is a sink
+        const int base = q0 + 64 * half;
+        const int c_lo = j - base;
+        const int c_end = j < p.sinks ? 64 : (int)min((int64_t)64, (int64_t)(j - base) + p.window);
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c < c_lo || c >= c_end) x[c] = 0u;
+      }
+      uint32_t pk[32];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) pk[c] = pack2<T>(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1]));
+      tmem_st32(ts, pk);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready);
+      ok = mbar_wait_warp(dp_full, (uint32_t)it & 1u);
+      if (!ok) break;
+      tc_fence_after();
+      if (BwdRange<T>::scaled && it == 0) f = s_factor[0];
+      const float fu = f * BwdRange<T>::unshift;
+      auto ds = [&](uint32_t pr, uint32_t dp, float dl) {
+        return __uint_as_float(pr) * (BwdRange<T>::scaled ? fmaf(__uint_as_float(dp), fu, -dl) : __uint_as_float(dp) - dl);
+      };
+      tmem_ld32(td, y);
+      tmem_ld32(td + 32, y + 32);
+      tmem_wait_ld32(y);
+      tmem_wait_ld32(y + 32);
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        const float4 d4 = *reinterpret_cast<const float4*>(st + 128 + c);
+        pk[c >> 1] = pack2<T>(ds(x[c], y[c], d4.x), ds(x[c + 1], y[c + 1], d4.y));
+        pk[(c >> 1) + 1] = pack2<T>(ds(x[c + 2], y[c + 2], d4.z), ds(x[c + 3], y[c + 3], d4.w));
+      }
+      tmem_st32(td, pk);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(ds_ready); mbar_arrive(&st_empty[it & 1]); }
+    }
+    if (ok && nit > 0) ok = mbar_wait_warp(done, 0);
+    if (!ok) *abort_flag = 1;
+    tc_fence_after();
+    if (ok) {
+      // warps 0-3 write dK, warps 4-7 dV
+      const float mul = half == 0 ? p.scale / f : BwdRange<T>::unshift;
+      const uint32_t acc = tmem + (half == 0 ? kDk : kDv) + lane_off;
+      const bool parts = kt < sp.part_tiles;
+      const bool live = j < n && nit > 0;
+      float* part = nullptr;
+      if (parts) {
+        part = far ? dkv_far_part(sp, (int64_t)p.B * p.Hk, hs, chunk, bh, kt, D) : dkv_near_part(sp, (int64_t)p.B * p.Hk, hs, bh, kt, D);
+        part += ((int64_t)half * kTcRows + row) * D;
+      }
+      T* dst = static_cast<T*>(half == 0 ? p.dk : p.dv) + (((int64_t)b * p.T + j) * p.Hk + hk) * D;
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t o[32];
+        if (nit > 0) { tmem_ld32(acc + c0, o); tmem_wait_ld32(o); }
+        if (parts) {
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (live) w = make_float4(__uint_as_float(o[v * 4]) * mul, __uint_as_float(o[v * 4 + 1]) * mul, __uint_as_float(o[v * 4 + 2]) * mul,
+                                      __uint_as_float(o[v * 4 + 3]) * mul);
+            *reinterpret_cast<float4*>(part + c0 + v * 4) = w;
+          }
+        } else if (j < p.T) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (live) {
+              w.x = pack2<T>(__uint_as_float(o[v * 8]) * mul, __uint_as_float(o[v * 8 + 1]) * mul);
+              w.y = pack2<T>(__uint_as_float(o[v * 8 + 2]) * mul, __uint_as_float(o[v * 8 + 3]) * mul);
+              w.z = pack2<T>(__uint_as_float(o[v * 8 + 4]) * mul, __uint_as_float(o[v * 8 + 5]) * mul);
+              w.w = pack2<T>(__uint_as_float(o[v * 8 + 6]) * mul, __uint_as_float(o[v * 8 + 7]) * mul);
+            }
+            *reinterpret_cast<uint4*>(dst + c0 + v * 8) = w;
+          }
+        }
+      }
+    }
+  }
+  tc_finish(tmem, 512, warp, 8, abort_flag, p.error_flag);
+}
+
+// dK and dV of the key tiles that came in parts: blockIdx.x = (sample and key head, key tile).
+template <typename T, int D>
+__global__ void __launch_bounds__(256)
+sw_dkv_join_kernel(const TcParams p, const DkvSplit sp) {
+  const int kt = blockIdx.x % sp.part_tiles, bh = blockIdx.x / sp.part_tiles, b = bh / p.Hk, hk = bh % p.Hk;
+  const int64_t all = (int64_t)p.B * p.Hk;
+  for (int e = threadIdx.x; e < 2 * kTcRows * D / 8; e += 256) {
+    const int at = e * 8, which = at / (kTcRows * D), row = at / D % kTcRows, d = at % D, j = kt * kTcRows + row;
+    if (j >= p.T) continue;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    auto take = [&](const float* part) {
+      const float4 u = *reinterpret_cast<const float4*>(part + at), v = *reinterpret_cast<const float4*>(part + at + 4);
+      acc[0] += u.x; acc[1] += u.y; acc[2] += u.z; acc[3] += u.w;
+      acc[4] += v.x; acc[5] += v.y; acc[6] += v.z; acc[7] += v.w;
+    };
+    for (int hs = 0; hs < sp.hsplit; ++hs) {
+      take(dkv_near_part(sp, all, hs, bh, kt, D));
+      if (kt < sp.sink_tiles)
+        for (int c = 0; c < sp.far_chunks; ++c) take(dkv_far_part(sp, all, hs, c, bh, kt, D));
+    }
+    T* dst = static_cast<T*>(which == 0 ? p.dk : p.dv) + (((int64_t)b * p.T + j) * p.Hk + hk) * D + d;
+    Vec16<T> w;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) w.v[q] = Cvt<T>::from_f(acc[q]);
+    st16(dst, w);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+static DkvSplit dkv_split(const SwParams& p) {
+  DkvSplit s{};
+  s.tiles = (p.T + kTcRows - 1) / kTcRows;
+  s.near_span = (int)(((int64_t)kTcRows - 2 + p.window) / kTcRows);
+  if (s.near_span > s.tiles - 1) s.near_span = s.tiles - 1;
+  const int far = s.tiles - 1 - s.near_span;             // query tiles behind the windows of the first key tile
+  if (far > 0 && p.sinks > 0) {
+    s.sink_tiles = (p.sinks + kTcRows - 1) / kTcRows;
+    s.far_chunks = (far + s.near_span) / (s.near_span + 1);
+  }
+  // fewer CTAs than two for each SM: the heads of a group are walked side by side instead of one after another
+  const int group = p.Hq / p.Hk;
+  s.hsplit = 1;
+  for (int k = 1; k <= group; ++k)
+    if (group % k == 0) { s.hsplit = k; if ((int64_t)p.B * p.Hk * s.tiles * k >= 2 * sm_count()) break; }
+  s.part_tiles = s.hsplit > 1 ? s.tiles : s.sink_tiles;
+  s.items = p.B * p.Hk * s.hsplit;
+  return s;
+}
+
+static int64_t dkv_part_floats(const SwParams& p) {
+  const DkvSplit s = dkv_split(p);
+  return ((int64_t)s.hsplit * p.B * p.Hk * s.part_tiles + (int64_t)s.hsplit * s.far_chunks * p.B * p.Hk * s.sink_tiles) * 2 * kTcRows * p.D;
+}
+
+template <typename T, int D>
+static int tc_backward(const SwParams& p, float* parts, int bf16, int* error_flag, cudaStream_t st) {
+  CUtensorMap mq, mk, mv, mg;
+  int rc = tc_map(&mq, p.q, bf16, p.B, p.T, p.Hq, D, p.sq);
+  if (!rc) rc = tc_map(&mk, p.k, bf16, p.B, p.T, p.Hk, D, p.sk);
+  if (!rc) rc = tc_map(&mv, p.v, bf16, p.B, p.T, p.Hk, D, p.sv);
+  if (!rc) rc = tc_map(&mg, p.dout, bf16, p.B, p.T, p.Hq, D, p.sdo);
+  if (rc) return rc;
+  TcParams t = tc_params(p, error_flag);
+  t.items = p.B * p.Hq;
+  DkvSplit s = dkv_split(p);
+  s.parts = parts;
+  if (s.part_tiles && (!parts || (uintptr_t)parts % 16)) return -3;
+  const int64_t gq = (int64_t)s.tiles * t.items, gk = ((int64_t)s.tiles + (int64_t)s.sink_tiles * s.far_chunks) * s.items;
+  if (gq > 0x7fffffff || gk > 0x7fffffff) return -2;
+  static unsigned long long seen = 0;
+  if (first_on_device(&seen)) {
+    cudaFuncSetAttribute(sw_dq_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DqSmem<D>::total);
+    cudaFuncSetAttribute(sw_dkv_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DkvSmem<D>::total);
+  }
+  sw_dq_tc_kernel<T, D><<<(unsigned)gq, kFwdThreads, DqSmem<D>::total, st>>>(mq, mk, mv, mg, t, bf16);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return (int)e;
+  sw_dkv_tc_kernel<T, D><<<(unsigned)gk, kFwdThreads, DkvSmem<D>::total, st>>>(mq, mk, mv, mg, t, s, bf16);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || !s.part_tiles) return (int)e;
+  sw_dkv_join_kernel<T, D><<<(unsigned)(s.part_tiles * p.B * p.Hk), 256, 0, st>>>(t, s);
+  return (int)cudaGetLastError();
+}
