@@ -575,13 +575,13 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   tc_finish(tmem, 512, warp, 8, abort_flag, p.error_flag);
 }
 
-// dK and dV of the key tiles that came in parts: blockIdx.x = (sample and key head, key tile).
+// dK and dV of the key tiles that came in parts: blockIdx.x = (sample and key head, key tile), blockIdx.y a stretch of the tile.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 sw_dkv_join_kernel(const TcParams p, const DkvSplit sp) {
   const int kt = blockIdx.x % sp.part_tiles, bh = blockIdx.x / sp.part_tiles, b = bh / p.Hk, hk = bh % p.Hk;
   const int64_t all = (int64_t)p.B * p.Hk;
-  for (int e = threadIdx.x; e < 2 * kTcRows * D / 8; e += 256) {
+  for (int e = blockIdx.y * 256 + threadIdx.x; e < 2 * kTcRows * D / 8; e += 256 * gridDim.y) {
     const int at = e * 8, which = at / (kTcRows * D), row = at / D % kTcRows, d = at % D, j = kt * kTcRows + row;
     if (j >= p.T) continue;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -655,6 +655,6 @@ static int tc_backward(const SwParams& p, float* parts, int bf16, int* error_fla
   sw_dkv_tc_kernel<T, D><<<(unsigned)gk, kFwdThreads, DkvSmem<D>::total, st>>>(mq, mk, mv, mg, t, s, bf16);
   e = cudaGetLastError();
   if (e != cudaSuccess || !s.part_tiles) return (int)e;
-  sw_dkv_join_kernel<T, D><<<(unsigned)(s.part_tiles * p.B * p.Hk), 256, 0, st>>>(t, s);
+  sw_dkv_join_kernel<T, D><<<dim3((unsigned)(s.part_tiles * p.B * p.Hk), 2 * kTcRows * D / 8 / 256), 256, 0, st>>>(t, s);
   return (int)cudaGetLastError();
 }
