@@ -1,6 +1,4 @@
 """Helpers shared by the kernel wrappers."""
-import contextlib
-
 import torch
 
 from . import lib, ptr, stream_ptr, count_launch, check
@@ -52,9 +50,27 @@ def job_wide(choice):
 def on_device(t):
     """Context in which the device of ``t`` is the current one (the raw launchers start their kernels there); the caller's
     current device is put back on exit."""
-    if t.device.index == torch.cuda.current_device():
+    if t.get_device() == torch._C._cuda_getDevice():
         return _HERE
     return torch.cuda.device(t.device)
 
 
-_HERE = contextlib.nullcontext()
+def raw_stream(t):
+    """Handle of the current stream of the device of ``t``."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def address(t):
+    """Address of a tensor's data for a launcher (0 = no tensor)."""
+    return 0 if t is None else t.data_ptr()
+
+
+class _Here(object):
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_HERE = _Here()

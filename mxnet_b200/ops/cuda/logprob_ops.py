@@ -2,8 +2,8 @@
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import lib, ptr, stream_ptr, count_launch, check
-from ._util import dt, on_device
+from . import lib, count_launch, check
+from ._util import DT, address, on_device, raw_stream
 
 
 def _forward(x, tokens, k, ignore, keep):
@@ -13,10 +13,10 @@ def _forward(x, tokens, k, ignore, keep):
     ent = torch.empty(rows, dtype=torch.float32, device=dev)
     top_lp = torch.empty((rows, k), dtype=torch.float32, device=dev) if k else None
     top_id = torch.empty((rows, k), dtype=torch.int64, device=dev) if k else None
-    stat = torch.empty((rows, 2), dtype=torch.float32, device=dev) if keep else None
+    stat = torch.empty((rows, 3), dtype=torch.float32, device=dev) if keep else None
     with on_device(x):
-        check(lib().mxb_logprob_forward(dt(x), ptr(x), ptr(tokens), ptr(lp), ptr(ent), ptr(top_lp), ptr(top_id), ptr(stat), rows, cols,
-                                        k, ignore, stream_ptr(dev)), 'token_log_probs')
+        check(lib().mxb_logprob_forward(DT[x.dtype], x.data_ptr(), tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(), address(top_lp),
+                                        address(top_id), address(stat), rows, cols, k, ignore, raw_stream(x)), 'token_log_probs')
     count_launch(1)
     return lp, ent, top_lp, top_id, stat
 
@@ -25,7 +25,7 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, tokens, k, ignore):
         lp, ent, top_lp, top_id, stat = _forward(x, tokens, k, ignore, True)
-        ctx.save_for_backward(x, tokens, stat, ent, top_id)
+        ctx.save_for_backward(x, tokens, stat, top_id)
         ctx.args = (k, ignore)
         ctx.set_materialize_grads(False)
         if not k:
@@ -36,20 +36,17 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g_lp, g_ent, g_top=None, _=None):
-        x, tokens, stat, ent, top_id = ctx.saved_tensors
+        x, tokens, stat, top_id = ctx.saved_tensors
         k, ignore = ctx.args
         rows, cols = x.shape
         g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
         dx = torch.empty_like(x)
         with on_device(x):
-            check(lib().mxb_logprob_backward(dt(x), ptr(x), ptr(dx), ptr(tokens), ptr(stat), ptr(ent), ptr(g_lp), ptr(g_ent), ptr(g_top),
-                                             ptr(top_id), rows, cols, k, ignore, stream_ptr(x.device)), 'token_log_probs backward')
+            check(lib().mxb_logprob_backward(DT[x.dtype], x.data_ptr(), dx.data_ptr(), tokens.data_ptr(), stat.data_ptr(), address(g_lp),
+                                             address(g_ent), address(g_top), address(top_id), rows, cols, k, ignore, raw_stream(x)),
+                  'token_log_probs backward')
         count_launch(1)
         return dx, None, None, None
-
-
-def max_top():
-    return lib().mxb_logprob_max_top()
 
 
 def token_log_probs(x, tokens, k, ignore):

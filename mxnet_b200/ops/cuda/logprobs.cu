@@ -146,7 +146,7 @@ struct LogProbParams {
   float* entropy;
   float* top_lp;           // [rows, k] or null
   int64_t* top_id;
-  float* stat;             // [rows, 2]: m and log1p(r), read by the backward pass (or null)
+  float* stat;             // [rows, 3]: m, log1p(r) and the entropy, read by the backward pass (or null)
   int64_t rows;
   int cols, k;
   int64_t ignore;
@@ -208,8 +208,9 @@ logprob_fwd_kernel(const LogProbParams p) {
       else if (t < 0 || t >= p.cols) lp = NAN;                    // no such token
       else lp = empty ? -INFINITY : (Cvt<T>::to_f(x[t]) - all.m) - lt;
       p.log_prob[row] = lp;
-      p.entropy[row] = empty ? 0.f : lt + all.w / (1.f + all.r);
-      if (p.stat) { p.stat[2 * row] = all.m; p.stat[2 * row + 1] = lt; }
+      const float ent = empty ? 0.f : lt + all.w / (1.f + all.r);
+      p.entropy[row] = ent;
+      if (p.stat) { p.stat[3 * row] = all.m; p.stat[3 * row + 1] = lt; p.stat[3 * row + 2] = ent; }
     }
     if (p.k) {
       for (int half = 1; half < nw; half <<= 1) {
@@ -277,7 +278,6 @@ struct LogProbGradParams {
   void* dx;
   const int64_t* tokens;
   const float* stat;
-  const float* entropy;
   const float* g_lp;       // each may be null
   const float* g_ent;
   const float* g_top;
@@ -295,7 +295,7 @@ logprob_bwd_kernel(const LogProbGradParams p) {
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + row * p.cols;
     T* dx = static_cast<T*>(p.dx) + row * p.cols;
-    const float m = p.stat[2 * row], lt = p.stat[2 * row + 1], ent = p.entropy[row];
+    const float m = p.stat[3 * row], lt = p.stat[3 * row + 1], ent = p.stat[3 * row + 2];
     const int64_t t = p.tokens[row];
     float gl = p.g_lp ? p.g_lp[row] : 0.f;
     if (t == p.ignore) gl = 0.f;
@@ -354,9 +354,7 @@ inline int lp_threads(int cols, int size) {
 
 using namespace mxb;
 
-MXB_EXPORT int mxb_logprob_max_top(void) { return kLpMaxTop; }
-
-// x: [rows, cols]; tokens: [rows]; top_lp / top_id: [rows, k] (k may be 0); stat: [rows, 2] floats for the backward pass.
+// x: [rows, cols]; tokens: [rows]; top_lp / top_id: [rows, k] (k may be 0); stat: [rows, 3] floats for the backward pass.
 MXB_EXPORT int mxb_logprob_forward(int dtype, const void* x, const int64_t* tokens, float* log_prob, float* entropy, float* top_lp,
                                    int64_t* top_id, float* stat, int64_t rows, int cols, int k, int64_t ignore, void* stream) {
   if (rows < 1 || cols < 1 || k < 0 || k > kLpMaxTop || k > cols) return -2;
@@ -372,11 +370,11 @@ MXB_EXPORT int mxb_logprob_forward(int dtype, const void* x, const int64_t* toke
 }
 
 // dx: [rows, cols] of the logits' type; g_lp, g_ent: [rows] floats, g_top: [rows, k] floats (each may be null).
-MXB_EXPORT int mxb_logprob_backward(int dtype, const void* x, void* dx, const int64_t* tokens, const float* stat, const float* entropy,
+MXB_EXPORT int mxb_logprob_backward(int dtype, const void* x, void* dx, const int64_t* tokens, const float* stat,
                                     const float* g_lp, const float* g_ent, const float* g_top, const int64_t* top_id, int64_t rows,
                                     int cols, int k, int64_t ignore, void* stream) {
   if (rows < 1 || cols < 1 || k < 0 || k > kLpMaxTop || k > cols) return -2;
-  LogProbGradParams p{x, dx, tokens, stat, entropy, g_lp, g_ent, g_top, top_id, rows, cols, k, ignore};
+  LogProbGradParams p{x, dx, tokens, stat, g_lp, g_ent, g_top, top_id, rows, cols, k, ignore};
   cudaStream_t st = (cudaStream_t)stream;
   const int64_t cap = (int64_t)sm_count() * 64;
   const unsigned grid = (unsigned)(rows < cap ? rows : cap);

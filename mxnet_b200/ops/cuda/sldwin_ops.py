@@ -5,10 +5,9 @@ import ctypes as C
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import lib, ptr, stream_ptr, count_launch, check
-from ._util import dt, on_device
+from . import lib, count_launch, check
+from ._util import DT, address, on_device, raw_stream
 
-MAX_DIM = 256
 _DIMS7, _DIMS6 = C.c_int * 7, C.c_int * 6
 _S6, _S12 = C.c_int64 * 6, C.c_int64 * 12
 
@@ -19,9 +18,9 @@ _report = []          # a word of pinned host memory that the kernels set when a
 def _error_word():
     if not _report:
         if torch.cuda.is_current_stream_capturing():
-            return C.c_void_p(0)                                  # a capture allows no allocation of host memory
+            return 0                                              # a capture allows no allocation of host memory
         word = torch.zeros(1, dtype=torch.int32).pin_memory()
-        _report.extend((word, C.c_void_p(word.data_ptr()), C.c_int.from_address(word.data_ptr())))
+        _report.extend((word, word.data_ptr(), C.c_int.from_address(word.data_ptr())))
     elif _report[2].value:
         _report[2].value = 0
         raise RuntimeError('an earlier call reported a barrier time-out inside its kernel: its results are not valid')
@@ -42,14 +41,15 @@ def _rows(t):
 
 
 def _forward(q, k, v, valid, window, sinks, scale, keep):
-    B, T, Hq, D = q.shape
-    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if keep else None
+    B, T, Hq, D = shape = q.shape
+    dtype, dev = q.dtype, q.device
+    out = torch.empty(shape, dtype=dtype, device=dev)
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev) if keep else None
     dims = _DIMS7(B, T, Hq, k.shape[2], D, window, sinks)
     strides = _S12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
     with on_device(q):
-        check(lib().mxb_sldwin_forward(dt(q), ptr(q), ptr(k), ptr(v), ptr(valid), ptr(out), ptr(lse), dims, strides, scale,
-                                       _error_word(), stream_ptr(q.device)), 'sldwin_attention')
+        check(lib().mxb_sldwin_forward(DT[dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), address(valid), out.data_ptr(), address(lse),
+                                       dims, strides, scale, _error_word(), raw_stream(q)), 'sldwin_attention')
     count_launch(1)
     return out, lse
 
@@ -67,56 +67,72 @@ class _SldwinAttention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, valid, out, lse = ctx.saved_tensors
         window, sinks, scale = ctx.args
-        B, T, Hq, D = q.shape
-        Hk = k.shape[2]
+        B, T, Hq, D = shape = q.shape
+        kshape = k.shape
+        dtype, dev = q.dtype, q.device
         dout = _rows(dout)
-        dq = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
-        dk = torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device)
-        dv = torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device)
-        delta = torch.empty(B * Hq * (T + (T + 127) // 128), dtype=torch.float32, device=q.device)
-        dims = _DIMS7(B, T, Hq, Hk, D, window, sinks)
+        dq = torch.empty(shape, dtype=dtype, device=dev)
+        dk = torch.empty(kshape, dtype=dtype, device=dev)
+        dv = torch.empty(kshape, dtype=dtype, device=dev)
+        dims = _DIMS7(B, T, Hq, kshape[2], D, window, sinks)
         strides = _S12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *dout.stride()[:3])
-        words = lib().mxb_sldwin_backward_parts(dt(q), dims)      # key gradients that several blocks sum up
-        parts = torch.empty(words, dtype=torch.float32, device=q.device) if words else None
+        L, code = lib(), DT[dtype]
+        # workspace: rowsum(dO * O) and the largest |dO| of each query tile, then key gradients that several blocks sum up
+        rows = (B * Hq * (T + (T + 127) // 128) + 3) // 4 * 4
+        parts = L.mxb_sldwin_backward_parts(code, dims)
+        work = torch.empty(rows + parts, dtype=torch.float32, device=dev)
+        at = work.data_ptr()
         with on_device(q):
-            check(lib().mxb_sldwin_backward(dt(q), ptr(q), ptr(k), ptr(v), ptr(valid), ptr(out), ptr(dout), ptr(lse), ptr(delta), ptr(parts),
-                                            ptr(dq), ptr(dk), ptr(dv), dims, strides, scale, _error_word(), stream_ptr(q.device)),
-                  'sldwin_attention backward')
-        count_launch(3 if words else 2)
+            check(L.mxb_sldwin_backward(code, q.data_ptr(), k.data_ptr(), v.data_ptr(), address(valid), out.data_ptr(), dout.data_ptr(),
+                                        lse.data_ptr(), at, at + 4 * rows if parts else 0, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                        dims, strides, scale, _error_word(), raw_stream(q)), 'sldwin_attention backward')
+        count_launch(3 if parts else 2)
         return dq, dk, dv, None, None, None, None
 
 
 def attention(q, k, v, valid, window, sinks, scale):
     q, k, v = _rows(q), _rows(k), _rows(v)
     if valid is not None:
-        valid = valid.to(torch.int32).contiguous()
+        valid = _int32(valid)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _SldwinAttention.apply(q, k, v, valid, window, sinks, scale)
     return _forward(q, k, v, valid, window, sinks, scale, False)[0]
+
+
+def _int32(valid):
+    """Lengths as the kernels read them (real ones are cut, values beyond 32 bits stay beyond every length)."""
+    if valid.dtype == torch.int32 and valid.is_contiguous():
+        return valid
+    return valid.clamp(-1, (1 << 31) - 128).to(torch.int32).contiguous()
 
 
 def cache_fill(k, v, key_cache, value_cache, valid, sinks):
     B, T, H, D = k.shape
     k, v = _rows(k), _rows(v)
     if valid is not None:
-        valid = valid.to(torch.int32).contiguous()
+        valid = _int32(valid)
     dims = _DIMS6(B, T, H, D, key_cache.shape[1], sinks)
     strides = _S12(*k.stride()[:3], *v.stride()[:3], *key_cache.stride()[:3], *value_cache.stride()[:3])
     with on_device(k):
-        check(lib().mxb_cache_fill(dt(k), ptr(k), ptr(v), ptr(key_cache), ptr(value_cache), ptr(valid), dims, strides,
-                                   stream_ptr(k.device)), 'sldwin_cache_fill')
+        check(lib().mxb_cache_fill(DT[k.dtype], k.data_ptr(), v.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), address(valid),
+                                   dims, strides, raw_stream(k)), 'sldwin_cache_fill')
     count_launch(1)
 
 
+def _dense(t):
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def attention_step(q, k, v, key_cache, value_cache, positions, window, sinks, scale):
-    B, Hq, D = q.shape
-    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
-    positions = positions.to(torch.int64).contiguous()
-    out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
+    B, Hq, D = shape = q.shape
+    q, k, v = _dense(q), _dense(k), _dense(v)
+    if positions.dtype != torch.int64 or not positions.is_contiguous():
+        positions = positions.to(torch.int64).contiguous()
+    out = torch.empty(shape, dtype=q.dtype, device=q.device)
     dims = _DIMS7(B, Hq, k.shape[1], D, key_cache.shape[1], window, sinks)
     strides = _S6(*key_cache.stride()[:3], *value_cache.stride()[:3])
     with on_device(q):
-        check(lib().mxb_sldwin_step(dt(q), ptr(q), ptr(k), ptr(v), ptr(key_cache), ptr(value_cache), ptr(positions), ptr(out), dims,
-                                    strides, scale, stream_ptr(q.device)), 'sldwin_attention_step')
+        check(lib().mxb_sldwin_step(DT[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+                                    positions.data_ptr(), out.data_ptr(), dims, strides, scale, raw_stream(q)), 'sldwin_attention_step')
     count_launch(1)
     return out

@@ -25,14 +25,24 @@ def _need(ok, what, *args):
 
 
 def _kernels(t):
-    if not t.is_cuda or t.dtype not in _KERNEL_TYPES or t.numel() == 0 or not env.get('MXNET_B200_KERNELS'):
-        return False
-    from . import cuda
-    return cuda.available()
+    return t.is_cuda and t.dtype in _KERNEL_TYPES and t.numel() > 0 and env.get('MXNET_B200_KERNELS')
+
+
+def _alike(first, *others):
+    """Floating-point arrays of one type on one device."""
+    t, dev = first.dtype, first.device
+    for o in others:
+        if o.dtype is not t or o.device != dev:
+            return False
+    return t.is_floating_point
+
+
+def _plain(t):
+    """``t`` outside of its graph."""
+    return t.detach() if t.requires_grad else t
 
 
 def _same(name, first, **others):
-    """Arrays of one call share a type and a device."""
     _need(first.is_floating_point(), '%s: floating-point arrays expected, got %s', name, first.dtype)
     for k, t in others.items():
         _need(t.dtype == first.dtype, '%s: %s has type %s, expected %s', name, k, t.dtype, first.dtype)
@@ -97,6 +107,29 @@ def rotary_inv_freq(dim=64, base=10000.0, scaling='none', factor=1.0, original_l
     return torch.tensor(f, dtype=torch.float64).to(td).to(dev)
 
 
+def _rotary_fits(data, positions, inv_freq):
+    if data.dim() != 4:
+        return False
+    B, T, _, D = data.shape
+    at = positions.shape
+    return data.is_floating_point() and (at == (T,) or at == (B, T)) and inv_freq.dim() == 1 and 1 <= inv_freq.shape[0] <= D // 2 and \
+        inv_freq.is_floating_point() and not positions.is_complex() and positions.dtype != torch.bool and \
+        positions.device == data.device and inv_freq.device == data.device
+
+
+def _rotary_refuse(name, data, positions, inv_freq):
+    _need(positions is not None and inv_freq is not None, '%s: data, positions and inv_freq are required', name)
+    _need(data.dim() == 4, '%s: data must be (B, T, H, D), got %s', name, tuple(data.shape))
+    _need(data.is_floating_point(), '%s: data must be floating point, got %s', name, data.dtype)
+    B, T, H, D = data.shape
+    _need(tuple(positions.shape) in ((T,), (B, T)), '%s: positions must be (%d,) or (%d, %d), got %s', name, T, B, T, tuple(positions.shape))
+    _need(inv_freq.dim() == 1 and 1 <= inv_freq.shape[0] <= D // 2, '%s: inv_freq must be (R / 2,) with 2 <= R <= %d, got %s', name, D,
+          tuple(inv_freq.shape))
+    _need(inv_freq.is_floating_point() and not positions.is_complex() and positions.dtype != torch.bool,
+          '%s: inv_freq must be floating point and positions numbers, got %s and %s', name, inv_freq.dtype, positions.dtype)
+    raise MXNetError('%s: arrays on %s, %s and %s, expected one device' % (name, data.device, positions.device, inv_freq.device))
+
+
 @register('_contrib_rotary_embedding', '_npx_rotary_embedding', inputs=('data', 'positions', 'inv_freq'),
           defaults={'interleaved': False, 'scale': 1.0})
 def rotary_embedding(data, positions=None, inv_freq=None, interleaved=False, scale=1.0):
@@ -108,21 +141,13 @@ def rotary_embedding(data, positions=None, inv_freq=None, interleaved=False, sca
     ``scale``; the channels behind them pass through.  Angles are formed in 64 bits.  Returns a new (B, T, H, D) array;
     differentiable in ``data``."""
     name = 'rotary_embedding'
-    _need(positions is not None and inv_freq is not None, '%s: data, positions and inv_freq are required', name)
-    _need(data.dim() == 4, '%s: data must be (B, T, H, D), got %s', name, tuple(data.shape))
-    _need(data.is_floating_point(), '%s: data must be floating point, got %s', name, data.dtype)
+    if positions is None or inv_freq is None or not _rotary_fits(data, positions, inv_freq):
+        _rotary_refuse(name, data, positions, inv_freq)
     B, T, H, D = data.shape
-    _need(tuple(positions.shape) in ((T,), (B, T)), '%s: positions must be (%d,) or (%d, %d), got %s', name, T, B, T, tuple(positions.shape))
-    _need(inv_freq.dim() == 1 and 1 <= inv_freq.shape[0] <= D // 2, '%s: inv_freq must be (R / 2,) with 2 <= R <= %d, got %s', name, D,
-          tuple(inv_freq.shape))
-    _need(inv_freq.is_floating_point() and not positions.is_complex() and positions.dtype != torch.bool,
-          '%s: inv_freq must be floating point and positions numbers, got %s and %s', name, inv_freq.dtype, positions.dtype)
-    _need(positions.device == data.device and inv_freq.device == data.device, '%s: arrays on %s, %s and %s, expected one device', name,
-          data.device, positions.device, inv_freq.device)
-    positions, inv_freq, scale = positions.detach(), inv_freq.detach(), float(scale)
+    positions, inv_freq, scale = _plain(positions), _plain(inv_freq), float(scale)
     if _kernels(data) and D <= 1024 and H <= 4096 and B * T < (1 << 30):
         from .cuda import rotary_ops
-        return rotary_ops.rotary_embedding(data, positions, inv_freq, bool(interleaved), scale)
+        return rotary_ops.rotary_embedding(data, positions, inv_freq, 1 if interleaved else 0, scale)
     R = 2 * inv_freq.shape[0]
     x = _work(data)
     angle = positions.double().unsqueeze(-1) * inv_freq.double()
@@ -140,16 +165,42 @@ def rotary_embedding(data, positions=None, inv_freq=None, interleaved=False, sca
 # sliding-window attention with sinks
 # ------------------------------------------------------------------------------------------
 def _window_args(name, window, sinks, scale, D):
-    window, sinks = _whole(name, 'window', window or 0), _whole(name, 'sinks', sinks or 0)
-    _need(window >= 0 and sinks >= 0, '%s: window and sinks must not be negative, got %d and %d', name, window, sinks)
+    if type(window) is not int or type(sinks) is not int:
+        window, sinks = _whole(name, 'window', window or 0), _whole(name, 'sinks', sinks or 0)
+    if window < 0 or sinks < 0:
+        _need(False, '%s: window and sinks must not be negative, got %d and %d', name, window, sinks)
     return window, sinks, 1.0 / math.sqrt(D) if scale is None else float(scale)
+
+
+def _heads_fit(query, key, value, axes):
+    if query.dim() != axes or key.dim() != axes:
+        return False
+    qs, ks = query.shape, key.shape
+    return qs[:-2] == ks[:-2] and qs[-1] == ks[-1] and ks == value.shape and ks[-2] >= 1 and qs[-2] % ks[-2] == 0 and qs[-1] >= 1 and \
+        _alike(query, key, value)
+
+
+def _heads_refuse(name, query, key, value, lead):
+    _need(key is not None and value is not None, '%s: query, key and value are required', name)
+    form = '(%s, H, D)' % ', '.join(lead)
+    n = len(lead) + 2
+    _need(query.dim() == n and key.dim() == n, '%s: query and key must be %s, got %s and %s', name, form, tuple(query.shape), tuple(key.shape))
+    qs, ks = tuple(query.shape), tuple(key.shape)
+    _need(qs[:-2] == ks[:-2] and qs[-1] == ks[-1] and ks == tuple(value.shape), '%s: query, key and value must agree in all but the heads, '
+          'key and value in these too, got %s, %s and %s', name, qs, ks, tuple(value.shape))
+    _need(ks[-2] >= 1 and qs[-2] % ks[-2] == 0, '%s: %d query heads are not a multiple of %d key heads', name, qs[-2], ks[-2])
+    _need(qs[-1] >= 1, '%s: heads have no channels', name)
+    _same(name, query, key=key, value=value)
+    raise MXNetError('%s: bad arguments' % name)
 
 
 def _lengths(name, valid_length, B, device):
     if valid_length is not None:
-        _need(tuple(valid_length.shape) in ((B,), (B, 1)), '%s: valid_length must be (%d,), got %s', name, B, tuple(valid_length.shape))
-        _need(valid_length.device == device, '%s: valid_length is on %s, expected %s', name, valid_length.device, device)
-        valid_length = valid_length.detach().reshape(B)
+        if valid_length.shape != (B,) or valid_length.device != device:
+            _need(tuple(valid_length.shape) in ((B,), (B, 1)), '%s: valid_length must be (%d,), got %s', name, B, tuple(valid_length.shape))
+            _need(valid_length.device == device, '%s: valid_length is on %s, expected %s', name, valid_length.device, device)
+            valid_length = valid_length.reshape(B)
+        valid_length = _plain(valid_length)
     return valid_length
 
 
@@ -174,15 +225,10 @@ def sldwin_attention(query, key=None, value=None, valid_length=None, window=0, s
 
     Returns (B, T, Hq, D); differentiable in query, key and value.  The (T, T) scores are not stored on the GPU."""
     name = 'sldwin_attention'
-    _need(key is not None and value is not None, '%s: query, key and value are required', name)
-    _need(query.dim() == 4 and key.dim() == 4, '%s: query and key must be (B, T, H, D), got %s and %s', name, tuple(query.shape),
-          tuple(key.shape))
+    if key is None or value is None or not _heads_fit(query, key, value, 4):
+        _heads_refuse(name, query, key, value, ('B', 'T'))
     B, T, Hq, D = query.shape
     Hk = key.shape[2]
-    _need(tuple(key.shape) == (B, T, Hk, D) and value.shape == key.shape, '%s: key and value must be (%d, %d, Hk, %d), got %s and %s',
-          name, B, T, D, tuple(key.shape), tuple(value.shape))
-    _need(Hk >= 1 and Hq % Hk == 0, '%s: %d query heads are not a multiple of %d key heads', name, Hq, Hk)
-    _same(name, query, key=key, value=value)
     window, sinks, scale = _window_args(name, window, sinks, scale, D)
     valid = _lengths(name, valid_length, B, query.device)
     if _kernels(query) and D <= 256 and T <= (1 << 30):
@@ -209,20 +255,30 @@ def sldwin_attention(query, key=None, value=None, valid_length=None, window=0, s
     return out.permute(0, 3, 1, 2, 4).reshape(B, T, Hq, D).to(query.dtype)
 
 
+def _adjacent(t):
+    """Channels next to one another, and no two elements of the array in one place."""
+    s, n = t.stride(), t.shape
+    return (s[3] == 1 or n[3] == 1) and (s[0] > 0 or n[0] == 1) and (s[1] > 0 or n[1] == 1) and (s[2] > 0 or n[2] == 1)
+
+
 def _cache_args(name, key_cache, value_cache, B, Hk, D, sinks, like):
+    if key_cache is not None and value_cache is not None and key_cache.dim() == 4:
+        n = key_cache.shape
+        if n[0] == B and n[2] == Hk and n[3] == D and n[1] > sinks and value_cache.shape == n and _alike(like, key_cache, value_cache) and \
+                (B == 0 or (_adjacent(key_cache) and _adjacent(value_cache))):
+            return
     _need(key_cache is not None and value_cache is not None, '%s: key_cache and value_cache are required', name)
     _need(key_cache.dim() == 4 and tuple(key_cache.shape[:1] + key_cache.shape[2:]) == (B, Hk, D) and value_cache.shape == key_cache.shape,
           '%s: caches must be (%d, C, %d, %d), got %s and %s', name, B, Hk, D, tuple(key_cache.shape), tuple(value_cache.shape))
     _same(name, like, key_cache=key_cache, value_cache=value_cache)
     _need(key_cache.shape[1] > sinks, '%s: a cache of %d rows has no room beside %d sinks', name, key_cache.shape[1], sinks)
-    for which, t in (('key_cache', key_cache), ('value_cache', value_cache)):
-        _need(t.numel() == 0 or t.stride(3) == 1 or D == 1, '%s: the channels of %s must be adjacent', name, which)
-        _need(all(t.stride(a) > 0 or t.shape[a] == 1 for a in range(4)) or t.numel() == 0, '%s: %s is an expanded view', name, which)
+    raise MXNetError('%s: the channels of a cache must be adjacent, and no axis an expanded one' % name)
 
 
 def _no_gradient(name, *arrays):
-    _need(not (torch.is_grad_enabled() and any(a.requires_grad for a in arrays)),
-          '%s updates its caches in place and has no gradient: call it outside of autograd.record(), or on detached arrays', name)
+    if torch.is_grad_enabled():
+        _need(not any(a.requires_grad for a in arrays), '%s updates its caches in place and has no gradient: call it '
+              'outside of autograd.record(), or on detached arrays', name)
 
 
 def _written(*arrays):
@@ -286,21 +342,19 @@ def sldwin_attention_step(query, key=None, value=None, key_cache=None, value_cac
 
     Returns (B, Hq, D).  Has no gradient."""
     name = 'sldwin_attention_step'
-    _need(key is not None and value is not None and positions is not None, '%s: query, key, value, caches and positions are required', name)
-    _need(query.dim() == 3 and key.dim() == 3, '%s: query and key must be (B, H, D), got %s and %s', name, tuple(query.shape),
-          tuple(key.shape))
+    _need(positions is not None, '%s: positions are required', name)
+    if key is None or value is None or not _heads_fit(query, key, value, 3):
+        _heads_refuse(name, query, key, value, ('B',))
     B, Hq, D = query.shape
     Hk = key.shape[1]
-    _need(tuple(key.shape) == (B, Hk, D) and value.shape == key.shape, '%s: key and value must be (%d, Hk, %d), got %s and %s', name, B, D,
-          tuple(key.shape), tuple(value.shape))
-    _need(Hk >= 1 and Hq % Hk == 0, '%s: %d query heads are not a multiple of %d key heads', name, Hq, Hk)
-    _same(name, query, key=key, value=value)
     window, sinks, scale = _window_args(name, window, sinks, scale, D)
     _cache_args(name, key_cache, value_cache, B, Hk, D, sinks, query)
-    _need(tuple(positions.shape) in ((B,), (B, 1)) and positions.device == query.device, '%s: positions must be (%d,) on %s, got %s on %s',
-          name, B, query.device, tuple(positions.shape), positions.device)
+    if positions.shape != (B,) or positions.device != query.device:
+        _need(tuple(positions.shape) in ((B,), (B, 1)) and positions.device == query.device, '%s: positions must be (%d,) on %s, got %s on %s',
+              name, B, query.device, tuple(positions.shape), positions.device)
+        positions = positions.reshape(B)
     _no_gradient(name, query, key, value, key_cache, value_cache)
-    positions = positions.detach().reshape(B)
+    positions = _plain(positions)
     ring = key_cache.shape[1] - sinks
     window = min(window, ring) or ring
     if _kernels(query) and D <= 256:
@@ -346,22 +400,26 @@ def token_log_probs(logits, tokens=None, topk=0, ignore_label=-1):
     name = 'token_log_probs'
     _need(tokens is not None, '%s: logits and tokens are required', name)
     _need(logits.dim() >= 1 and logits.is_floating_point(), '%s: logits must be floating-point (..., V), got %s of %s', name,
-          tuple(logits.shape), logits.dtype)
-    V = logits.shape[-1]
-    lead = tuple(logits.shape[:-1])
-    _need(tuple(tokens.shape) == lead, '%s: tokens must be %s, got %s', name, lead, tuple(tokens.shape))
+          logits.shape, logits.dtype)
+    shape = logits.shape
+    V, lead = shape[-1], shape[:-1]
+    _need(tokens.shape == lead, '%s: tokens must be %s, got %s', name, tuple(lead), tuple(tokens.shape))
     _need(tokens.device == logits.device, '%s: tokens are on %s, expected %s', name, tokens.device, logits.device)
     k, ignore = _whole(name, 'topk', topk or 0), _whole(name, 'ignore_label', ignore_label)
-    _need(0 <= k <= min(V, _MAX_TOP), '%s: topk must be between 0 and %d, got %d', name, min(V, _MAX_TOP), k)
     _need(V >= 1, '%s: logits have no entries', name)
-    tok = tokens.detach().reshape(-1).long()
-    x = logits.reshape(-1, V)
+    _need(0 <= k <= min(V, _MAX_TOP), '%s: topk must be between 0 and %d, got %d', name, min(V, _MAX_TOP), k)
+    flat = len(shape) == 2
+    tok, x = _plain(tokens), logits
+    if not flat:
+        tok, x = tok.reshape(-1), x.reshape(-1, V)
+    if tok.dtype != torch.int64:
+        tok = tok.long()
     if _kernels(logits) and V < (1 << 31) - 1024:
         from .cuda import logprob_ops
         res = logprob_ops.token_log_probs(x.contiguous(), tok.contiguous(), k, ignore)
     else:
         res = _token_log_probs(_work(x), tok, k, ignore)
-    return tuple(r.reshape(lead if i < 2 else lead + (k,)) for i, r in enumerate(res))
+    return res if flat else tuple(r.reshape(lead if i < 2 else lead + (k,)) for i, r in enumerate(res))
 
 
 def _token_log_probs(x, tok, k, ignore):
