@@ -7,64 +7,140 @@
 //   backward: with h = dL/dentropy and G = dL/dlogp_token + sum of the alternatives' gradients,
 //     dx_i = -p_i (G + h (log p_i + entropy)) + [i = token] dL/dlogp_token + [i = alternative j] dL/dtop_j.
 //
-// The forward pass reads the logits once and keeps (m, r, w) for each thread, rescaled when the thread's maximum moves.
+// The forward pass reads the logits once; each thread keeps (maximum, sum, weighted sum), moved to a new maximum at most once
+// for 64 bytes.  The thread that holds the row's only largest element cannot tell a small rest from that element's 1: its
+// few vectors are added up again without it by one warp, out of cache.
 // Alternatives: the k-th largest of the threads' maxima is a lower bound of the k-th largest element, so only the elements
-// of threads whose maximum reaches it (k of them, more with ties) are read a second time, out of cache; a warp keeps its 32
-// best as one sorted entry for each lane.  Equal logits rank by the lower index.
+// of threads whose maximum reaches it (k of them, more with ties) are read a second time; a warp keeps its 32 best as one
+// sorted entry for each lane.  Equal logits rank by the lower index.
+// Few rows: a cluster of CTAs shares a row and joins over distributed shared memory.
 #include "common.cuh"
 
 namespace mxb {
 
 constexpr int kLpMaxTop = 32;
 
-struct RowStat { float m, r, w; };       // m = -inf: nothing yet (total 0)
+struct RowStat { float m, r, w; };       // m = -inf: nothing yet (total 0); otherwise the total is 1 + r
 
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ RowStat rs_merge(const RowStat& a, const RowStat& b) {
   const bool a_hi = a.m >= b.m;
   const RowStat hi = a_hi ? a : b, lo = a_hi ? b : a;
-  if (!(lo.m > -INFINITY)) return {hi.m, hi.r + (lo.r != lo.r ? lo.r : 0.f), hi.w};   // an empty side only passes a NaN on
+  if (!(lo.m > -INFINITY)) return hi;
+  if (hi.m == INFINITY) return {hi.m, NAN, NAN};
   const float d = hi.m - lo.m, f = exp2f(-d * kLog2e);
   // f = 0 (a gap beyond the range of exp, such as to a mask of the type's lowest value): d times the total may overflow
-  return {hi.m, hi.r + (1.f + lo.r) * f, f > 0.f ? hi.w + f * (lo.w + d * (1.f + lo.r)) : hi.w + 0.f * lo.r};
+  return {hi.m, hi.r + (1.f + lo.r) * f, f > 0.f ? hi.w + f * (lo.w + d * (1.f + lo.r)) : hi.w};
 }
 
-template <int N>
-__device__ __forceinline__ void rs_add(RowStat& s, const float (&x)[N]) {
-  float cm = x[0];
-#pragma unroll
-  for (int j = 1; j < N; ++j) cm = fmaxf(cm, x[j]);
-  if (cm <= s.m && s.m > -INFINITY) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float d = s.m - x[j], e = exp2f(-d * kLog2e);
-      s.r += e;
-      s.w += e > 0.f ? e * d : e;                         // e = 0 covers x = -inf, where e d would be 0 * inf; a NaN stays one
-    }
-    return;
-  }
-  if (cm > s.m) {
-    if (s.m > -INFINITY) {
-      const float d = cm - s.m, f = exp2f(-d * kLog2e), t = 1.f + s.r;
-      s.w = f * (s.w + d * t);
-      s.r = t * f;
-      if (!(f > 0.f)) s.w = f;
-    }
-    s.m = cm;
-    bool one = true;                                      // one element of the maximum is the 1 of the total
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (one && x[j] == cm) { one = false; continue; }
-      const float d = cm - x[j], e = exp2f(-d * kLog2e);
-      s.r += e;
-      s.w += e > 0.f ? e * d : e;
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < N; ++j) if (x[j] != x[j]) s.r = x[j];   // nothing but NaN (and -inf) so far
+__device__ __forceinline__ float max_nan(float a, float b) {      // a NaN stays
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack_f2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack_f2(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 add_f2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul_f2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma_f2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// 16 bytes of logits as they lie in memory.
+template <typename T> struct LpVec;
+template <> struct LpVec<float> {
+  static constexpr int pairs = 2;
+  static __device__ __forceinline__ float top(const uint4& v) {
+    return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  static __device__ __forceinline__ void pair(const uint4& v, int i, float& a, float& b) {
+    a = __uint_as_float(i ? v.z : v.x);
+    b = __uint_as_float(i ? v.w : v.y);
+  }
+};
+template <> struct LpVec<__half> {
+  static constexpr int pairs = 4;
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float top(const uint4& v) {
+    const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
+    return max_nan(f.x, f.y);
+  }
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+  static __device__ __forceinline__ void pair(const uint4& v, int i, float& a, float& b) {
+    const uint32_t w = i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    a = f.x;
+    b = f.y;
+  }
+};
+template <> struct LpVec<__nv_bfloat16> {
+  static constexpr int pairs = 4;
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float top(const uint4& v) {
+    const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
+    return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+  static __device__ __forceinline__ void pair(const uint4& v, int i, float& a, float& b) {
+    const uint32_t w = i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w));
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xffff0000u);
+  }
+};
+
+// A thread's share of a row: s = sum of exp(x - m), w = sum of exp(x - m) (x - m), m the largest element (a NaN stays).
+constexpr float kFar = -1e4f;            // differences are cut here: exp is 0 there, and 0 * -inf does not arise
+struct ThreadStat {
+  float m = -INFINITY;
+  f32x2 s = 0, w = 0;                    // two sums side by side
+  __device__ __forceinline__ void move(float top) {
+    const float mn = max_nan(m, top);
+    if (mn != m) {
+      const float d = fmaxf(m - mn, kFar), f = exp2f(d * kLog2e);
+      const f32x2 ff = pack_f2(f, f);
+      w = mul_f2(fma_f2(s, pack_f2(d, d), w), ff);
+      s = mul_f2(s, ff);
+      m = mn;
+    }
+  }
+  // after move(): adds a pair of elements
+  __device__ __forceinline__ void add(float a, float b, f32x2 neg_m) {
+    float d0, d1, t0, t1;
+    unpack_f2(add_f2(pack_f2(a, b), neg_m), d0, d1);
+    const f32x2 d = pack_f2(fmaxf(d0, kFar), fmaxf(d1, kFar));
+    unpack_f2(mul_f2(d, pack_f2(kLog2e, kLog2e)), t0, t1);
+    const f32x2 e = pack_f2(exp2f(t0), exp2f(t1));
+    s = add_f2(s, e);
+    w = fma_f2(e, d, w);
+  }
+  __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
+};
 
 // Values in the order of their bits as unsigned numbers; a NaN ranks first.
 __device__ __forceinline__ uint32_t lp_order(float v) {
@@ -150,126 +226,241 @@ struct LogProbParams {
   int64_t rows;
   int cols, k;
   int64_t ignore;
+  int share;               // CTAs of a cluster that share a row
+  int part;                // elements of each one's part
 };
 
+template <typename V> __device__ __forceinline__ V lp_remote(const V* local, uint32_t rank);
+template <> __device__ __forceinline__ float lp_remote<float>(const float* local, uint32_t rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+template <> __device__ __forceinline__ uint64_t lp_remote<uint64_t>(const uint64_t* local, uint32_t rank) {
+  uint32_t at;
+  uint64_t v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void lp_cluster_sync() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
+
+constexpr int kLpThreads = 512;
+constexpr int kLpBatch = 4;              // vectors of a thread on their way at once
+
 template <typename T>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(kLpThreads, 2)
 logprob_fwd_kernel(const LogProbParams p) {
   constexpr int V = 16 / sizeof(T);
-  __shared__ RowStat red[32];
-  __shared__ uint32_t best32[32][32];
-  __shared__ uint64_t best64[32][32];
-  __shared__ uint16_t winners[1024];
+  typedef LpVec<T> L;
+  __shared__ float red_m[16], red_s[16], red_w[16];
+  __shared__ int red_n[16], red_who[16];
+  __shared__ RowStat part_stat;
+  __shared__ uint64_t best[16][32];      // lists of the warps; best[0]: of this CTA
+  __shared__ uint16_t winners[kLpThreads];
   __shared__ int nwin;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nth = blockDim.x, nw = nth >> 5;
+  const int rank = blockIdx.x % p.share;
+  const int64_t step = gridDim.x / p.share;
+  for (int64_t row = blockIdx.x / p.share; row < p.rows; row += step) {
     const T* x = static_cast<const T*>(p.x) + row * p.cols;
-    const RowCut<T> cut(x, p.cols);
-    const T* body = x + cut.head;
-    RowStat s{-INFINITY, 0.f, 0.f};
-    if (tid < cut.loose) {
-      const float v[1] = {Cvt<T>::to_f(x[cut.loose_index(tid)])};
-      rs_add(s, v);
-    }
-    for (int i = tid; i < cut.vecs; i += blockDim.x) {
-      const Vec16<T> a = ld16(body + (int64_t)i * V);
-      float v[V];
+    const int from = min(p.cols, rank * p.part), len = min(p.part, p.cols - from);
+    const T* xp = x + from;
+    const RowCut<T> cut(xp, len);
+    const uint4* body = reinterpret_cast<const uint4*>(xp + cut.head);
+    ThreadStat t;
+    float loose = -INFINITY;
+    if (tid < cut.loose) loose = Cvt<T>::to_f(xp[cut.loose_index(tid)]);
+    t.move(loose);
+    t.add(loose, -INFINITY, pack_f2(-t.base(), -t.base()));
+    for (int i0 = tid; i0 < cut.vecs; i0 += nth * kLpBatch) {
+      uint4 v[kLpBatch];
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = Cvt<T>::to_f(a.v[j]);
-      rs_add(s, v);
-    }
-    RowStat all = s;
+      for (int u = 0; u < kLpBatch; ++u) v[u] = i0 + u * nth < cut.vecs ? body[i0 + u * nth] : L::none();
+      float top = L::top(v[0]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const RowStat b{__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.r, o), __shfl_xor_sync(0xffffffffu, all.w, o)};
-      all = rs_merge(all, b);
+      for (int u = 1; u < kLpBatch; ++u) top = max_nan(top, L::top(v[u]));
+      t.move(top);
+      const f32x2 neg = pack_f2(-t.base(), -t.base());
+#pragma unroll
+      for (int u = 0; u < kLpBatch; ++u)
+#pragma unroll
+        for (int j = 0; j < L::pairs; ++j) {
+          float a, b;
+          L::pair(v[u], j, a, b);
+          t.add(a, b, neg);
+        }
     }
-    if (lane == 0) red[warp] = all;
+    // ---------------------------------------------------------------- the CTA's maximum
+    float m = t.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) red_m[warp] = m;
     uint32_t mine = 0;
     if (p.k) {
-      mine = warp_sort_desc(lp_order(s.m));
-      best32[warp][lane] = mine;
+      mine = warp_sort_desc(lp_order(t.m));
+      best[warp][lane] = mine;
     }
     if (tid == 0) nwin = 0;
     __syncthreads();
-    all = lane < nw ? red[lane] : RowStat{-INFINITY, 0.f, 0.f};
+    m = red_m[0];
+    for (int w = 1; w < nw; ++w) m = max_nan(m, red_m[w]);
+    // ---------------------------------------------------------------- its sums; whose thread holds the maximum alone
+    const bool holds = t.m == m;
+    float s0, s1, w0, w1;
+    unpack_f2(t.s, s0, s1);
+    unpack_f2(t.w, w0, w1);
+    float s = s0 + s1, w = w0 + w1;
+    {
+      const float d = m == -INFINITY ? 0.f : fmaxf(t.m - m, kFar), f = exp2f(d * kLog2e);
+      w = f * (w + d * s);
+      s *= f;
+    }
+    const uint32_t who = __ballot_sync(0xffffffffu, holds);
+    const float s_all = warp_sum(holds ? 0.f : s), w_all = warp_sum(holds ? 0.f : w);       // the others'
+    const float s_own = warp_sum(holds ? s : 0.f), w_own = warp_sum(holds ? w : 0.f);
+    if (lane == 0) { red_n[warp] = __popc(who); red_who[warp] = who ? warp * 32 + __ffs(who) - 1 : -1; red_s[warp] = s_all; red_w[warp] = w_all; }
+    __syncthreads();
+    int n = 0, holder = -1;
+    for (int q = 0; q < nw; ++q) { n += red_n[q]; if (red_who[q] >= 0) holder = red_who[q]; }
+    if (n == 1) {
+      // one thread holds the maximum: its elements again, without one of that value
+      if (warp == holder >> 5) {
+        const int h = holder;
+        float r = 0.f, wr = 0.f;
+        bool spent = false;              // some lane before has left its element out
+        auto rest = [&](float v, bool skip) {
+          if (skip) return;
+          const float d = fmaxf(v - m, kFar), e = exp2f(d * kLog2e);
+          r += e;
+          wr += e * d;
+        };
+        if (h < cut.loose) {
+          const float v = Cvt<T>::to_f(xp[cut.loose_index(h)]);
+          spent = v == m;
+          rest(v, lane != 0 || spent);
+        }
+        const int rounds = (cut.vecs - h + nth - 1) / nth;
+        for (int r0 = 0; r0 < rounds; r0 += 32) {
+          const int i = h + (r0 + lane) * nth;
+          uint4 v = L::none();
+          if (r0 + lane < rounds) v = body[i];
+          const uint32_t has = __ballot_sync(0xffffffffu, L::top(v) == m);
+          bool skip = !spent && has && lane == __ffs(has) - 1;
+          spent = spent || has;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const RowStat b{__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.r, o), __shfl_xor_sync(0xffffffffu, all.w, o)};
-      all = rs_merge(all, b);
-    }
-    const bool empty = all.m == -INFINITY && all.r == all.r;      // nothing is possible: every log probability is -inf
-    if (all.m == INFINITY) all.r = NAN;
-    const float lt = log1pf(all.r);
+          for (int j = 0; j < L::pairs; ++j) {
+            float a, b;
+            L::pair(v, j, a, b);
+            const bool sa = skip && a == m;
+            if (sa) skip = false;
+            rest(a, sa);
+            const bool sb = skip && b == m;
+            if (sb) skip = false;
+            rest(b, sb);
+          }
+        }
+        r = warp_sum(r);
+        wr = warp_sum(wr);
+        if (lane == 0) { red_s[warp] += r; red_w[warp] += wr; }
+      }
+    } else if (lane == 0) { red_s[warp] += s_own; red_w[warp] += w_own; }
+    __syncthreads();
     if (tid == 0) {
-      const int64_t t = p.tokens[row];
-      float lp;
-      if (t == p.ignore) lp = 0.f;
-      else if (t < 0 || t >= p.cols) lp = NAN;                    // no such token
-      else lp = empty ? -INFINITY : (Cvt<T>::to_f(x[t]) - all.m) - lt;
-      p.log_prob[row] = lp;
-      const float ent = empty ? 0.f : lt + all.w / (1.f + all.r);
-      p.entropy[row] = ent;
-      if (p.stat) { p.stat[3 * row] = all.m; p.stat[3 * row + 1] = lt; p.stat[3 * row + 2] = ent; }
+      float r = 0.f, wr = 0.f;
+      for (int q = 0; q < nw; ++q) { r += red_s[q]; wr += red_w[q]; }
+      if (n != 1) r -= 1.f;
+      RowStat st{m, r, -wr};
+      if (m == -INFINITY) st = {-INFINITY, 0.f, 0.f};
+      if (m != m || m == INFINITY) st = {INFINITY, NAN, NAN};
+      part_stat = st;
     }
+    // ---------------------------------------------------------------- the CTA's most probable elements
     if (p.k) {
       for (int half = 1; half < nw; half <<= 1) {
         if ((warp & (2 * half - 1)) == 0 && warp + half < nw) {
-          mine = warp_merge_desc(mine, best32[warp + half][lane]);
-          best32[warp][lane] = mine;
+          mine = warp_merge_desc(mine, (uint32_t)best[warp + half][lane]);
+          best[warp][lane] = mine;
         }
         __syncthreads();
       }
-      uint32_t bound = best32[0][p.k - 1];
-      if (all.r != all.r) bound = 0;                              // a NaN somewhere: look at everything
-      if (lp_order(s.m) >= bound) winners[atomicAdd(&nwin, 1)] = (uint16_t)tid;
+      uint32_t bound = (uint32_t)best[0][p.k - 1];
+      if (m != m) bound = 0;                                      // a NaN somewhere: look at everything
+      if (lp_order(t.m) >= bound || bound == 0) winners[atomicAdd(&nwin, 1)] = (uint16_t)tid;
       __syncthreads();
       uint64_t list = 0;
-      const int n = nwin;
-      for (int wi = warp; wi < n; wi += nw) {
-        const int who = winners[wi];
+      const int nwinners = nwin;
+      for (int wi = warp; wi < nwinners; wi += nw) {
+        const int h = winners[wi];
         {
           uint64_t key = 0;
-          if (lane == 0 && who < cut.loose) {
-            const int c = cut.loose_index(who);
-            const float v = Cvt<T>::to_f(x[c]);
-            if (lp_order(v) >= bound) key = lp_key(v, (uint32_t)c);
+          if (lane == 0 && h < cut.loose) {
+            const int c = cut.loose_index(h);
+            const float v = Cvt<T>::to_f(xp[c]);
+            if (lp_order(v) >= bound) key = lp_key(v, (uint32_t)(from + c));
           }
           warp_insert(list, key, p.k);
         }
-        const int rounds = (cut.vecs - who + (int)blockDim.x - 1) / (int)blockDim.x;    // vectors of that thread
+        const int rounds = (cut.vecs - h + nth - 1) / nth;        // vectors of that thread
         for (int r0 = 0; r0 < rounds; r0 += 32) {
-          const int i = who + (r0 + lane) * (int)blockDim.x;
+          const int i = h + (r0 + lane) * nth;
           const bool in = r0 + lane < rounds;
-          Vec16<T> a;
-          if (in) a = ld16(body + (int64_t)i * V);
+          uint4 v = L::none();
+          if (in) v = body[i];
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            uint64_t key = 0;
-            if (in) {
-              const float v = Cvt<T>::to_f(a.v[j]);
-              if (lp_order(v) >= bound) key = lp_key(v, (uint32_t)(cut.head + i * V + j));
-            }
-            warp_insert(list, key, p.k);
+          for (int j = 0; j < L::pairs; ++j) {
+            float a, b;
+            L::pair(v, j, a, b);
+            const uint32_t at = (uint32_t)(from + cut.head + i * V + 2 * j);
+            warp_insert(list, in && lp_order(a) >= bound ? lp_key(a, at) : 0, p.k);
+            warp_insert(list, in && lp_order(b) >= bound ? lp_key(b, at + 1) : 0, p.k);
           }
         }
       }
-      best64[warp][lane] = list;
+      __syncthreads();                                            // everyone has read the bound
+      best[warp][lane] = list;
       __syncthreads();
       for (int half = 1; half < nw; half <<= 1) {
         if ((warp & (2 * half - 1)) == 0 && warp + half < nw) {
-          list = warp_merge_desc(list, best64[warp + half][lane]);
-          best64[warp][lane] = list;
+          list = warp_merge_desc(list, best[warp + half][lane]);
+          best[warp][lane] = list;
         }
         __syncthreads();
       }
-      if (warp == 0 && lane < p.k) {
+    }
+    // ---------------------------------------------------------------- the row's results
+    if (p.share > 1) lp_cluster_sync();
+    else __syncthreads();
+    if (rank == 0 && warp == 0) {
+      RowStat all = part_stat;
+      uint64_t list = best[0][lane];
+      for (int c = 1; c < p.share; ++c) {
+        all = rs_merge(all, {lp_remote(&part_stat.m, c), lp_remote(&part_stat.r, c), lp_remote(&part_stat.w, c)});
+        if (p.k) list = warp_merge_desc(list, lp_remote(&best[0][lane], c));
+      }
+      const bool empty = all.m == -INFINITY;                      // nothing is possible: every log probability is -inf
+      const float lt = log1pf(all.r);
+      if (lane == 0) {
+        const int64_t tok = p.tokens[row];
+        float lp;
+        if (tok == p.ignore) lp = 0.f;
+        else if (tok < 0 || tok >= p.cols) lp = NAN;              // no such token
+        else lp = empty ? -INFINITY : (Cvt<T>::to_f(x[tok]) - all.m) - lt;
+        p.log_prob[row] = lp;
+        const float ent = empty ? 0.f : lt + all.w / (1.f + all.r);
+        p.entropy[row] = ent;
+        if (p.stat) { p.stat[3 * row] = all.m; p.stat[3 * row + 1] = lt; p.stat[3 * row + 2] = ent; }
+      }
+      if (lane < p.k) {
         const float v = lp_value(list);
         p.top_lp[row * p.k + lane] = empty ? -INFINITY : (v - all.m) - lt;
         p.top_id[row * p.k + lane] = (int64_t)(uint32_t)~(uint32_t)list;
       }
     }
-    __syncthreads();                                              // the shared lists belong to the next row now
+    if (p.share > 1) lp_cluster_sync();                           // the shared lists belong to the next row now
+    else __syncthreads();
   }
 }
 
@@ -346,8 +537,29 @@ logprob_bwd_kernel(const LogProbGradParams p) {
 inline int lp_threads(int cols, int size) {
   const int64_t want = ((int64_t)cols * size + 63) / 64;          // four 16-byte vectors of each thread, while the block grows
   int t = 32;
-  while (t < 512 && t < want) t <<= 1;
+  while (t < kLpThreads && t < want) t <<= 1;
   return t;
+}
+
+template <typename T>
+static int logprob_forward(LogProbParams p, cudaStream_t st) {
+  // Rows are shared while that fills no more than two CTAs on every SM and leaves each CTA 16 KB (a part with less has too little
+  // to read for the joins it causes).
+  p.share = 1;
+  while (p.share < 8 && p.rows * p.share * 2 <= 2 * sm_count() && (int64_t)p.cols * sizeof(T) / (p.share * 2) >= 16384) p.share <<= 1;
+  p.part = p.share == 1 ? p.cols : ((p.cols + p.share - 1) / p.share + 63) / 64 * 64;
+  const int64_t cap = (int64_t)sm_count() * 64;
+  const int64_t rows = p.rows < cap ? p.rows : cap;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(rows * p.share));
+  cfg.blockDim = dim3(lp_threads(p.part, sizeof(T)));
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = p.share; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = p.share > 1 ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, logprob_fwd_kernel<T>, p);
 }
 
 }  // namespace mxb
@@ -358,15 +570,12 @@ using namespace mxb;
 MXB_EXPORT int mxb_logprob_forward(int dtype, const void* x, const int64_t* tokens, float* log_prob, float* entropy, float* top_lp,
                                    int64_t* top_id, float* stat, int64_t rows, int cols, int k, int64_t ignore, void* stream) {
   if (rows < 1 || cols < 1 || k < 0 || k > kLpMaxTop || k > cols) return -2;
-  LogProbParams p{x, tokens, log_prob, entropy, top_lp, top_id, stat, rows, cols, k, ignore};
+  LogProbParams p{x, tokens, log_prob, entropy, top_lp, top_id, stat, rows, cols, k, ignore, 1, cols};
   cudaStream_t st = (cudaStream_t)stream;
-  const int64_t cap = (int64_t)sm_count() * 64;
-  const unsigned grid = (unsigned)(rows < cap ? rows : cap);
-  if (dtype == kF32) logprob_fwd_kernel<float><<<grid, lp_threads(cols, 4), 0, st>>>(p);
-  else if (dtype == kF16) logprob_fwd_kernel<__half><<<grid, lp_threads(cols, 2), 0, st>>>(p);
-  else if (dtype == kBF16) logprob_fwd_kernel<__nv_bfloat16><<<grid, lp_threads(cols, 2), 0, st>>>(p);
-  else return -1;
-  return (int)cudaGetLastError();
+  if (dtype == kF32) return logprob_forward<float>(p, st);
+  if (dtype == kF16) return logprob_forward<__half>(p, st);
+  if (dtype == kBF16) return logprob_forward<__nv_bfloat16>(p, st);
+  return -1;
 }
 
 // dx: [rows, cols] of the logits' type; g_lp, g_ent: [rows] floats, g_top: [rows, k] floats (each may be null).
