@@ -256,7 +256,7 @@ logprob_fwd_kernel(const LogProbParams p) {
   constexpr int V = 16 / sizeof(T);
   typedef LpVec<T> L;
   __shared__ float red_m[16], red_s[16], red_w[16];
-  __shared__ int red_n[16], red_who[16];
+  __shared__ int holders, holder;        // threads that hold the maximum, one of them
   __shared__ RowStat part_stat;
   __shared__ uint64_t best[16][32];      // lists of the warps; best[0]: of this CTA
   __shared__ uint16_t winners[kLpThreads];
@@ -285,13 +285,15 @@ logprob_fwd_kernel(const LogProbParams p) {
       t.move(top);
       const f32x2 neg = pack_f2(-t.base(), -t.base());
 #pragma unroll
-      for (int u = 0; u < kLpBatch; ++u)
+      for (int u = 0; u < kLpBatch; ++u) {
+        if (i0 + u * nth >= cut.vecs) break;
 #pragma unroll
         for (int j = 0; j < L::pairs; ++j) {
           float a, b;
           L::pair(v[u], j, a, b);
           t.add(a, b, neg);
         }
+      }
     }
     // ---------------------------------------------------------------- the CTA's maximum
     float m = t.m;
@@ -303,10 +305,11 @@ logprob_fwd_kernel(const LogProbParams p) {
       mine = warp_sort_desc(lp_order(t.m));
       best[warp][lane] = mine;
     }
-    if (tid == 0) nwin = 0;
+    if (tid == 0) { nwin = 0; holders = 0; }
     __syncthreads();
-    m = red_m[0];
-    for (int w = 1; w < nw; ++w) m = max_nan(m, red_m[w]);
+    m = red_m[lane < nw ? lane : 0];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     // ---------------------------------------------------------------- its sums; whose thread holds the maximum alone
     const bool holds = t.m == m;
     float s0, s1, w0, w1;
@@ -318,13 +321,11 @@ logprob_fwd_kernel(const LogProbParams p) {
       w = f * (w + d * s);
       s *= f;
     }
-    const uint32_t who = __ballot_sync(0xffffffffu, holds);
     const float s_all = warp_sum(holds ? 0.f : s), w_all = warp_sum(holds ? 0.f : w);       // the others'
-    const float s_own = warp_sum(holds ? s : 0.f), w_own = warp_sum(holds ? w : 0.f);
-    if (lane == 0) { red_n[warp] = __popc(who); red_who[warp] = who ? warp * 32 + __ffs(who) - 1 : -1; red_s[warp] = s_all; red_w[warp] = w_all; }
+    if (lane == 0) { red_s[warp] = s_all; red_w[warp] = w_all; }
+    if (holds) { atomicAdd(&holders, 1); holder = tid; }          // with several holders any of them will do: it is not used then
     __syncthreads();
-    int n = 0, holder = -1;
-    for (int q = 0; q < nw; ++q) { n += red_n[q]; if (red_who[q] >= 0) holder = red_who[q]; }
+    const int n = holders;
     if (n == 1) {
       // one thread holds the maximum: its elements again, without one of that value
       if (warp == holder >> 5) {
@@ -366,16 +367,19 @@ logprob_fwd_kernel(const LogProbParams p) {
         wr = warp_sum(wr);
         if (lane == 0) { red_s[warp] += r; red_w[warp] += wr; }
       }
-    } else if (lane == 0) { red_s[warp] += s_own; red_w[warp] += w_own; }
+    } else {
+      const float s_own = warp_sum(holds ? s : 0.f), w_own = warp_sum(holds ? w : 0.f);
+      if (lane == 0) { red_s[warp] += s_own; red_w[warp] += w_own; }
+    }
     __syncthreads();
-    if (tid == 0) {
-      float r = 0.f, wr = 0.f;
-      for (int q = 0; q < nw; ++q) { r += red_s[q]; wr += red_w[q]; }
+    if (warp == 0) {
+      float r = warp_sum(lane < nw ? red_s[lane] : 0.f);
+      const float wr = warp_sum(lane < nw ? red_w[lane] : 0.f);
       if (n != 1) r -= 1.f;
       RowStat st{m, r, -wr};
       if (m == -INFINITY) st = {-INFINITY, 0.f, 0.f};
       if (m != m || m == INFINITY) st = {INFINITY, NAN, NAN};
-      part_stat = st;
+      if (lane == 0) part_stat = st;
     }
     // ---------------------------------------------------------------- the CTA's most probable elements
     if (p.k) {
@@ -534,10 +538,10 @@ logprob_bwd_kernel(const LogProbGradParams p) {
   }
 }
 
-inline int lp_threads(int cols, int size) {
+inline int lp_threads(int cols, int size, int most) {
   const int64_t want = ((int64_t)cols * size + 63) / 64;          // four 16-byte vectors of each thread, while the block grows
   int t = 32;
-  while (t < kLpThreads && t < want) t <<= 1;
+  while (t < most && t < want) t <<= 1;
   return t;
 }
 
@@ -552,7 +556,8 @@ static int logprob_forward(LogProbParams p, cudaStream_t st) {
   const int64_t rows = p.rows < cap ? p.rows : cap;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * p.share));
-  cfg.blockDim = dim3(lp_threads(p.part, sizeof(T)));
+  // blocks of 256 threads: their joins and rescans overlap with other blocks' reading; 512 where one block is all an SM gets
+  cfg.blockDim = dim3(lp_threads(p.part, sizeof(T), rows * p.share <= sm_count() ? kLpThreads : 256));
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -587,9 +592,9 @@ MXB_EXPORT int mxb_logprob_backward(int dtype, const void* x, void* dx, const in
   cudaStream_t st = (cudaStream_t)stream;
   const int64_t cap = (int64_t)sm_count() * 64;
   const unsigned grid = (unsigned)(rows < cap ? rows : cap);
-  if (dtype == kF32) logprob_bwd_kernel<float><<<grid, lp_threads(cols, 4), 0, st>>>(p);
-  else if (dtype == kF16) logprob_bwd_kernel<__half><<<grid, lp_threads(cols, 2), 0, st>>>(p);
-  else if (dtype == kBF16) logprob_bwd_kernel<__nv_bfloat16><<<grid, lp_threads(cols, 2), 0, st>>>(p);
+  if (dtype == kF32) logprob_bwd_kernel<float><<<grid, lp_threads(cols, 4, kLpThreads), 0, st>>>(p);
+  else if (dtype == kF16) logprob_bwd_kernel<__half><<<grid, lp_threads(cols, 2, kLpThreads), 0, st>>>(p);
+  else if (dtype == kBF16) logprob_bwd_kernel<__nv_bfloat16><<<grid, lp_threads(cols, 2, kLpThreads), 0, st>>>(p);
   else return -1;
   return (int)cudaGetLastError();
 }
