@@ -54,6 +54,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 struct TcParams {
   const int* valid;
   const void* o;                         // backward: forward output, contiguous [B, T, Hq, D]
@@ -330,7 +336,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(x[c]));
+      for (int c = 0; c < 128; c += 2) mx[c >> 1 & 3] = max3(mx[c >> 1 & 3], __uint_as_float(x[c]), __uint_as_float(x[c + 1]));
       const float mt = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc);
       const bool move = mt > m + kMaxLag || m == -INFINITY;
       if (__any_sync(0xffffffffu, move)) {
@@ -352,21 +358,25 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
       first = false;
       const float off = kPShift - (m == -INFINITY ? 0.f : m);
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      const f32x2 sc2 = pack_f2(sc, sc), off2 = pack_f2(off, off);
+      f32x2 part[2] = {0, 0};
 #pragma unroll
       for (int c0 = 0; c0 < 128; c0 += 32) {
         uint32_t pk[16];
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
-          const float e0 = ex2(fmaf(__uint_as_float(x[c0 + c]), sc, off));
-          const float e1 = ex2(fmaf(__uint_as_float(x[c0 + c + 1]), sc, off));
-          part[c & 2] += e0;
-          part[(c & 2) + 1] += e1;
+          float e0, e1;
+          unpack_f2(fma_f2(pack_f2(__uint_as_float(x[c0 + c]), __uint_as_float(x[c0 + c + 1])), sc2, off2), e0, e1);
+          e0 = ex2(e0);
+          e1 = ex2(e1);
+          part[c >> 1 & 1] = add_f2(part[c >> 1 & 1], pack_f2(e0, e1));
           pk[c >> 1] = pack2<T>(e0, e1);
         }
         tmem_st16(ts + (c0 >> 1), pk);
       }
-      l += (part[0] + part[1]) + (part[2] + part[3]);
+      float l0, l1;
+      unpack_f2(add_f2(part[0], part[1]), l0, l1);
+      l += l0 + l1;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
