@@ -112,20 +112,31 @@ __device__ __forceinline__ void tc_clear_rows(uint8_t* tile, int from) {
   fence_async_smem();
   __syncwarp();
 }
-// S[128, 128] = A B^T over D channels, both tiles row by row in shared memory.
+// One lane of a converged warp.  The warps that issue MMAs run their loops as a whole and elect a lane only around the
+// instructions: their operands then stay in uniform registers, where an issue inside a one-lane branch moves each of them there
+// every time (80 cycles for an MMA instead of its 45).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ int warp_uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// S[128, 128] = A B^T over D channels, both tiles row by row in shared memory (descriptors of their first boxes).
 template <int D>
-__device__ __forceinline__ void tc_scores(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc) {
+__device__ __forceinline__ void tc_scores(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc) {
 #pragma unroll
   for (int k = 0; k < D / 16; ++k) {
-    const uint32_t o = (uint32_t)(k >> 2) * kTcHalf;
-    umma(tmem_d, make_desc(a + o) + 2 * (k & 3), make_desc(b + o) + 2 * (k & 3), idesc, k > 0 ? 1u : 0u);
+    const uint64_t o = (uint64_t)((k >> 2) * (kTcHalf >> 4) + 2 * (k & 3));
+    umma(tmem_d, a + o, b + o, idesc, k > 0 ? 1u : 0u);
   }
 }
-// O[128, D] (+)= P[128, 128] V[128, D], P in TMEM (two values to a column), V row by row in shared memory.
-__device__ __forceinline__ void tc_accumulate(uint32_t tmem_d, uint32_t tmem_p, uint32_t v, uint32_t idesc, uint32_t carry) {
+// O[128, D] (+)= P[128, 128] V[128, D], P in TMEM (two values to a column; its second half `split` columns behind the first),
+// V row by row in shared memory.
+__device__ __forceinline__ void tc_accumulate(uint32_t tmem_d, uint32_t tmem_p, uint32_t split, uint64_t v, uint32_t idesc, uint32_t carry) {
 #pragma unroll
   for (int k = 0; k < 8; ++k)
-    umma_ts(tmem_d, tmem_p + 8 * k, make_desc_mn(v + (uint32_t)k * 2048u, kTcHalf), idesc, k > 0 ? 1u : carry);
+    umma_ts(tmem_d, tmem_p + (k < 4 ? 8 * k : split + 8 * (k - 4)), v + (uint64_t)k * 128u, idesc, k > 0 ? 1u : carry);
 }
 
 __device__ __forceinline__ void tc_finish(uint32_t tmem_base, uint32_t cols, int warp, int alloc_warp, volatile int* abort_flag, int* error_flag) {
@@ -173,7 +184,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
            *p_full = bars + 12, *o_full = bars + 14, *patch = bars + 15, *drain = bars + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   // the last tiles of causal attention are the longest: they start first
   const int tiles = p.T / kTcRows + (p.T % kTcRows ? 1 : 0);
@@ -181,7 +192,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int qb = qblocks - 1 - (int)(blockIdx.x / p.items), item = blockIdx.x % p.items;
   const int hcount = p.qpair ? p.Hq / 2 : p.Hq;
   const int b = item / hcount, h0 = (item % hcount) * (p.qpair ? 2 : 1), hk = h0 / (p.Hq / p.Hk);
-  const int n = tc_valid(p, b);
+  const int n = warp_uniform(tc_valid(p, b));
   const int qa = p.qpair ? qb * kTcRows : qb * 2 * kTcRows;
   const int qstep = p.qpair ? 0 : kTcRows, hstep = p.qpair ? 1 : 0;
   const KeyRange r0(qa, n, p.window, p.sinks), r1(qa + qstep, n, p.window, p.sinks);
@@ -203,7 +214,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = warp_uniform(*tmem_slot);
 
   if (warp == 9) {
     // ---------------------------------------------------------------- loads
@@ -255,51 +266,54 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
   } else if (warp == 8) {
     // ---------------------------------------------------------------- products
-    if (lane == 0 && ntiles > 0) {
+    if (ntiles > 0) {
       const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
-      const uint32_t sq = smem_u32(smem + L::q), sk = smem_u32(smem + L::k), sv = smem_u32(smem + L::v);
+      const uint64_t dq = make_desc(smem_u32(smem + L::q)), dk = make_desc(smem_u32(smem + L::k)),
+                     dv = make_desc_mn(smem_u32(smem + L::v), kTcHalf);
+      constexpr uint64_t step = L::tile >> 4;
       bool ok = true;
-      uint32_t pphase[2] = {0, 0}, started[2] = {0, 0};
+      uint32_t pphase = 0, started = 0;                           // bit s: of query tile s
       for (int s = 0; s < 2 && ok; ++s) {
         const KeyRange& r = s ? r1 : r0;
         if (r.count() == 0) continue;
-        ok = mbar_wait(&q_full[s], 0);
+        ok = mbar_wait_warp(&q_full[s], 0);
         if (ok && r.has(key_tile(0))) {
-          ok = mbar_wait(&k_full[0], 0);
+          ok = mbar_wait_warp(&k_full[0], 0);
           tc_fence_after();
-          if (ok) { tc_scores<D>(tmem + 128 * s, sq + s * L::tile, sk, id_s); umma_commit(&s_full[s]); }
+          if (ok && elect_one()) { tc_scores<D>(tmem + 128 * s, dq + s * step, dk, id_s); umma_commit(&s_full[s]); }
         }
       }
-      umma_commit(&k_empty[0]);
+      if (elect_one()) umma_commit(&k_empty[0]);
       for (int j = 0; j < ntiles && ok; ++j) {
         const int kt = key_tile(j), next = j + 1 < ntiles ? key_tile(j + 1) : -1;
         const int st = j % kFwdStages, sn = (j + 1) % kFwdStages;
         const uint32_t ph = (uint32_t)(j / kFwdStages) & 1u, pn = (uint32_t)((j + 1) / kFwdStages) & 1u;
-        for (int s = 0; s < 2 && ok; ++s) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
           const KeyRange& r = s ? r1 : r0;
-          if (r.has(kt)) {
-            ok = mbar_wait(&v_full[st], ph) && mbar_wait(&p_full[s], pphase[s]);
-            if (!ok) break;
-            pphase[s] ^= 1u;
+          if (ok && r.has(kt)) {
+            ok = mbar_wait_warp(&v_full[st], ph) && mbar_wait_warp(&p_full[s], pphase >> s & 1u);
+            pphase ^= 1u << s;
             tc_fence_after();
-            tc_accumulate(tmem + 256 + D * s, tmem + 128 * s, sv + st * L::tile, id_o, started[s]);
-            started[s] = 1u;
+            if (ok && elect_one()) tc_accumulate(tmem + 256 + D * s, tmem + 128 * s, 32, dv + st * step, id_o, started >> s & 1u);
+            started |= 1u << s;
           }
-          if (next >= 0 && r.has(next)) {
-            ok = mbar_wait(&k_full[sn], pn);
-            if (!ok) break;
+          if (ok && next >= 0 && r.has(next)) {
+            ok = mbar_wait_warp(&k_full[sn], pn);
             tc_fence_after();
-            tc_scores<D>(tmem + 128 * s, sq + s * L::tile, sk + sn * L::tile, id_s);
-            umma_commit(&s_full[s]);                              // complete only after P V of this tile, issued before it
+            if (ok && elect_one()) {
+              tc_scores<D>(tmem + 128 * s, dq + s * step, dk + sn * step, id_s);
+              umma_commit(&s_full[s]);                            // complete only after P V of this tile, issued before it
+            }
           }
         }
-        if (ok) {
+        if (ok && elect_one()) {
           umma_commit(&v_empty[st]);
           if (next >= 0) umma_commit(&k_empty[sn]);
         }
       }
-      if (ok) umma_commit(o_full);
-      else { *abort_flag = 1; umma_commit(drain); mbar_wait(drain, 0); }
+      if (elect_one()) umma_commit(ok ? o_full : drain);
+      if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
     }
   } else {
     // ---------------------------------------------------------------- softmax

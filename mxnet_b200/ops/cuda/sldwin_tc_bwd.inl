@@ -40,12 +40,12 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
            *dp_empty = bars + 12, *ds_full = bars + 13, *done = bars + 14, *patch = bars + 15, *drain = bars + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   const int tiles = p.T / kTcRows + (p.T % kTcRows ? 1 : 0);
   const int qt = tiles - 1 - (int)(blockIdx.x / p.items), item = blockIdx.x % p.items;
   const int b = item / p.Hq, h = item % p.Hq, hk = h / (p.Hq / p.Hk);
-  const int n = tc_valid(p, b);
+  const int n = warp_uniform(tc_valid(p, b));
   const int q0 = qt * kTcRows;
   const KeyRange r(q0, n, p.window, p.sinks);
   const int ntiles = r.count();
@@ -63,7 +63,7 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = warp_uniform(*tmem_slot);
   constexpr uint32_t kDp = 256, kDq = 384;
 
   if (warp == 9) {
@@ -108,41 +108,46 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
     }
   } else if (warp == 8) {
-    if (lane == 0 && ntiles > 0) {
+    if (ntiles > 0) {
       const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
-      const uint32_t sq = smem_u32(smem + L::q), sg = smem_u32(smem + L::g), sk = smem_u32(smem + L::k), sv = smem_u32(smem + L::v);
-      bool ok = mbar_wait(qg_full, 0);
+      const uint64_t dq = make_desc(smem_u32(smem + L::q)), dg = make_desc(smem_u32(smem + L::g)), dk = make_desc(smem_u32(smem + L::k)),
+                     dv = make_desc(smem_u32(smem + L::v)), dkm = make_desc_mn(smem_u32(smem + L::k), kTcHalf);
+      constexpr uint64_t step = L::tile >> 4;
+      bool ok = mbar_wait_warp(qg_full, 0);
       auto scores = [&](int j) {
-        ok = mbar_wait(&k_full[j % L::kst], (uint32_t)(j / L::kst) & 1u);
+        ok = mbar_wait_warp(&k_full[j % L::kst], (uint32_t)(j / L::kst) & 1u);
         tc_fence_after();
-        if (ok) tc_scores<D>(tmem + 128 * (j & 1), sq, sk + (j % L::kst) * L::tile, id_s);
+        if (ok && elect_one()) tc_scores<D>(tmem + 128 * (j & 1), dq, dk + (j % L::kst) * step, id_s);
       };
       auto dprobs = [&](int j) {
-        ok = mbar_wait(&v_full[j % L::vst], (uint32_t)(j / L::vst) & 1u);
+        ok = mbar_wait_warp(&v_full[j % L::vst], (uint32_t)(j / L::vst) & 1u);
         tc_fence_after();
-        if (ok) { tc_scores<D>(tmem + kDp, sg, sv + (j % L::vst) * L::tile, id_s); umma_commit(sd_full); umma_commit(&v_empty[j % L::vst]); }
+        if (ok && elect_one()) {
+          tc_scores<D>(tmem + kDp, dg, dv + (j % L::vst) * step, id_s);
+          umma_commit(sd_full);
+          umma_commit(&v_empty[j % L::vst]);
+        }
       };
       if (ok) scores(0);
       if (ok) dprobs(0);
       if (ok && ntiles > 1) scores(1);
       for (int j = 0; j < ntiles && ok; ++j) {
         if (j + 1 < ntiles) {
-          ok = mbar_wait(dp_empty, (uint32_t)j & 1u);             // dP of this tile is in registers
+          ok = mbar_wait_warp(dp_empty, (uint32_t)j & 1u);        // dP of this tile is in registers
           if (ok) dprobs(j + 1);
           if (!ok) break;
         }
-        ok = mbar_wait(ds_full, (uint32_t)j & 1u);
+        ok = mbar_wait_warp(ds_full, (uint32_t)j & 1u);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t ds = tmem + 128 * (j & 1), kt = sk + (j % L::kst) * L::tile;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_ts(tmem + kDq, ds + (k < 4 ? 8 * k : 64 + 8 * (k - 4)), make_desc_mn(kt + (uint32_t)k * 2048u, kTcHalf), id_o, (j > 0 || k > 0) ? 1u : 0u);
-        umma_commit(&k_empty[j % L::kst]);
+        if (elect_one()) {
+          tc_accumulate(tmem + kDq, tmem + 128 * (j & 1), 64, dkm + (j % L::kst) * step, id_o, j > 0 ? 1u : 0u);
+          umma_commit(&k_empty[j % L::kst]);
+        }
         if (j + 2 < ntiles) scores(j + 2);                        // over S and dS of this tile, read by the product before it
       }
-      if (ok) umma_commit(done);
-      else { *abort_flag = 1; umma_commit(drain); mbar_wait(drain, 0); }
+      if (elect_one()) umma_commit(ok ? done : drain);
+      if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
     }
   } else {
     const int half = warp >> 2, quad = warp & 3;
@@ -314,7 +319,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* s_factor = reinterpret_cast<float*>(tmem_slot + 2);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   if (smem_u32(smem) & 1023u) {                                    // swizzled tiles lie on 1024-byte boundaries
     if (threadIdx.x == 0 && p.error_flag) *static_cast<volatile int*>(p.error_flag) = 1;
@@ -326,7 +331,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const bool far = unit >= sp.tiles;
   const int kt = far ? (unit - sp.tiles) % sp.sink_tiles : unit;
   const int chunk = far ? (unit - sp.tiles) / sp.sink_tiles : 0;
-  const int n = tc_valid(p, b);
+  const int n = warp_uniform(tc_valid(p, b));
   const int k0 = kt * kTcRows;
   const int last_tile = n > 0 ? (n - 1) / kTcRows : -1;
   const int qlo = far ? kt + sp.near_span + 1 + chunk * (sp.near_span + 1) : kt;
@@ -347,7 +352,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = warp_uniform(*tmem_slot);
   constexpr uint32_t kDp = 128, kDv = 256, kDk = 256 + D;
 
   if (warp == 9) {
@@ -421,44 +426,46 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
     }
   } else if (warp == 8) {
-    if (lane == 0 && nit > 0) {
+    if (nit > 0) {
       const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
-      const uint32_t sk = smem_u32(smem + L::k), sv = smem_u32(smem + L::v), sq = smem_u32(smem + L::q), sg = smem_u32(smem + L::g);
-      bool ok = mbar_wait(kv_full, 0);
+      const uint64_t dk = make_desc(smem_u32(smem + L::k)), dv = make_desc(smem_u32(smem + L::v)), dq = make_desc(smem_u32(smem + L::q)),
+                     dg = make_desc(smem_u32(smem + L::g)), dqm = make_desc_mn(smem_u32(smem + L::q), kTcHalf),
+                     dgm = make_desc_mn(smem_u32(smem + L::g), kTcHalf);
+      constexpr uint64_t step = L::tile >> 4;
+      bool ok = mbar_wait_warp(kv_full, 0);
       auto scores = [&](int it) {
-        ok = mbar_wait(&q_full[it % L::qst], (uint32_t)(it / L::qst) & 1u);
+        ok = mbar_wait_warp(&q_full[it % L::qst], (uint32_t)(it / L::qst) & 1u);
         tc_fence_after();
-        if (ok) { tc_scores<D>(tmem, sk, sq + (it % L::qst) * L::tile, id_s); umma_commit(s_full); }
+        if (ok && elect_one()) { tc_scores<D>(tmem, dk, dq + (it % L::qst) * step, id_s); umma_commit(s_full); }
       };
       auto dprobs = [&](int it) {
-        ok = mbar_wait(&g_full[it % L::gst], (uint32_t)(it / L::gst) & 1u);
+        ok = mbar_wait_warp(&g_full[it % L::gst], (uint32_t)(it / L::gst) & 1u);
         tc_fence_after();
-        if (ok) { tc_scores<D>(tmem + kDp, sv, sg + (it % L::gst) * L::tile, id_s); umma_commit(dp_full); }
-      };
-      auto add = [&](uint32_t acc, uint32_t a, uint32_t tile, bool carry) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_ts(tmem + acc, a + (k < 4 ? 8 * k : 64 + 8 * (k - 4)), make_desc_mn(tile + (uint32_t)k * 2048u, kTcHalf), id_o, (carry || k > 0) ? 1u : 0u);
+        if (ok && elect_one()) { tc_scores<D>(tmem + kDp, dv, dg + (it % L::gst) * step, id_s); umma_commit(dp_full); }
       };
       if (ok) scores(0);
       if (ok) dprobs(0);
       for (int it = 0; it < nit && ok; ++it) {
-        ok = mbar_wait(p_ready, (uint32_t)it & 1u);
+        ok = mbar_wait_warp(p_ready, (uint32_t)it & 1u);
         if (!ok) break;
         tc_fence_after();
-        add(kDv, tmem, sg + (it % L::gst) * L::tile, it > 0);
-        umma_commit(&g_empty[it % L::gst]);                       // dP of this tile was issued before: dO is done with
+        if (elect_one()) {
+          tc_accumulate(tmem + kDv, tmem, 64, dgm + (it % L::gst) * step, id_o, it > 0 ? 1u : 0u);
+          umma_commit(&g_empty[it % L::gst]);                     // dP of this tile was issued before: dO is done with
+        }
         if (it + 1 < nit) scores(it + 1);
         if (!ok) break;
-        ok = mbar_wait(ds_ready, (uint32_t)it & 1u);
+        ok = mbar_wait_warp(ds_ready, (uint32_t)it & 1u);
         if (!ok) break;
         tc_fence_after();
-        add(kDk, tmem + kDp, sq + (it % L::qst) * L::tile, it > 0);
-        umma_commit(&q_empty[it % L::qst]);
+        if (elect_one()) {
+          tc_accumulate(tmem + kDk, tmem + kDp, 64, dqm + (it % L::qst) * step, id_o, it > 0 ? 1u : 0u);
+          umma_commit(&q_empty[it % L::qst]);
+        }
         if (it + 1 < nit) dprobs(it + 1);
       }
-      if (ok) umma_commit(done);
-      else { *abort_flag = 1; umma_commit(drain); mbar_wait(drain, 0); }
+      if (elect_one()) umma_commit(ok ? done : drain);
+      if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
     }
   } else {
     const int half = warp >> 2, quad = warp & 3;
