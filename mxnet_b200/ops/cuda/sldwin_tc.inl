@@ -60,6 +60,23 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// 2^x on the fp32 pipes, for x <= 2^6: n + f with f in [-1/2, 1/2], 2^f by the degree-4 polynomial of least relative error (3e-6,
+// far below the half step of P's type), n added to the exponent.  Arguments are cut at -126.
+constexpr float kRoundMagic = 12582912.f;                 // 1.5 * 2^23: adding it rounds to a whole number in the low bits
+__device__ __forceinline__ f32x2 exp2_poly(float a, float b) {
+  const f32x2 x = pack_f2(fmaxf(a, -126.f), fmaxf(b, -126.f)), magic = pack_f2(kRoundMagic, kRoundMagic);
+  const f32x2 n = add_f2(x, magic);
+  const f32x2 f = add_f2(x, mul_f2(add_f2(n, pack_f2(-kRoundMagic, -kRoundMagic)), pack_f2(-1.f, -1.f)));
+  f32x2 y = fma_f2(f, pack_f2(0.009570102f, 0.009570102f), pack_f2(0.055917863f, 0.055917863f));
+  y = fma_f2(y, f, pack_f2(0.24024744f, 0.24024744f));
+  y = fma_f2(y, f, pack_f2(0.6931218f, 0.6931218f));
+  y = fma_f2(y, f, pack_f2(0.9999993f, 0.9999993f));
+  float y0, y1, n0, n1;
+  unpack_f2(y, y0, y1);
+  unpack_f2(n, n0, n1);
+  return pack_f2(__uint_as_float(__float_as_uint(y0) + (__float_as_uint(n0) << 23)), __uint_as_float(__float_as_uint(y1) + (__float_as_uint(n1) << 23)));
+}
+
 struct TcParams {
   const int* valid;
   const void* o;                         // backward: forward output, contiguous [B, T, Hq, D]
@@ -95,6 +112,11 @@ struct KeyRange {
   __device__ __forceinline__ bool has(int kt) const { return kt <= hi && (kt >= lo || kt < ns); }
   __device__ __forceinline__ int count() const { return hi < lo ? 0 : ns + hi - lo + 1; }
 };
+
+// Bits of 32 neighbouring keys that a query sees: keys up to `hi`, of them those behind `gone` and those up to `sink` (indexes
+// relative to the first of the 32).
+__device__ __forceinline__ uint32_t tc_upto(int last) { return last < 0 ? 0u : (last >= 31 ? 0xffffffffu : 0xffffffffu >> (31 - last)); }
+__device__ __forceinline__ uint32_t tc_seen(int hi, int gone, int sink) { return tc_upto(hi) & (~tc_upto(gone) | tc_upto(sink)); }
 
 // One [128 x D] tile: D / 64 boxes on one barrier.
 template <int D>
@@ -133,9 +155,10 @@ __device__ __forceinline__ void tc_scores(uint32_t tmem_d, uint64_t a, uint64_t 
 }
 // O[128, D] (+)= P[128, 128] V[128, D], P in TMEM (two values to a column; its second half `split` columns behind the first),
 // V row by row in shared memory.
+template <int kFrom = 0, int kTo = 8>
 __device__ __forceinline__ void tc_accumulate(uint32_t tmem_d, uint32_t tmem_p, uint32_t split, uint64_t v, uint32_t idesc, uint32_t carry) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
+  for (int k = kFrom; k < kTo; ++k)
     umma_ts(tmem_d, tmem_p + (k < 4 ? 8 * k : split + 8 * (k - 4)), v + (uint64_t)k * 128u, idesc, k > 0 ? 1u : carry);
 }
 
@@ -158,10 +181,11 @@ __device__ __forceinline__ uint32_t tc_alloc(uint32_t* slot, uint32_t cols) {
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// Warps 0-3 and 4-7: the softmax of query tiles 0 and 1, one thread for each row; warp 8: MMA issue and TMEM; warp 9: TMA.
+// Warps 0-3 and 4-7: the softmax of query tiles 0 and 1, one thread for each row; warp 8: MMA issue and TMEM; warp 9: TMA;
+// warps 10 and 11 complete the warpgroup that gives its registers to the others.
 // The two tiles take turns: while one's scores are in the hands of its row threads, the tensor cores work for the other.
 // TMEM columns: S0 | S1 (128 each; P over the first 64 of its S), O0 | O1 (D each).
-constexpr int kFwdThreads = 320;
+constexpr int kFwdThreads = 384;         // launched with 168 registers each: 2 x 128 x 224 + 128 x 56 of the 64512
 constexpr int kFwdStages = 2;
 template <int D> struct FwdSmem {
   static constexpr uint32_t tile = (D / 64) * kTcHalf;
@@ -171,6 +195,24 @@ template <int D> struct FwdSmem {
 // P is kept 2^6 times its value, so that in fp16 a weight keeps its digits down to 2^-20 of the row's largest; the running
 // maximum may lag behind by 8 (2^14 in all, far from the type's largest) before the output is rescaled.
 constexpr float kPShift = 6.f, kMaxLag = 8.f;
+constexpr int kPolyPairs = 2;
+
+// 32 columns of a row: P = 2^(score sc + off), its sums, and its values in the operand type.  Of every 8 pairs kPolyPairs go
+// through the polynomial (the MUFU pipe alone takes 1024 cycles for a tile); not where keys are hidden, which get exactly 0.
+template <typename T, bool kPoly>
+__device__ __forceinline__ void tc_weigh(const uint32_t* x, f32x2 sc2, f32x2 off2, f32x2 (&part)[2], uint32_t (&pk)[16]) {
+#pragma unroll
+  for (int c = 0; c < 32; c += 2) {
+    float e0, e1;
+    unpack_f2(fma_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, off2), e0, e1);
+    f32x2 e;
+    if (kPoly && (c >> 1) * kPolyPairs % 8 < kPolyPairs) e = exp2_poly(e0, e1);
+    else e = pack_f2(ex2(e0), ex2(e1));
+    part[c >> 1 & 1] = add_f2(part[c >> 1 & 1], e);
+    unpack_f2(e, e0, e1);
+    pk[c >> 1] = pack2<T>(e0, e1);
+  }
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kFwdThreads, 1)
@@ -181,8 +223,8 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
   uint64_t *q_full = bars, *k_full = bars + 2, *k_empty = bars + 4, *v_full = bars + 6, *v_empty = bars + 8, *s_full = bars + 10,
-           *p_full = bars + 12, *o_full = bars + 14, *patch = bars + 15, *drain = bars + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+           *p_half = bars + 12, *p_full = bars + 14, *o_full = bars + 16, *patch = bars + 17, *drain = bars + 18;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
@@ -204,7 +246,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1); mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1);
-      mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4);
+      mbar_init(&s_full[s], 1); mbar_init(&p_half[s], 4); mbar_init(&p_full[s], 4);
     }
     mbar_init(o_full, 1); mbar_init(patch, 1); mbar_init(drain, 1);
     *abort_flag = 0;
@@ -218,6 +260,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 
   if (warp == 9) {
     // ---------------------------------------------------------------- loads
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (ntiles > 0) {
       if (lane == 0) {
         for (int s = 0; s < 2; ++s) {
@@ -266,6 +309,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
   } else if (warp == 8) {
     // ---------------------------------------------------------------- products
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (ntiles > 0) {
       const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
       const uint64_t dq = make_desc(smem_u32(smem + L::q)), dk = make_desc(smem_u32(smem + L::k)),
@@ -292,10 +336,13 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         for (int s = 0; s < 2; ++s) {
           const KeyRange& r = s ? r1 : r0;
           if (ok && r.has(kt)) {
-            ok = mbar_wait_warp(&v_full[st], ph) && mbar_wait_warp(&p_full[s], pphase >> s & 1u);
+            ok = mbar_wait_warp(&v_full[st], ph) && mbar_wait_warp(&p_half[s], pphase >> s & 1u);
+            tc_fence_after();
+            if (ok && elect_one()) tc_accumulate<0, 4>(tmem + 256 + D * s, tmem + 128 * s, 32, dv + st * step, id_o, started >> s & 1u);
+            ok = ok && mbar_wait_warp(&p_full[s], pphase >> s & 1u);
             pphase ^= 1u << s;
             tc_fence_after();
-            if (ok && elect_one()) tc_accumulate(tmem + 256 + D * s, tmem + 128 * s, 32, dv + st * step, id_o, started >> s & 1u);
+            if (ok && elect_one()) tc_accumulate<4, 8>(tmem + 256 + D * s, tmem + 128 * s, 32, dv + st * step, id_o, 1u);
             started |= 1u << s;
           }
           if (ok && next >= 0 && r.has(next)) {
@@ -315,8 +362,11 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (elect_one()) umma_commit(ok ? o_full : drain);
       if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
     }
+  } else if (warp >= 10) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   } else {
     // ---------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int s = warp >> 2, quad = warp & 3;
     const int row = quad * 32 + lane;
     const int q0 = qa + s * qstep, i = q0 + row, h = h0 + s * hstep;
@@ -342,11 +392,12 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const int k0 = kt * kTcRows;
       const bool whole = k0 + kTcRows - 1 <= q0 && (q0 + kTcRows - 1 - k0 < p.window || k0 + kTcRows <= p.sinks);
       if (!whole) {
-        const int c_hi = i - k0, c_sink = p.sinks - k0;
-        const int c_lo = i - k0 >= p.window ? i - k0 - p.window + 1 : 0;
 #pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (c > c_hi || (c < c_lo && c >= c_sink)) x[c] = 0xff800000u;
+        for (int c0 = 0; c0 < 128; c0 += 32) {
+          const uint32_t w = tc_seen(i - k0 - c0, i - p.window - k0 - c0, p.sinks - 1 - k0 - c0);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) if (!(w >> c & 1u)) x[c0 + c] = 0xff800000u;
+        }
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -377,24 +428,19 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
       for (int c0 = 0; c0 < 128; c0 += 32) {
         uint32_t pk[16];
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          float e0, e1;
-          unpack_f2(fma_f2(pack_f2(__uint_as_float(x[c0 + c]), __uint_as_float(x[c0 + c + 1])), sc2, off2), e0, e1);
-          e0 = ex2(e0);
-          e1 = ex2(e1);
-          part[c >> 1 & 1] = add_f2(part[c >> 1 & 1], pack_f2(e0, e1));
-          pk[c >> 1] = pack2<T>(e0, e1);
-        }
+        if (whole) tc_weigh<T, true>(x + c0, sc2, off2, part, pk);
+        else tc_weigh<T, false>(x + c0, sc2, off2, part, pk);
         tmem_st16(ts + (c0 >> 1), pk);
+        if (c0 == 32 || c0 == 96) {                               // the first half of P V starts under the second half's exponentials
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(c0 == 32 ? &p_half[s] : &p_full[s]);
+        }
       }
       float l0, l1;
       unpack_f2(add_f2(part[0], part[1]), l0, l1);
       l += l0 + l1;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[s]);
     }
     if (ok && ntiles > 0) ok = mbar_wait_warp(o_full, 0);
     if (!ok) *abort_flag = 1;

@@ -20,6 +20,7 @@ __device__ __forceinline__ float bwd_factor(float amax) {          // 2^(3 - e) 
 // Warps 0-3: columns 0..63 of the scores, warps 4-7: columns 64..127; warp 8: MMA and TMEM; warp 9: TMA.
 // TMEM columns: S of even tiles | S of odd tiles | dP (128 each) | dQ (D).  dS lies over the S it comes from: each half of the
 // columns over its own part.
+constexpr int kBwdThreads = 320;
 template <int D> struct DqSmem {
   static constexpr uint32_t tile = (D / 64) * kTcHalf;
   static constexpr int kst = 3, vst = 2;
@@ -28,7 +29,7 @@ template <int D> struct DqSmem {
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+__global__ void __launch_bounds__(kBwdThreads, 1)
 sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g, const TcParams p, int bf16) {
   typedef DqSmem<D> L;
@@ -232,11 +233,12 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
       if (!whole) {
         const int base = k0 + 64 * half;
-        const int c_hi = i - base, c_sink = p.sinks - base;
-        const int c_lo = i - k0 >= p.window ? i - base - p.window + 1 : -64;
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c > c_hi || (c < c_lo && c >= c_sink)) x[c] = 0u;
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          const uint32_t w = tc_seen(i - base - c0, i - p.window - base - c0, p.sinks - 1 - base - c0);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) if (!(w >> c & 1u)) x[c0 + c] = 0u;
+        }
       }
       uint32_t pk[32];
 #pragma unroll
@@ -305,7 +307,7 @@ template <int D> struct DkvSmem {
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+__global__ void __launch_bounds__(kBwdThreads, 1)
 sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g, const TcParams p,
                  const DkvSplit sp, int bf16) {
@@ -498,11 +500,13 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (!whole) {
         // query i = base + c sees key j when c >= j - base, and c < j - base + window or j is a sink
         const int base = q0 + 64 * half;
-        const int c_lo = j - base;
-        const int c_end = j < p.sinks ? 64 : (int)min((int64_t)64, (int64_t)(j - base) + p.window);
+        const int last = j < p.sinks ? 63 : (int)min((int64_t)63, (int64_t)(j - base) + p.window - 1);
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c < c_lo || c >= c_end) x[c] = 0u;
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          const uint32_t w = tc_upto(last - c0) & ~tc_upto(j - base - 1 - c0);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) if (!(w >> c & 1u)) x[c0 + c] = 0u;
+        }
       }
       uint32_t pk[32];
 #pragma unroll
@@ -656,10 +660,10 @@ static int tc_backward(const SwParams& p, float* parts, int bf16, int* error_fla
     cudaFuncSetAttribute(sw_dq_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DqSmem<D>::total);
     cudaFuncSetAttribute(sw_dkv_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DkvSmem<D>::total);
   }
-  sw_dq_tc_kernel<T, D><<<(unsigned)gq, kFwdThreads, DqSmem<D>::total, st>>>(mq, mk, mv, mg, t, bf16);
+  sw_dq_tc_kernel<T, D><<<(unsigned)gq, kBwdThreads, DqSmem<D>::total, st>>>(mq, mk, mv, mg, t, bf16);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
-  sw_dkv_tc_kernel<T, D><<<(unsigned)gk, kFwdThreads, DkvSmem<D>::total, st>>>(mq, mk, mv, mg, t, s, bf16);
+  sw_dkv_tc_kernel<T, D><<<(unsigned)gk, kBwdThreads, DkvSmem<D>::total, st>>>(mq, mk, mv, mg, t, s, bf16);
   e = cudaGetLastError();
   if (e != cudaSuccess || !s.part_tiles) return (int)e;
   sw_dkv_join_kernel<T, D><<<dim3((unsigned)(s.part_tiles * p.B * p.Hk), 2 * kTcRows * D / 8 / 256), 256, 0, st>>>(t, s);
