@@ -332,11 +332,12 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const int kt = key_tile(j), next = j + 1 < ntiles ? key_tile(j + 1) : -1;
         const int st = j % kFwdStages, sn = (j + 1) % kFwdStages;
         const uint32_t ph = (uint32_t)(j / kFwdStages) & 1u, pn = (uint32_t)((j + 1) / kFwdStages) & 1u;
+        ok = mbar_wait_warp(&v_full[st], ph);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const KeyRange& r = s ? r1 : r0;
           if (ok && r.has(kt)) {
-            ok = mbar_wait_warp(&v_full[st], ph) && mbar_wait_warp(&p_half[s], pphase >> s & 1u);
+            ok = mbar_wait_warp(&p_half[s], pphase >> s & 1u);
             tc_fence_after();
             if (ok && elect_one()) tc_accumulate<0, 4>(tmem + 256 + D * s, tmem + 128 * s, 32, dv + st * step, id_o, started >> s & 1u);
             ok = ok && mbar_wait_warp(&p_full[s], pphase >> s & 1u);
@@ -346,7 +347,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             started |= 1u << s;
           }
           if (ok && next >= 0 && r.has(next)) {
-            ok = mbar_wait_warp(&k_full[sn], pn);
+            if (s == 0 || !r0.has(next)) ok = mbar_wait_warp(&k_full[sn], pn);
             tc_fence_after();
             if (ok && elect_one()) {
               tc_scores<D>(tmem + 128 * s, dq + s * step, dk + sn * step, id_s);
@@ -395,6 +396,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
         for (int c0 = 0; c0 < 128; c0 += 32) {
           const uint32_t w = tc_seen(i - k0 - c0, i - p.window - k0 - c0, p.sinks - 1 - k0 - c0);
+          if (__all_sync(0xffffffffu, w == 0xffffffffu)) continue;
 #pragma unroll
           for (int c = 0; c < 32; ++c) if (!(w >> c & 1u)) x[c0 + c] = 0xff800000u;
         }
