@@ -16,6 +16,45 @@ __device__ __forceinline__ float bwd_factor(float amax) {          // 2^(3 - e) 
   return e < -30 || e > 16 ? 1.f : __uint_as_float((uint32_t)(127 + 3 - e) << 23);
 }
 
+// Of every 8 pairs of exponentials kBwdPoly go through the polynomial where no key is hidden.
+constexpr int kBwdPoly = 3;
+template <bool kPoly>
+__device__ __forceinline__ f32x2 bwd_exp(int pair, f32x2 y) {
+  float a, b;
+  unpack_f2(y, a, b);
+  return kPoly && pair * kBwdPoly % 8 < kBwdPoly ? exp2_poly(a, b) : pack_f2(ex2(a), ex2(b));
+}
+// 64 columns of a row: x = scores, y = dP  ->  x = P (f dP + neg_delta)
+template <typename T, bool kPoly>
+__device__ __forceinline__ void bwd_ds(uint32_t (&x)[64], const uint32_t (&y)[64], float sc, float neg_lse, float f, float neg_delta) {
+  const f32x2 sc2 = pack_f2(sc, sc), l2 = pack_f2(neg_lse, neg_lse), f2 = pack_f2(f, f), d2 = pack_f2(neg_delta, neg_delta);
+#pragma unroll
+  for (int c = 0; c < 64; c += 2) {
+    const f32x2 pr = bwd_exp<kPoly>(c >> 1, fma_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, l2));
+    const f32x2 dp = pack_f2(__uint_as_float(y[c]), __uint_as_float(y[c + 1]));
+    float a, b;
+    unpack_f2(mul_f2(pr, BwdRange<T>::scaled ? fma_f2(dp, f2, d2) : add_f2(dp, d2)), a, b);
+    x[c] = __float_as_uint(a);
+    x[c + 1] = __float_as_uint(b);
+  }
+}
+// 64 columns of a key's row: x = scores  ->  x = P, with the columns' own log-sum-exps
+template <bool kPoly>
+__device__ __forceinline__ void bwd_probs(uint32_t (&x)[64], const float* lse, float sc) {
+  const f32x2 sc2 = pack_f2(sc, sc);
+#pragma unroll
+  for (int c = 0; c < 64; c += 4) {
+    const float4 l = *reinterpret_cast<const float4*>(lse + c);   // negated
+    float a, b;
+    unpack_f2(bwd_exp<kPoly>(c >> 1, fma_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, pack_f2(l.x, l.y))), a, b);
+    x[c] = __float_as_uint(a);
+    x[c + 1] = __float_as_uint(b);
+    unpack_f2(bwd_exp<kPoly>((c >> 1) + 1, fma_f2(pack_f2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), sc2, pack_f2(l.z, l.w))), a, b);
+    x[c + 2] = __float_as_uint(a);
+    x[c + 3] = __float_as_uint(b);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ dQ
 // Warps 0-3: columns 0..63 of the scores, warps 4-7: columns 64..127; warp 8: MMA and TMEM; warp 9: TMA.
 // TMEM columns: S of even tiles | S of odd tiles | dP (128 each) | dQ (D).  dS lies over the S it comes from: each half of the
@@ -226,16 +265,14 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (half == 0 && i < p.T) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = live ? sum : 0.f;
         delta = sum * f;
       }
-#pragma unroll
-      for (int c = 0; c < 64; ++c) {
-        const float pr = ex2(fmaf(__uint_as_float(x[c]), sc, -lse));
-        x[c] = __float_as_uint(pr * (BwdRange<T>::scaled ? fmaf(__uint_as_float(y[c]), f, -delta) : __uint_as_float(y[c]) - delta));
-      }
+      if (whole) bwd_ds<T, true>(x, y, sc, -lse, f, -delta);
+      else bwd_ds<T, false>(x, y, sc, -lse, f, -delta);
       if (!whole) {
         const int base = k0 + 64 * half;
 #pragma unroll
         for (int c0 = 0; c0 < 64; c0 += 32) {
           const uint32_t w = tc_seen(i - base - c0, i - p.window - base - c0, p.sinks - 1 - base - c0);
+          if (__all_sync(0xffffffffu, w == 0xffffffffu)) continue;
 #pragma unroll
           for (int c = 0; c < 32; ++c) if (!(w >> c & 1u)) x[c0 + c] = 0u;
         }
@@ -313,7 +350,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                  const DkvSplit sp, int bf16) {
   typedef DkvSmem<D> L;
   extern __shared__ __align__(1024) uint8_t smem[];
-  float* s_stat = reinterpret_cast<float*>(smem + L::stat);        // [2 stages][lse 128 | delta 128]
+  float* s_stat = reinterpret_cast<float*>(smem + L::stat);        // [2 stages][-lse 128 | -delta 128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
   uint64_t *kv_full = bars, *q_full = bars + 1, *q_empty = bars + 4, *g_full = bars + 7, *g_empty = bars + 9, *st_full = bars + 11,
            *st_empty = bars + 13, *s_full = bars + 15, *dp_full = bars + 16, *p_ready = bars + 17, *ds_ready = bars + 18, *done = bars + 19,
@@ -412,8 +449,8 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int c = lane + 32 * e;
-          st[c] = q0 + c < n ? p.lse[at + c] - BwdRange<T>::shift : INFINITY;
-          st[128 + c] = q0 + c < n ? p.delta[at + c] * f : 0.f;
+          st[c] = q0 + c < n ? BwdRange<T>::shift - p.lse[at + c] : -INFINITY;
+          st[128 + c] = q0 + c < n ? -p.delta[at + c] * f : 0.f;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&st_full[it & 1]);
@@ -488,15 +525,9 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tmem_ld32(ts + 32, x + 32);
       tmem_wait_ld32(x);
       tmem_wait_ld32(x + 32);
-#pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const float4 l4 = *reinterpret_cast<const float4*>(st + c);
-        x[c] = __float_as_uint(ex2(fmaf(__uint_as_float(x[c]), sc, -l4.x)));
-        x[c + 1] = __float_as_uint(ex2(fmaf(__uint_as_float(x[c + 1]), sc, -l4.y)));
-        x[c + 2] = __float_as_uint(ex2(fmaf(__uint_as_float(x[c + 2]), sc, -l4.z)));
-        x[c + 3] = __float_as_uint(ex2(fmaf(__uint_as_float(x[c + 3]), sc, -l4.w)));
-      }
       const bool whole = k0 + kTcRows - 1 <= q0 && (q0 + kTcRows - 1 - k0 < p.window || k0 + kTcRows <= p.sinks);
+      if (whole) bwd_probs<true>(x, st, sc);
+      else bwd_probs<false>(x, st, sc);
       if (!whole) {
         // query i = base + c sees key j when c >= j - base, and c < j - base + window or j is a sink
         const int base = q0 + 64 * half;
@@ -504,6 +535,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
         for (int c0 = 0; c0 < 64; c0 += 32) {
           const uint32_t w = tc_upto(last - c0) & ~tc_upto(j - base - 1 - c0);
+          if (__all_sync(0xffffffffu, w == 0xffffffffu)) continue;
 #pragma unroll
           for (int c = 0; c < 32; ++c) if (!(w >> c & 1u)) x[c0 + c] = 0u;
         }
@@ -521,18 +553,18 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tc_fence_after();
       if (BwdRange<T>::scaled && it == 0) f = s_factor[0];
       const float fu = f * BwdRange<T>::unshift;
-      auto ds = [&](uint32_t pr, uint32_t dp, float dl) {
-        return __uint_as_float(pr) * (BwdRange<T>::scaled ? fmaf(__uint_as_float(dp), fu, -dl) : __uint_as_float(dp) - dl);
-      };
+      const f32x2 fu2 = pack_f2(fu, fu);
       tmem_ld32(td, y);
       tmem_ld32(td + 32, y + 32);
       tmem_wait_ld32(y);
       tmem_wait_ld32(y + 32);
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const float4 d4 = *reinterpret_cast<const float4*>(st + 128 + c);
-        pk[c >> 1] = pack2<T>(ds(x[c], y[c], d4.x), ds(x[c + 1], y[c + 1], d4.y));
-        pk[(c >> 1) + 1] = pack2<T>(ds(x[c + 2], y[c + 2], d4.z), ds(x[c + 3], y[c + 3], d4.w));
+      for (int c = 0; c < 64; c += 2) {
+        const float2 d2 = *reinterpret_cast<const float2*>(st + 128 + c);
+        const f32x2 dp = pack_f2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), nd = pack_f2(d2.x, d2.y);
+        float a, b;
+        unpack_f2(mul_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), BwdRange<T>::scaled ? fma_f2(dp, fu2, nd) : add_f2(dp, nd)), a, b);
+        pk[c >> 1] = pack2<T>(a, b);
       }
       tmem_st32(td, pk);
       tmem_wait_st();
