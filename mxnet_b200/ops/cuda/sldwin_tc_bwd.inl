@@ -367,9 +367,11 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int unit = blockIdx.x / sp.items, item = blockIdx.x % sp.items;
   const int hs = item % sp.hsplit, bh = item / sp.hsplit, b = bh / p.Hk, hk = bh % p.Hk;
   const int group = p.Hq / p.Hk, heads = group / sp.hsplit, h_first = hk * group + hs * heads;
-  const bool far = unit >= sp.tiles;
-  const int kt = far ? (unit - sp.tiles) % sp.sink_tiles : unit;
-  const int chunk = far ? (unit - sp.tiles) / sp.sink_tiles : 0;
+  // far chunks, all of them full, start first; near tiles follow from the first key tile, whose walks are the longest
+  const int nfar = sp.sink_tiles * sp.far_chunks;
+  const bool far = unit < nfar;
+  const int kt = far ? unit % sp.sink_tiles : unit - nfar;
+  const int chunk = far ? unit / sp.sink_tiles : 0;
   const int n = warp_uniform(tc_valid(p, b));
   const int k0 = kt * kTcRows;
   const int last_tile = n > 0 ? (n - 1) / kTcRows : -1;
