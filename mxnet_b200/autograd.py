@@ -186,6 +186,27 @@ def _head_grads(heads, head_grads):
     return out
 
 
+class _Here(object):
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_HERE = _Here()
+
+
+def _calling_thread(tensors):
+    """Scope of a gradient pass whose heads lie on one device: it runs on the thread that asked for it.  The tensor library's
+    worker of that device would do the same work in the same order after two thread switches (30 to 200 us, as the machine
+    schedules them); heads on several devices keep their workers, which run side by side."""
+    first = tensors[0].device
+    if first.type == 'cuda' and all(t.device == first for t in tensors[1:]):
+        return torch.autograd.set_multithreading_enabled(False)
+    return _HERE
+
+
 def backward(heads, head_grads=None, retain_graph=False, train_mode=True):  # pylint: disable=redefined-outer-name
     """Compute gradients of ``heads`` w.r.t. every marked variable (``MXAutogradBackwardEx``)."""
     if isinstance(heads, NDArray):
@@ -206,7 +227,8 @@ def backward(heads, head_grads=None, retain_graph=False, train_mode=True):  # py
     grads = _head_grads(heads, head_grads)
     prev = set_training(train_mode)
     try:
-        torch.autograd.backward(tensors, grads, retain_graph=retain_graph)
+        with _calling_thread(tensors):
+            torch.autograd.backward(tensors, grads, retain_graph=retain_graph)
     finally:
         set_training(prev)
     if not retain_graph:
@@ -229,8 +251,9 @@ def grad(heads, variables, head_grads=None, retain_graph=None, create_graph=Fals
         retain_graph = create_graph
     prev = set_training(train_mode)
     try:
-        with torch.enable_grad():
-            res = torch.autograd.grad([h._data for h in heads], [v._data for v in variables],
+        tensors = [h._data for h in heads]
+        with torch.enable_grad(), _calling_thread(tensors):
+            res = torch.autograd.grad(tensors, [v._data for v in variables],
                                       _head_grads(heads, head_grads), retain_graph=retain_graph,
                                       create_graph=create_graph, allow_unused=True)
     finally:

@@ -403,3 +403,27 @@ def test_second_derivatives_are_refused_not_wrong():
     g, = torch.autograd.grad(lp.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), x)
+
+
+def test_a_gradient_pass_of_one_device_runs_on_the_calling_thread():
+    import threading
+    seen = []
+
+    class Spy(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            seen.append(threading.get_ident())
+            return g * 2
+    x = nd.NDArray(torch.ones(3, device=dev()))
+    x.attach_grad()
+    for ask in (lambda y: y.backward(), lambda y: autograd.grad(y, x, nd.NDArray(torch.ones(3, device=dev())))):
+        with autograd.record():
+            with torch.enable_grad():
+                y = nd.NDArray(Spy.apply(x._data))
+        ask(y)
+    assert seen == [threading.get_ident()] * 2 and x.grad._data.tolist() == [4.0 / 2] * 3
+    assert torch._C._is_multithreading_enabled() if hasattr(torch._C, '_is_multithreading_enabled') else True
