@@ -153,13 +153,13 @@ __device__ __forceinline__ void tc_scores(uint32_t tmem_d, uint64_t a, uint64_t 
     umma(tmem_d, a + o, b + o, idesc, k > 0 ? 1u : 0u);
   }
 }
-// O[128, D] (+)= P[128, 128] V[128, D], P in TMEM (two values to a column; its second half `split` columns behind the first),
-// V row by row in shared memory.
-template <int kFrom = 0, int kTo = 8>
-__device__ __forceinline__ void tc_accumulate(uint32_t tmem_d, uint32_t tmem_p, uint32_t split, uint64_t v, uint32_t idesc, uint32_t carry) {
+// O[128, D] (+)= P[128, 128] V[128, D], k-steps kFrom .. kTo - 1 of 16.  P lies in TMEM, two values to a column, over the scores it
+// was made of: a thread's share of kSteps k-steps starts where its 16 kSteps columns of scores did.  V row by row in shared memory.
+template <int kSteps, int kFrom = 0, int kTo = 8>
+__device__ __forceinline__ void tc_accumulate(uint32_t tmem_d, uint32_t tmem_p, uint64_t v, uint32_t idesc, uint32_t carry) {
 #pragma unroll
   for (int k = kFrom; k < kTo; ++k)
-    umma_ts(tmem_d, tmem_p + (k < 4 ? 8 * k : split + 8 * (k - 4)), v + (uint64_t)k * 128u, idesc, k > 0 ? 1u : carry);
+    umma_ts(tmem_d, tmem_p + k / kSteps * 16 * kSteps + k % kSteps * 8, v + (uint64_t)k * 128u, idesc, k > 0 ? 1u : carry);
 }
 
 __device__ __forceinline__ void tc_finish(uint32_t tmem_base, uint32_t cols, int warp, int alloc_warp, volatile int* abort_flag, int* error_flag) {
@@ -339,11 +339,11 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           if (ok && r.has(kt)) {
             ok = mbar_wait_warp(&p_half[s], pphase >> s & 1u);
             tc_fence_after();
-            if (ok && elect_one()) tc_accumulate<0, 4>(tmem + 256 + D * s, tmem + 128 * s, 32, dv + st * step, id_o, started >> s & 1u);
+            if (ok && elect_one()) tc_accumulate<8, 0, 4>(tmem + 256 + D * s, tmem + 128 * s, dv + st * step, id_o, started >> s & 1u);
             ok = ok && mbar_wait_warp(&p_full[s], pphase >> s & 1u);
             pphase ^= 1u << s;
             tc_fence_after();
-            if (ok && elect_one()) tc_accumulate<4, 8>(tmem + 256 + D * s, tmem + 128 * s, 32, dv + st * step, id_o, 1u);
+            if (ok && elect_one()) tc_accumulate<8, 4, 8>(tmem + 256 + D * s, tmem + 128 * s, dv + st * step, id_o, 1u);
             started |= 1u << s;
           }
           if (ok && next >= 0 && r.has(next)) {

@@ -24,12 +24,12 @@ __device__ __forceinline__ f32x2 bwd_exp(int pair, f32x2 y) {
   unpack_f2(y, a, b);
   return kPoly && pair * kBwdPoly % 8 < kBwdPoly ? exp2_poly(a, b) : pack_f2(ex2(a), ex2(b));
 }
-// 64 columns of a row: x = scores, y = dP  ->  x = P (f dP + neg_delta)
+// 32 columns of a row: x = scores, y = dP  ->  x = P (f dP + neg_delta)
 template <typename T, bool kPoly>
-__device__ __forceinline__ void bwd_ds(uint32_t (&x)[64], const uint32_t (&y)[64], float sc, float neg_lse, float f, float neg_delta) {
+__device__ __forceinline__ void bwd_ds(uint32_t (&x)[32], const uint32_t (&y)[32], float sc, float neg_lse, float f, float neg_delta) {
   const f32x2 sc2 = pack_f2(sc, sc), l2 = pack_f2(neg_lse, neg_lse), f2 = pack_f2(f, f), d2 = pack_f2(neg_delta, neg_delta);
 #pragma unroll
-  for (int c = 0; c < 64; c += 2) {
+  for (int c = 0; c < 32; c += 2) {
     const f32x2 pr = bwd_exp<kPoly>(c >> 1, fma_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, l2));
     const f32x2 dp = pack_f2(__uint_as_float(y[c]), __uint_as_float(y[c + 1]));
     float a, b;
@@ -38,12 +38,12 @@ __device__ __forceinline__ void bwd_ds(uint32_t (&x)[64], const uint32_t (&y)[64
     x[c + 1] = __float_as_uint(b);
   }
 }
-// 64 columns of a key's row: x = scores  ->  x = P, with the columns' own log-sum-exps
+// 32 columns of a key's row: x = scores  ->  x = P, with the columns' own log-sum-exps
 template <bool kPoly>
-__device__ __forceinline__ void bwd_probs(uint32_t (&x)[64], const float* lse, float sc) {
+__device__ __forceinline__ void bwd_probs(uint32_t (&x)[32], const float* lse, float sc) {
   const f32x2 sc2 = pack_f2(sc, sc);
 #pragma unroll
-  for (int c = 0; c < 64; c += 4) {
+  for (int c = 0; c < 32; c += 4) {
     const float4 l = *reinterpret_cast<const float4*>(lse + c);   // negated
     float a, b;
     unpack_f2(bwd_exp<kPoly>(c >> 1, fma_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, pack_f2(l.x, l.y))), a, b);
@@ -56,15 +56,14 @@ __device__ __forceinline__ void bwd_probs(uint32_t (&x)[64], const float* lse, f
 }
 
 // ------------------------------------------------------------------------------------------------ dQ
-// Warps 0-3: columns 0..63 of the scores, warps 4-7: columns 64..127; warp 8: MMA and TMEM; warp 9: TMA.
-// TMEM columns: S of even tiles | S of odd tiles | dP (128 each) | dQ (D).  dS lies over the S it comes from: each half of the
-// columns over its own part.
-constexpr int kBwdThreads = 320;
+// TMEM columns: S of even tiles | S of odd tiles | dP (128 each) | dQ (D).  dS lies over the S it comes from: each part of the
+// columns over its own.
+constexpr int kBwdThreads = 576, kBwdMma = 16, kBwdTma = 17;
 template <int D> struct DqSmem {
   static constexpr uint32_t tile = (D / 64) * kTcHalf;
   static constexpr int kst = 3, vst = 2;
-  static constexpr uint32_t q = 0, g = tile, k = 2 * tile, v = k + kst * tile, delta = v + vst * tile, bars = delta + 1088;
-  static constexpr uint32_t total = bars + 192 + 1024;
+  static constexpr uint32_t q = 0, g = tile, k = 2 * tile, v = k + kst * tile, delta = v + vst * tile, bars = delta + 1024;
+  static constexpr uint32_t total = bars + 256;
 };
 
 template <typename T, int D>
@@ -72,16 +71,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g, const TcParams p, int bf16) {
   typedef DqSmem<D> L;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  float* s_delta = reinterpret_cast<float*>(smem + L::delta);      // [2][128]
+  extern __shared__ __align__(1024) uint8_t smem[];
+  float* s_delta = reinterpret_cast<float*>(smem + L::delta);      // [128], then the warps' largest |dO|
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
   uint64_t *qg_full = bars, *k_full = bars + 1, *k_empty = bars + 4, *v_full = bars + 7, *v_empty = bars + 9, *sd_full = bars + 11,
            *dp_empty = bars + 12, *ds_full = bars + 13, *done = bars + 14, *patch = bars + 15, *drain = bars + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-
+  if (smem_u32(smem) & 1023u) {                                    // swizzled tiles lie on 1024-byte boundaries
+    if (threadIdx.x == 0 && p.error_flag) *static_cast<volatile int*>(p.error_flag) = 1;
+    return;
+  }
   const int tiles = p.T / kTcRows + (p.T % kTcRows ? 1 : 0);
   const int qt = tiles - 1 - (int)(blockIdx.x / p.items), item = blockIdx.x % p.items;
   const int b = item / p.Hq, h = item % p.Hq, hk = h / (p.Hq / p.Hk);
@@ -95,18 +96,18 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     mbar_init(qg_full, 1);
     for (int s = 0; s < L::kst; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
     for (int s = 0; s < L::vst; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
-    mbar_init(sd_full, 1); mbar_init(dp_empty, 8); mbar_init(ds_full, 8); mbar_init(done, 1); mbar_init(patch, 1); mbar_init(drain, 1);
+    mbar_init(sd_full, 1); mbar_init(dp_empty, 16); mbar_init(ds_full, 16); mbar_init(done, 1); mbar_init(patch, 1); mbar_init(drain, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) tc_alloc(tmem_slot, 512);
+  if (warp == kBwdMma) tc_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = warp_uniform(*tmem_slot);
   constexpr uint32_t kDp = 256, kDq = 384;
 
-  if (warp == 9) {
+  if (warp == kBwdTma) {
     if (ntiles > 0) {
       if (lane == 0) {
         mbar_expect_tx(qg_full, 2 * L::tile);
@@ -147,7 +148,7 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == kBwdMma) {
     if (ntiles > 0) {
       const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
       const uint64_t dq = make_desc(smem_u32(smem + L::q)), dg = make_desc(smem_u32(smem + L::g)), dk = make_desc(smem_u32(smem + L::k)),
@@ -181,7 +182,7 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          tc_accumulate(tmem + kDq, tmem + 128 * (j & 1), 64, dkm + (j % L::kst) * step, id_o, j > 0 ? 1u : 0u);
+          tc_accumulate<2>(tmem + kDq, tmem + 128 * (j & 1), dkm + (j % L::kst) * step, id_o, j > 0 ? 1u : 0u);
           umma_commit(&k_empty[j % L::kst]);
         }
         if (j + 2 < ntiles) scores(j + 2);                        // over S and dS of this tile, read by the product before it
@@ -190,45 +191,49 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
     }
   } else {
-    const int half = warp >> 2, quad = warp & 3;
+    const int part = warp >> 2, quad = warp & 3;
     const int row = quad * 32 + lane, i = q0 + row;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const bool live = i < n;
-    // delta = rowsum(dO * O), half of the channels in each warpgroup, while the first products run
-    float part = 0.f, lse = INFINITY, big = 0.f;
-    if (live) {
-      const T* orow = static_cast<const T*>(p.o) + (((int64_t)b * p.T + i) * p.Hq + h) * D + half * (D / 2);
-      const T* grow = static_cast<const T*>(p.dout) + b * p.sdo.b + i * p.sdo.t + h * p.sdo.h + half * (D / 2);
+    // delta = rowsum(dO * O) while the first products run: 8 rows for each warp, whole rows side by side in a load
+    constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+    float big = 0.f;
 #pragma unroll
-      for (int v = 0; v < D / 16; ++v) {
-        const Vec16<T> a = ld16(orow + v * 8), g = ld16(grow + v * 8);
+    for (int r0 = 0; r0 < 8; r0 += kRows) {
+      const int rr = warp * 8 + r0 + lane / kLanes, ch = lane % kLanes * 8;
+      float dot = 0.f;
+      if (q0 + rr < n) {
+        const Vec16<T> a = ld16(static_cast<const T*>(p.o) + (((int64_t)b * p.T + q0 + rr) * p.Hq + h) * D + ch);
+        const Vec16<T> g = ld16(static_cast<const T*>(p.dout) + b * p.sdo.b + (int64_t)(q0 + rr) * p.sdo.t + h * p.sdo.h + ch);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float ge = Cvt<T>::to_f(g.v[e]);
-          part += Cvt<T>::to_f(a.v[e]) * ge;
+          dot += Cvt<T>::to_f(a.v[e]) * ge;
           if (BwdRange<T>::scaled) big = fmaxf(big, fabsf(ge));
         }
       }
-      lse = p.lse[((int64_t)b * p.Hq + h) * p.T + i];
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      if (lane % kLanes == 0) s_delta[rr] = dot;
     }
-    s_delta[half * 128 + row] = part;
     if (BwdRange<T>::scaled) {
       big = warp_max(big);
-      if (lane == 0) s_delta[256 + warp] = big;
+      if (lane == 0) s_delta[128 + warp] = big;
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float lse = live ? p.lse[((int64_t)b * p.Hq + h) * p.T + i] : INFINITY;
+    asm volatile("bar.sync 1, 512;" ::: "memory");
     // Rows whose keys are all in one tile get delta from the sum of P dP instead of from the rounded output: with few keys the
     // output's rounding is not small beside dP - delta.
     const bool one_tile = ntiles == 1;
-    float delta = one_tile ? 0.f : s_delta[row] + s_delta[128 + row];
+    float delta = s_delta[row];
     float f = 1.f;
     if (BwdRange<T>::scaled) {
 #pragma unroll
-      for (int w = 0; w < 8; ++w) big = fmaxf(big, s_delta[256 + w]);
+      for (int w = 0; w < 16; ++w) big = fmaxf(big, s_delta[128 + w]);
       if (threadIdx.x == 0) p.gmax[((int64_t)b * p.Hq + h) * tiles + qt] = big;
       f = bwd_factor(big);
     }
-    if (half == 0 && i < p.T && !one_tile) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = delta;
+    if (part == 0 && i < p.T && !one_tile) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = delta;
     delta *= f;
     const float out_scale = p.scale / f;
     const float sc = p.scale * kSwLog2e;
@@ -236,51 +241,45 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     for (int j = 0; j < ntiles; ++j) {
       const int kt = key_tile(j);
       ok = mbar_wait_warp(sd_full, (uint32_t)j & 1u);
-      if (!ok) break;
+      if (!ok) {
+        if (one_tile) asm volatile("bar.sync 1, 512;" ::: "memory");           // the warps that got through wait there
+        break;
+      }
       tc_fence_after();
-      const uint32_t ts = tmem + 128 * (j & 1) + 64 * half + lane_off, td = tmem + kDp + 64 * half + lane_off;
-      uint32_t x[64], y[64];
+      const uint32_t ts = tmem + 128 * (j & 1) + 32 * part + lane_off, td = tmem + kDp + 32 * part + lane_off;
+      uint32_t x[32], y[32];
       tmem_ld32(ts, x);
-      tmem_ld32(ts + 32, x + 32);
       tmem_ld32(td, y);
-      tmem_ld32(td + 32, y + 32);
       tmem_wait_ld32(x);
-      tmem_wait_ld32(x + 32);
       tmem_wait_ld32(y);
-      tmem_wait_ld32(y + 32);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dp_empty);
       const int k0 = kt * kTcRows;
       const bool whole = k0 + kTcRows - 1 <= q0 && (q0 + kTcRows - 1 - k0 < p.window || k0 + kTcRows <= p.sinks);
+      const int base = k0 + 32 * part;
+      const uint32_t seen = whole ? 0xffffffffu : tc_seen(i - base, i - p.window - base, p.sinks - 1 - base);
       if (one_tile) {
         float sum = 0.f;
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (k0 + 64 * half + c <= i && (i - (k0 + 64 * half + c) < p.window || k0 + 64 * half + c < p.sinks))
-            sum += ex2(fmaf(__uint_as_float(x[c]), sc, -lse)) * __uint_as_float(y[c]);
-        s_delta[half * 128 + row] = sum;                          // nobody reads the first sums in this case
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        sum = s_delta[row] + s_delta[128 + row];
-        if (half == 0 && i < p.T) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = live ? sum : 0.f;
+        for (int c = 0; c < 32; ++c) if (seen >> c & 1u) sum += ex2(fmaf(__uint_as_float(x[c]), sc, -lse)) * __uint_as_float(y[c]);
+        float* s_sum = reinterpret_cast<float*>(smem + L::k + L::tile);        // [4][128] in a stage that a single tile leaves unused
+        s_sum[part * 128 + row] = sum;
+        asm volatile("bar.sync 1, 512;" ::: "memory");
+        sum = (s_sum[row] + s_sum[128 + row]) + (s_sum[256 + row] + s_sum[384 + row]);
+        if (part == 0 && i < p.T) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = live ? sum : 0.f;
         delta = sum * f;
       }
       if (whole) bwd_ds<T, true>(x, y, sc, -lse, f, -delta);
       else bwd_ds<T, false>(x, y, sc, -lse, f, -delta);
-      if (!whole) {
-        const int base = k0 + 64 * half;
+      if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
 #pragma unroll
-        for (int c0 = 0; c0 < 64; c0 += 32) {
-          const uint32_t w = tc_seen(i - base - c0, i - p.window - base - c0, p.sinks - 1 - base - c0);
-          if (__all_sync(0xffffffffu, w == 0xffffffffu)) continue;
-#pragma unroll
-          for (int c = 0; c < 32; ++c) if (!(w >> c & 1u)) x[c0 + c] = 0u;
-        }
+        for (int c = 0; c < 32; ++c) if (!(seen >> c & 1u)) x[c] = 0u;
       }
-      uint32_t pk[32];
+      uint32_t pk[16];
 #pragma unroll
-      for (int c = 0; c < 32; ++c) pk[c] = pack2<T>(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1]));
-      tmem_st32(ts, pk);
+      for (int c = 0; c < 16; ++c) pk[c] = pack2<T>(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1]));
+      tmem_st16(ts, pk);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -289,29 +288,26 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (ok && ntiles > 0) ok = mbar_wait_warp(done, 0);
     if (!ok) *abort_flag = 1;
     tc_fence_after();
-    if (ok) {
-      T* dst = static_cast<T*>(p.dq) + (((int64_t)b * p.T + i) * p.Hq + h) * D + half * (D / 2);
-#pragma unroll 1
-      for (int c0 = 0; c0 < D / 2; c0 += 32) {
-        uint32_t o[32];
-        if (ntiles > 0) { tmem_ld32(tmem + kDq + half * (D / 2) + c0 + lane_off, o); tmem_wait_ld32(o); }
-        if (i < p.T) {
+    if (ok && 32 * part < D) {
+      T* dst = static_cast<T*>(p.dq) + (((int64_t)b * p.T + i) * p.Hq + h) * D + 32 * part;
+      uint32_t o[32];
+      if (ntiles > 0) { tmem_ld32(tmem + kDq + 32 * part + lane_off, o); tmem_wait_ld32(o); }
+      if (i < p.T) {
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (live) {
-              w.x = pack2<T>(__uint_as_float(o[v * 8]) * out_scale, __uint_as_float(o[v * 8 + 1]) * out_scale);
-              w.y = pack2<T>(__uint_as_float(o[v * 8 + 2]) * out_scale, __uint_as_float(o[v * 8 + 3]) * out_scale);
-              w.z = pack2<T>(__uint_as_float(o[v * 8 + 4]) * out_scale, __uint_as_float(o[v * 8 + 5]) * out_scale);
-              w.w = pack2<T>(__uint_as_float(o[v * 8 + 6]) * out_scale, __uint_as_float(o[v * 8 + 7]) * out_scale);
-            }
-            *reinterpret_cast<uint4*>(dst + c0 + v * 8) = w;
+        for (int v = 0; v < 4; ++v) {
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (live) {
+            w.x = pack2<T>(__uint_as_float(o[v * 8]) * out_scale, __uint_as_float(o[v * 8 + 1]) * out_scale);
+            w.y = pack2<T>(__uint_as_float(o[v * 8 + 2]) * out_scale, __uint_as_float(o[v * 8 + 3]) * out_scale);
+            w.z = pack2<T>(__uint_as_float(o[v * 8 + 4]) * out_scale, __uint_as_float(o[v * 8 + 5]) * out_scale);
+            w.w = pack2<T>(__uint_as_float(o[v * 8 + 6]) * out_scale, __uint_as_float(o[v * 8 + 7]) * out_scale);
           }
+          *reinterpret_cast<uint4*>(dst + v * 8) = w;
         }
       }
     }
   }
-  tc_finish(tmem, 512, warp, 8, abort_flag, p.error_flag);
+  tc_finish(tmem, 512, warp, kBwdMma, abort_flag, p.error_flag);
 }
 
 // ------------------------------------------------------------------------------------------------ dK, dV
@@ -319,7 +315,7 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 // windows reach its keys.  A key tile that holds sinks is seen by all later queries as well: those far tiles go to CTAs of
 // their own in chunks as long as a window, and where keys are few the heads of a group are split over CTAs; such parts are
 // written in fp32 and added in a fixed order by a last small kernel.
-// TMEM columns: S^T | dP^T (128 each) | dV | dK (D each); P^T over S^T, dS^T over dP^T, each half of the columns over its own part.
+// TMEM columns: S^T | dP^T (128 each) | dV | dK (D each); P^T over S^T, dS^T over dP^T, each part of the columns over its own.
 struct DkvSplit {
   int tiles, near_span;                  // query tiles kt .. kt + near_span reach a key tile by their windows
   int sink_tiles, far_chunks;            // far CTAs: sink_tiles x far_chunks of near_span + 1 query tiles
@@ -383,20 +379,20 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
     for (int s = 0; s < L::qst; ++s) { mbar_init(&q_full[s], 1); mbar_init(&q_empty[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&g_full[s], 1); mbar_init(&g_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], 8); }
-    mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_ready, 8); mbar_init(ds_ready, 8); mbar_init(done, 1); mbar_init(patch, 1);
+    for (int s = 0; s < 2; ++s) { mbar_init(&g_full[s], 1); mbar_init(&g_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], 16); }
+    mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_ready, 16); mbar_init(ds_ready, 16); mbar_init(done, 1); mbar_init(patch, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) tc_alloc(tmem_slot, 512);
+  if (warp == kBwdMma) tc_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = warp_uniform(*tmem_slot);
   constexpr uint32_t kDp = 128, kDv = 256, kDk = 256 + D;
 
-  if (warp == 9) {
+  if (warp == kBwdTma) {
     if (nit > 0) {
       if (lane == 0) {
         mbar_expect_tx(kv_full, 2 * L::tile);
@@ -466,7 +462,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == kBwdMma) {
     if (nit > 0) {
       const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
       const uint64_t dk = make_desc(smem_u32(smem + L::k)), dv = make_desc(smem_u32(smem + L::v)), dq = make_desc(smem_u32(smem + L::q)),
@@ -491,7 +487,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          tc_accumulate(tmem + kDv, tmem, 64, dgm + (it % L::gst) * step, id_o, it > 0 ? 1u : 0u);
+          tc_accumulate<2>(tmem + kDv, tmem, dgm + (it % L::gst) * step, id_o, it > 0 ? 1u : 0u);
           umma_commit(&g_empty[it % L::gst]);                     // dP of this tile was issued before: dO is done with
         }
         if (it + 1 < nit) scores(it + 1);
@@ -500,7 +496,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          tc_accumulate(tmem + kDk, tmem + kDp, 64, dqm + (it % L::qst) * step, id_o, it > 0 ? 1u : 0u);
+          tc_accumulate<2>(tmem + kDk, tmem + kDp, dqm + (it % L::qst) * step, id_o, it > 0 ? 1u : 0u);
           umma_commit(&q_empty[it % L::qst]);
         }
         if (it + 1 < nit) dprobs(it + 1);
@@ -509,43 +505,39 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
     }
   } else {
-    const int half = warp >> 2, quad = warp & 3;
+    const int part = warp >> 2, quad = warp & 3;
     const int row = quad * 32 + lane, j = k0 + row;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-    const uint32_t ts = tmem + 64 * half + lane_off, td = tmem + kDp + 64 * half + lane_off;
+    const uint32_t ts = tmem + 32 * part + lane_off, td = tmem + kDp + 32 * part + lane_off;
     const float sc = p.scale * kSwLog2e;
     float f = 1.f;                                                // of dO in dS
     bool ok = true;
     for (int it = 0; it < nit; ++it) {
       const int q0 = (qlo + it % per_head) * kTcRows;
-      const float* st = s_stat + (it & 1) * 256 + 64 * half;
+      const float* st = s_stat + (it & 1) * 256 + 32 * part;
       ok = mbar_wait_warp(&st_full[it & 1], (uint32_t)(it / 2) & 1u) && mbar_wait_warp(s_full, (uint32_t)it & 1u);
       if (!ok) break;
       tc_fence_after();
-      uint32_t x[64], y[64];
+      uint32_t x[32], y[32];
       tmem_ld32(ts, x);
-      tmem_ld32(ts + 32, x + 32);
       tmem_wait_ld32(x);
-      tmem_wait_ld32(x + 32);
       const bool whole = k0 + kTcRows - 1 <= q0 && (q0 + kTcRows - 1 - k0 < p.window || k0 + kTcRows <= p.sinks);
       if (whole) bwd_probs<true>(x, st, sc);
       else bwd_probs<false>(x, st, sc);
       if (!whole) {
         // query i = base + c sees key j when c >= j - base, and c < j - base + window or j is a sink
-        const int base = q0 + 64 * half;
-        const int last = j < p.sinks ? 63 : (int)min((int64_t)63, (int64_t)(j - base) + p.window - 1);
+        const int base = q0 + 32 * part;
+        const int last = j < p.sinks ? 31 : (int)min((int64_t)31, (int64_t)(j - base) + p.window - 1);
+        const uint32_t w = tc_upto(last) & ~tc_upto(j - base - 1);
+        if (!__all_sync(0xffffffffu, w == 0xffffffffu)) {
 #pragma unroll
-        for (int c0 = 0; c0 < 64; c0 += 32) {
-          const uint32_t w = tc_upto(last - c0) & ~tc_upto(j - base - 1 - c0);
-          if (__all_sync(0xffffffffu, w == 0xffffffffu)) continue;
-#pragma unroll
-          for (int c = 0; c < 32; ++c) if (!(w >> c & 1u)) x[c0 + c] = 0u;
+          for (int c = 0; c < 32; ++c) if (!(w >> c & 1u)) x[c] = 0u;
         }
       }
-      uint32_t pk[32];
+      uint32_t pk[16];
 #pragma unroll
-      for (int c = 0; c < 32; ++c) pk[c] = pack2<T>(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1]));
-      tmem_st32(ts, pk);
+      for (int c = 0; c < 16; ++c) pk[c] = pack2<T>(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1]));
+      tmem_st16(ts, pk);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -557,18 +549,16 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const float fu = f * BwdRange<T>::unshift;
       const f32x2 fu2 = pack_f2(fu, fu);
       tmem_ld32(td, y);
-      tmem_ld32(td + 32, y + 32);
       tmem_wait_ld32(y);
-      tmem_wait_ld32(y + 32);
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {
+      for (int c = 0; c < 32; c += 2) {
         const float2 d2 = *reinterpret_cast<const float2*>(st + 128 + c);
         const f32x2 dp = pack_f2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), nd = pack_f2(d2.x, d2.y);
         float a, b;
         unpack_f2(mul_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), BwdRange<T>::scaled ? fma_f2(dp, fu2, nd) : add_f2(dp, nd)), a, b);
         pk[c >> 1] = pack2<T>(a, b);
       }
-      tmem_st32(td, pk);
+      tmem_st16(td, pk);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -578,19 +568,20 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (!ok) *abort_flag = 1;
     tc_fence_after();
     if (ok) {
-      // warps 0-3 write dK, warps 4-7 dV
-      const float mul = half == 0 ? p.scale / f : BwdRange<T>::unshift;
-      const uint32_t acc = tmem + (half == 0 ? kDk : kDv) + lane_off;
+      // parts 0 and 1 write the halves of dK, parts 2 and 3 those of dV
+      const int which = part >> 1, from = (part & 1) * (D / 2);
+      const float mul = which == 0 ? p.scale / f : BwdRange<T>::unshift;
+      const uint32_t acc = tmem + (which == 0 ? kDk : kDv) + from + lane_off;
       const bool parts = kt < sp.part_tiles;
       const bool live = j < n && nit > 0;
-      float* part = nullptr;
+      float* sum = nullptr;
       if (parts) {
-        part = far ? dkv_far_part(sp, (int64_t)p.B * p.Hk, hs, chunk, bh, kt, D) : dkv_near_part(sp, (int64_t)p.B * p.Hk, hs, bh, kt, D);
-        part += ((int64_t)half * kTcRows + row) * D;
+        sum = far ? dkv_far_part(sp, (int64_t)p.B * p.Hk, hs, chunk, bh, kt, D) : dkv_near_part(sp, (int64_t)p.B * p.Hk, hs, bh, kt, D);
+        sum += ((int64_t)which * kTcRows + row) * D + from;
       }
-      T* dst = static_cast<T*>(half == 0 ? p.dk : p.dv) + (((int64_t)b * p.T + j) * p.Hk + hk) * D;
+      T* dst = static_cast<T*>(which == 0 ? p.dk : p.dv) + (((int64_t)b * p.T + j) * p.Hk + hk) * D + from;
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32) {
+      for (int c0 = 0; c0 < D / 2; c0 += 32) {
         uint32_t o[32];
         if (nit > 0) { tmem_ld32(acc + c0, o); tmem_wait_ld32(o); }
         if (parts) {
@@ -599,7 +590,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
             if (live) w = make_float4(__uint_as_float(o[v * 4]) * mul, __uint_as_float(o[v * 4 + 1]) * mul, __uint_as_float(o[v * 4 + 2]) * mul,
                                       __uint_as_float(o[v * 4 + 3]) * mul);
-            *reinterpret_cast<float4*>(part + c0 + v * 4) = w;
+            *reinterpret_cast<float4*>(sum + c0 + v * 4) = w;
           }
         } else if (j < p.T) {
 #pragma unroll
@@ -617,7 +608,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
     }
   }
-  tc_finish(tmem, 512, warp, 8, abort_flag, p.error_flag);
+  tc_finish(tmem, 512, warp, kBwdMma, abort_flag, p.error_flag);
 }
 
 // dK and dV of the key tiles that came in parts: blockIdx.x = (sample and key head, key tile), blockIdx.y a stretch of the tile.
