@@ -196,17 +196,18 @@ template <int D> struct FwdSmem {
 // maximum may lag behind by 8 (2^14 in all, far from the type's largest) before the output is rescaled.
 constexpr float kPShift = 6.f, kMaxLag = 8.f;
 constexpr int kPolyPairs = 2;
+constexpr float kNoWeight = 1e-30f;       // a row that sees anything has weights from 2^6 / 2^8 up: below this it has none
 
 // 32 columns of a row: P = 2^(score sc + off), its sums, and its values in the operand type.  Of every 8 pairs kPolyPairs go
-// through the polynomial (the MUFU pipe alone takes 1024 cycles for a tile); not where keys are hidden, which get exactly 0.
-template <typename T, bool kPoly>
+// through the polynomial (the MUFU pipe alone takes 1024 cycles for a tile); there a hidden key gets 2^-126 in place of 0.
+template <typename T>
 __device__ __forceinline__ void tc_weigh(const uint32_t* x, f32x2 sc2, f32x2 off2, f32x2 (&part)[2], uint32_t (&pk)[16]) {
 #pragma unroll
   for (int c = 0; c < 32; c += 2) {
     float e0, e1;
     unpack_f2(fma_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, off2), e0, e1);
     f32x2 e;
-    if (kPoly && (c >> 1) * kPolyPairs % 8 < kPolyPairs) e = exp2_poly(e0, e1);
+    if ((c >> 1) * kPolyPairs % 8 < kPolyPairs) e = exp2_poly(e0, e1);
     else e = pack_f2(ex2(e0), ex2(e1));
     part[c >> 1 & 1] = add_f2(part[c >> 1 & 1], e);
     unpack_f2(e, e0, e1);
@@ -398,7 +399,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           const uint32_t w = tc_seen(i - k0 - c0, i - p.window - k0 - c0, p.sinks - 1 - k0 - c0);
           if (__all_sync(0xffffffffu, w == 0xffffffffu)) continue;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) if (!(w >> c & 1u)) x[c0 + c] = 0xff800000u;
+          for (int c = 0; c < 32; ++c) if (!(w & 1u << c)) x[c0 + c] = 0xff800000u;
         }
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -430,8 +431,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
       for (int c0 = 0; c0 < 128; c0 += 32) {
         uint32_t pk[16];
-        if (whole) tc_weigh<T, true>(x + c0, sc2, off2, part, pk);
-        else tc_weigh<T, false>(x + c0, sc2, off2, part, pk);
+        tc_weigh<T>(x + c0, sc2, off2, part, pk);
         tmem_st16(ts + (c0 >> 1), pk);
         if (c0 == 32 || c0 == 96) {                               // the first half of P V starts under the second half's exponentials
           tmem_wait_st();
@@ -449,7 +449,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     tc_fence_after();
     if (ok) {
       const bool live = i < n && r.count() > 0;
-      const float inv = live ? (l > 0.f || l != l ? 1.f / l : 0.f) : 0.f;
+      const float inv = live ? (l > kNoWeight || l != l ? 1.f / l : 0.f) : 0.f;
       T* orow = static_cast<T*>(p.out) + (((int64_t)b * p.T + i) * p.Hq + h) * D;
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 32) {
@@ -469,7 +469,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           }
         }
       }
-      if (i < p.T && p.lse) p.lse[((int64_t)b * p.Hq + h) * p.T + i] = live && (l > 0.f || l != l) ? m + log2f(l) - kPShift : INFINITY;
+      if (i < p.T && p.lse) p.lse[((int64_t)b * p.Hq + h) * p.T + i] = live && (l > kNoWeight || l != l) ? m + log2f(l) - kPShift : INFINITY;
     }
   }
   tc_finish(tmem, 512, warp, 8, abort_flag, p.error_flag);

@@ -16,21 +16,20 @@ __device__ __forceinline__ float bwd_factor(float amax) {          // 2^(3 - e) 
   return e < -30 || e > 16 ? 1.f : __uint_as_float((uint32_t)(127 + 3 - e) << 23);
 }
 
-// Of every 8 pairs of exponentials kBwdPoly go through the polynomial where no key is hidden.
+// Of every 8 pairs of exponentials kBwdPoly go through the polynomial.  What belongs to hidden keys is replaced by 0 afterwards.
 constexpr int kBwdPoly = 3;
-template <bool kPoly>
 __device__ __forceinline__ f32x2 bwd_exp(int pair, f32x2 y) {
   float a, b;
   unpack_f2(y, a, b);
-  return kPoly && pair * kBwdPoly % 8 < kBwdPoly ? exp2_poly(a, b) : pack_f2(ex2(a), ex2(b));
+  return pair * kBwdPoly % 8 < kBwdPoly ? exp2_poly(a, b) : pack_f2(ex2(a), ex2(b));
 }
 // 32 columns of a row: x = scores, y = dP  ->  x = P (f dP + neg_delta)
-template <typename T, bool kPoly>
+template <typename T>
 __device__ __forceinline__ void bwd_ds(uint32_t (&x)[32], const uint32_t (&y)[32], float sc, float neg_lse, float f, float neg_delta) {
   const f32x2 sc2 = pack_f2(sc, sc), l2 = pack_f2(neg_lse, neg_lse), f2 = pack_f2(f, f), d2 = pack_f2(neg_delta, neg_delta);
 #pragma unroll
   for (int c = 0; c < 32; c += 2) {
-    const f32x2 pr = bwd_exp<kPoly>(c >> 1, fma_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, l2));
+    const f32x2 pr = bwd_exp(c >> 1, fma_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, l2));
     const f32x2 dp = pack_f2(__uint_as_float(y[c]), __uint_as_float(y[c + 1]));
     float a, b;
     unpack_f2(mul_f2(pr, BwdRange<T>::scaled ? fma_f2(dp, f2, d2) : add_f2(dp, d2)), a, b);
@@ -39,17 +38,16 @@ __device__ __forceinline__ void bwd_ds(uint32_t (&x)[32], const uint32_t (&y)[32
   }
 }
 // 32 columns of a key's row: x = scores  ->  x = P, with the columns' own log-sum-exps
-template <bool kPoly>
 __device__ __forceinline__ void bwd_probs(uint32_t (&x)[32], const float* lse, float sc) {
   const f32x2 sc2 = pack_f2(sc, sc);
 #pragma unroll
   for (int c = 0; c < 32; c += 4) {
     const float4 l = *reinterpret_cast<const float4*>(lse + c);   // negated
     float a, b;
-    unpack_f2(bwd_exp<kPoly>(c >> 1, fma_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, pack_f2(l.x, l.y))), a, b);
+    unpack_f2(bwd_exp(c >> 1, fma_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, pack_f2(l.x, l.y))), a, b);
     x[c] = __float_as_uint(a);
     x[c + 1] = __float_as_uint(b);
-    unpack_f2(bwd_exp<kPoly>((c >> 1) + 1, fma_f2(pack_f2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), sc2, pack_f2(l.z, l.w))), a, b);
+    unpack_f2(bwd_exp((c >> 1) + 1, fma_f2(pack_f2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), sc2, pack_f2(l.z, l.w))), a, b);
     x[c + 2] = __float_as_uint(a);
     x[c + 3] = __float_as_uint(b);
   }
@@ -262,7 +260,7 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (one_tile) {
         float sum = 0.f;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) if (seen >> c & 1u) sum += ex2(fmaf(__uint_as_float(x[c]), sc, -lse)) * __uint_as_float(y[c]);
+        for (int c = 0; c < 32; ++c) if (seen & 1u << c) sum += ex2(fmaf(__uint_as_float(x[c]), sc, -lse)) * __uint_as_float(y[c]);
         float* s_sum = reinterpret_cast<float*>(smem + L::k + L::tile);        // [4][128] in a stage that a single tile leaves unused
         s_sum[part * 128 + row] = sum;
         asm volatile("bar.sync 1, 512;" ::: "memory");
@@ -270,11 +268,10 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (part == 0 && i < p.T) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = live ? sum : 0.f;
         delta = sum * f;
       }
-      if (whole) bwd_ds<T, true>(x, y, sc, -lse, f, -delta);
-      else bwd_ds<T, false>(x, y, sc, -lse, f, -delta);
+      bwd_ds<T>(x, y, sc, -lse, f, -delta);
       if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
 #pragma unroll
-        for (int c = 0; c < 32; ++c) if (!(seen >> c & 1u)) x[c] = 0u;
+        for (int c = 0; c < 32; ++c) if (!(seen & 1u << c)) x[c] = 0u;
       }
       uint32_t pk[16];
 #pragma unroll
@@ -522,8 +519,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tmem_ld32(ts, x);
       tmem_wait_ld32(x);
       const bool whole = k0 + kTcRows - 1 <= q0 && (q0 + kTcRows - 1 - k0 < p.window || k0 + kTcRows <= p.sinks);
-      if (whole) bwd_probs<true>(x, st, sc);
-      else bwd_probs<false>(x, st, sc);
+      bwd_probs(x, st, sc);
       if (!whole) {
         // query i = base + c sees key j when c >= j - base, and c < j - base + window or j is a sink
         const int base = q0 + 32 * part;
@@ -531,7 +527,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const uint32_t w = tc_upto(last) & ~tc_upto(j - base - 1);
         if (!__all_sync(0xffffffffu, w == 0xffffffffu)) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) if (!(w >> c & 1u)) x[c] = 0u;
+          for (int c = 0; c < 32; ++c) if (!(w & 1u << c)) x[c] = 0u;
         }
       }
       uint32_t pk[16];
