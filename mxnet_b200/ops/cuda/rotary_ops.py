@@ -9,16 +9,15 @@ _POS = {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int64: 3}
 
 
 def _run(x, positions, inv_freq, interleaved, scale, backward):
-    B, T, H, D = shape = x.shape
-    dtype = x.dtype
-    y = torch.empty(shape, dtype=dtype, device=x.device)
+    B, T, H, D = x.shape
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     sb, st, sh, _ = x.stride()
     if positions.dim() == 2:
         pos_sb, pos_st = positions.stride()
     else:
         pos_sb, pos_st = 0, positions.stride(0)
     with on_device(x):
-        check(lib().mxb_rotary(DT[dtype], x.data_ptr(), y.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), B, T, H, D,
+        check(lib().mxb_rotary(DT[x.dtype], x.data_ptr(), y.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), B, T, H, D,
                                2 * inv_freq.shape[0], sb, st, sh, pos_sb, pos_st, _POS[positions.dtype],
                                1 if inv_freq.dtype == torch.float64 else 0, interleaved, scale, backward, raw_stream(x)), 'rotary_embedding')
     count_launch(1)

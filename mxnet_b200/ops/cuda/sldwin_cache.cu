@@ -190,7 +190,7 @@ __device__ __forceinline__ float ld_cluster_f32(const float* local, uint32_t ran
 
 // blockIdx.x = ((sample, key head, chunk of 8 query heads), rank in the cluster)
 template <typename T, int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 step_tc_kernel(const StepParams p, int chunks, int csize) {
   constexpr int C16 = D / 64;                             // 64-channel parts of a row
   extern __shared__ float sm[];                           // [warps][8 heads][D + 2]: partial outputs, then m and l
@@ -343,12 +343,20 @@ static int step_tc(const StepParams& p, cudaStream_t st) {
   const int group = p.Hq / p.Hk, chunks = (group + 7) / 8;
   const int64_t units = (int64_t)p.B * p.Hk * chunks;
   const int64_t most = (int64_t)p.sinks + p.window < p.C ? (int64_t)p.sinks + p.window : p.C;      // keys that a token may see
-  // A cluster grows while its CTAs are too few to fill the device and every warp still has 16 keys to take.
-  int csize = 1;
-  const int nw = 4;
-  while (csize < 8 && units * csize < 12 * (int64_t)sm_count() && most > (int64_t)csize * nw * 16) csize <<= 1;
+  // A cluster grows while its CTAs leave SMs short of the four that fit one and every warp still has 16 keys to take (512 units of
+  // 4100 keys, head size 128: no cluster 176 us, clusters of 2 186 us, of 4 198 us).  Where clusters of 8 give no SM a second CTA,
+  // CTAs get 8 warps, and clusters 16 CTAs if keys are many (8 units of 131072 keys: 8 CTAs x 4 warps 370 us, 8 x 8 213 us, 16 x 8
+  // 155 us, 16 x 16 170 us).
+  int csize = 1, nw = 4;
+  while (csize < 8 && units * csize < 3 * (int64_t)sm_count() && most > (int64_t)csize * nw * 16) csize <<= 1;
+  if (csize == 8 && units * csize <= 2 * (int64_t)sm_count() && most > 8 * 8 * 16) {
+    nw = 8;
+    if (units * 16 <= 2 * (int64_t)sm_count() && most > 16 * 8 * 16) csize = 16;
+  }
   if (units * csize > 0x7fffffff) return -2;
   const size_t smem = (size_t)(nw + 1) * 8 * (D + 2) * sizeof(float);
+  static unsigned long long seen = 0;
+  if (first_on_device(&seen)) cudaFuncSetAttribute(step_tc_kernel<T, D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(units * csize));
   cfg.blockDim = dim3(nw * 32);

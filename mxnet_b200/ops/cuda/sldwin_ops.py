@@ -43,9 +43,9 @@ def _rows(t):
 
 
 def _forward(q, k, v, valid, window, sinks, scale, keep):
-    B, T, Hq, D = shape = q.shape
+    B, T, Hq, D = q.shape
     dtype, dev = q.dtype, q.device
-    out = torch.empty(shape, dtype=dtype, device=dev)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev) if keep else None
     dims = _DIMS7(B, T, Hq, k.shape[2], D, window, sinks)
     strides = _S12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
@@ -69,13 +69,13 @@ class _SldwinAttention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, valid, out, lse = ctx.saved_tensors
         window, sinks, scale = ctx.args
-        B, T, Hq, D = shape = q.shape
+        B, T, Hq, D = q.shape
         kshape = k.shape
         dtype, dev = q.dtype, q.device
         dout = _rows(dout)
-        dq = torch.empty(shape, dtype=dtype, device=dev)
-        dk = torch.empty(kshape, dtype=dtype, device=dev)
-        dv = torch.empty(kshape, dtype=dtype, device=dev)
+        dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+        dv = torch.empty_like(v, memory_format=torch.contiguous_format)
         dims = _DIMS7(B, T, Hq, kshape[2], D, window, sinks)
         strides = _S12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *dout.stride()[:3])
         L, code = lib(), DT[dtype]
@@ -126,11 +126,11 @@ def _dense(t):
 
 
 def attention_step(q, k, v, key_cache, value_cache, positions, window, sinks, scale):
-    B, Hq, D = shape = q.shape
+    B, Hq, D = q.shape
     q, k, v = _dense(q), _dense(k), _dense(v)
     if positions.dtype != torch.int64 or not positions.is_contiguous():
         positions = positions.to(torch.int64).contiguous()
-    out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q)
     dims = _DIMS7(B, Hq, k.shape[1], D, key_cache.shape[1], window, sinks)
     strides = _S6(*key_cache.stride()[:3], *value_cache.stride()[:3])
     with on_device(q):

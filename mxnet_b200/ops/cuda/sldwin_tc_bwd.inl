@@ -625,6 +625,7 @@ sw_dkv_join_kernel(const TcParams p, const DkvSplit sp) {
     for (int hs = 0; hs < sp.hsplit; ++hs) {
       take(dkv_near_part(sp, all, hs, bh, kt, D));
       if (kt < sp.sink_tiles)
+#pragma unroll 4
         for (int c = 0; c < sp.far_chunks; ++c) take(dkv_far_part(sp, all, hs, c, bh, kt, D));
     }
     T* dst = static_cast<T*>(which == 0 ? p.dk : p.dv) + (((int64_t)b * p.T + j) * p.Hk + hk) * D + d;
