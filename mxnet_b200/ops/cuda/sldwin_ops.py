@@ -105,6 +105,8 @@ def _int32(valid):
     """Lengths as the kernels read them (real ones are cut, values beyond 32 bits stay beyond every length)."""
     if valid.dtype == torch.int32 and valid.is_contiguous():
         return valid
+    if not valid.is_floating_point():
+        valid = valid.long()                                      # narrow and unsigned types do not hold the bounds below
     return valid.clamp(-1, (1 << 31) - 128).to(torch.int32).contiguous()
 
 

@@ -265,13 +265,14 @@ def _cache_args(name, key_cache, value_cache, B, Hk, D, sinks, like):
     if key_cache is not None and value_cache is not None and key_cache.dim() == 4:
         n = key_cache.shape
         if n[0] == B and n[2] == Hk and n[3] == D and n[1] > sinks and value_cache.shape == n and _alike(like, key_cache, value_cache) and \
-                (B == 0 or (_adjacent(key_cache) and _adjacent(value_cache))):
+                (B == 0 or (_adjacent(key_cache) and _adjacent(value_cache) and key_cache.data_ptr() != value_cache.data_ptr())):
             return
     _need(key_cache is not None and value_cache is not None, '%s: key_cache and value_cache are required', name)
     _need(key_cache.dim() == 4 and tuple(key_cache.shape[:1] + key_cache.shape[2:]) == (B, Hk, D) and value_cache.shape == key_cache.shape,
           '%s: caches must be (%d, C, %d, %d), got %s and %s', name, B, Hk, D, tuple(key_cache.shape), tuple(value_cache.shape))
     _same(name, like, key_cache=key_cache, value_cache=value_cache)
     _need(key_cache.shape[1] > sinks, '%s: a cache of %d rows has no room beside %d sinks', name, key_cache.shape[1], sinks)
+    _need(key_cache.data_ptr() != value_cache.data_ptr(), '%s: keys and values need caches of their own', name)
     raise MXNetError('%s: the channels of a cache must be adjacent, and no axis an expanded one' % name)
 
 
@@ -295,7 +296,8 @@ def sldwin_cache_fill(key, value=None, key_cache=None, value_cache=None, valid_l
     ``key``, ``value``: (B, T, Hk, D) of positions 0 .. T - 1; ``key_cache``, ``value_cache``: (B, C, Hk, D), C > sinks.  A cache
     keeps position p in row p while ``p < sinks`` and in row ``sinks + (p - sinks) % (C - sinks)`` behind: of a prompt longer than
     the cache the sinks and the last ``C - sinks`` positions stay.  ``valid_length``: (B,) lengths of the prompts (clipped to
-    0 .. T).  Rows of the caches that no position falls on are left as they were.  Returns the caches."""
+    0 .. T).  Rows of the caches that no position falls on are left as they were.  The caches may be views of larger arrays but must
+    not overlap one another, the keys or the values.  Returns the caches."""
     name = 'sldwin_cache_fill'
     _need(value is not None, '%s: key and value are required', name)
     _need(key.dim() == 4 and value.shape == key.shape, '%s: key and value must be (B, T, H, D), got %s and %s', name, tuple(key.shape),

@@ -115,6 +115,32 @@ def test_attention_ragged_and_what_lies_behind(dtype, D, window, sinks):
             assert not bool(b.masked_select(behind.expand_as(b)).any())
 
 
+@pytest.mark.parametrize('dtype', [torch.uint8, torch.int16, torch.int64, torch.float32, torch.float64])
+def test_lengths_of_any_number_type(dtype):
+    q, k, v = (randn(3, 140, 2, 64, dtype=torch.float16) for _ in range(3))
+    lengths = torch.tensor([0, 97, 140], device=dev())
+    want = op('sldwin_attention')(q, k, v, lengths.to(torch.int32), window=33)
+    assert torch.equal(op('sldwin_attention')(q, k, v, lengths.to(dtype), window=33), want)
+    assert torch.equal(op('sldwin_attention')(q, k, v, lengths.to(dtype).reshape(3, 1), window=33), want)
+    if dtype in (torch.int64, torch.float64):      # numbers that 32 bits do not hold are beyond every length, or below 0
+        huge = torch.tensor([-(10 ** 12), 97, 10 ** 12], device=dev()).to(dtype)
+        assert torch.equal(op('sldwin_attention')(q, k, v, huge, window=33), want)
+    caches = [torch.zeros(2, 3, 50, 2, 64, device=dev(), dtype=torch.float16) for _ in range(2)]
+    op('sldwin_cache_fill')(k, v, caches[0][0], caches[0][1], lengths.to(torch.int32), sinks=2)
+    op('sldwin_cache_fill')(k, v, caches[1][0], caches[1][1], lengths.to(dtype), sinks=2)
+    assert torch.equal(*caches)
+
+
+def test_a_reported_time_out_is_raised_by_the_next_call():
+    from mxnet_b200.ops.cuda import sldwin_ops
+    q = randn(1, 20, 1, 64, dtype=torch.float16)
+    want = op('sldwin_attention')(q, q, q)
+    sldwin_ops._report[2].value = 1               # what a kernel writes whose wait ran out
+    with pytest.raises(RuntimeError, match='time-out'):
+        op('sldwin_attention')(q, q, q)
+    assert torch.equal(op('sldwin_attention')(q, q, q), want)
+
+
 @pytest.mark.parametrize('D', [64, 128, 20])
 def test_attention_takes_views(D):
     T, dtype = 200, torch.bfloat16
@@ -282,6 +308,43 @@ def test_a_decoder_step_by_step_is_the_whole_sequence(npx, dtype, bound):
     # outputs of up to 4 in size: both sides round probabilities and the output, 4 half steps of 4 in all (bf16: 4 * 4 * 2^-8)
     run_decoder('cuda', dtype, npx, bound)
     run_decoder('cuda', dtype, npx, bound, T=150, more=9, window=140, sinks=3, D=64)
+
+
+def test_step_of_one_long_sequence():
+    """Few key heads and very many keys: the widest clusters."""
+    C, D = 70000, 128
+    q, k, v = (randn(1, h, D, dtype=torch.bfloat16) for h in (4, 2, 2))
+    kc, vc = randn(1, C, 2, D, dtype=torch.bfloat16), randn(1, C, 2, D, dtype=torch.bfloat16)
+    for window, pos in ((0, C - 1), (60000, 5 * C + 3), (300, 3 * C)):
+        got = op('sldwin_attention_step')(q, k, v, kc, vc, torch.tensor([pos], device=dev()), window=window, sinks=4)
+        # the definition on the rows that are seen, in 64 bits
+        held = torch.arange(C, device=dev())
+        held = torch.where(held < 4, held, pos - (pos - held) % (C - 4))
+        seen = (held <= pos) & ((held < 4) | ((held >= 4) & ((pos - held < window) if window else (held >= 0))))
+        K, V = kc[0, seen].double().repeat_interleave(2, 1), vc[0, seen].double().repeat_interleave(2, 1)
+        P = (torch.einsum('hd,khd->hk', q[0].double(), K) / math.sqrt(D)).softmax(-1)
+        want = torch.einsum('hk,khd->hd', P, V).cpu()[None]
+        mass = torch.einsum('hk,khd->hd', P, V.abs()).cpu()[None]
+        e = oracle.half(torch.bfloat16)
+        oracle.check(got, want, (e + oracle.FP32) * mass + e * want.abs())
+
+
+def test_caches_beyond_two_to_the_31_elements():
+    B, C, H, D = 3, 90000, 64, 128                # sample 2 starts at element 1.47e9, its last row lies behind 2^31
+    kc, vc = (torch.zeros(B, C, H, D, dtype=torch.float16, device=dev()) for _ in range(2))
+    k, v = (randn(B, 100, H, D, dtype=torch.float16) for _ in range(2))
+    q1, k1, v1 = (randn(B, H, D, dtype=torch.float16) for _ in range(3))
+    op('sldwin_cache_fill')(k, v, kc, vc, sinks=4)
+    assert torch.equal(kc[:, :100], k) and torch.equal(vc[:, :100], v)
+    kc[:, -100:], vc[:, -100:] = k, v
+    got = op('sldwin_attention_step')(q1, k1, v1, kc, vc, torch.full((B,), C - 1, device=dev()), window=60, sinks=4)
+    assert torch.equal(kc[:, -1], k1) and torch.equal(vc[:, -1], v1)
+    at = [0, 1, 2, 3] + list(range(C - 60, C))
+    K, V = kc[:, at].double(), vc[:, at].double()
+    P = (torch.einsum('bhd,bkhd->bhk', q1.double(), K) / math.sqrt(D)).softmax(-1)
+    want, mass = (torch.einsum('bhk,bkhd->bhd', P, t).cpu() for t in (V, V.abs()))
+    e = oracle.half(torch.float16)
+    oracle.check(got, want, (e + oracle.FP32) * mass + e * want.abs() + oracle.least(torch.float16))
 
 
 # -------------------------------------------------------------------------------------------------------- log probs

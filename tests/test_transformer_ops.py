@@ -269,6 +269,15 @@ def test_caches_refuse(change, attrs):
                                          positions=arr(torch.zeros(2)), **caches, **attrs)
 
 
+def test_caches_refuse_to_be_one_array():
+    c = arr(torch.zeros(2, 6, 2, 8))
+    with pytest.raises(MXNetError):
+        nd.contrib.sldwin_cache_fill(arr(torch.zeros(2, 4, 2, 8)), arr(torch.zeros(2, 4, 2, 8)), c, c)
+    with pytest.raises(MXNetError):
+        nd.contrib.sldwin_attention_step(arr(torch.zeros(2, 4, 8)), arr(torch.zeros(2, 2, 8)), arr(torch.zeros(2, 2, 8)), c, c,
+                                         arr(torch.zeros(2)))
+
+
 def test_step_and_fill_refuse_to_be_recorded():
     q, k, kc = arr(torch.zeros(2, 4, 8)), arr(torch.zeros(2, 2, 8)), arr(torch.zeros(2, 6, 2, 8))
     q.attach_grad()
