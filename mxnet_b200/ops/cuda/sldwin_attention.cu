@@ -235,12 +235,17 @@ static bool sw_shape_ok(const SwParams& p) {
          p.window <= p.T && p.sinks >= 0 && p.sinks <= p.T && p.T <= (1 << 30) && (int64_t)p.B * p.Hq <= 0x7fffffff;
 }
 
-static SwParams sw_params(const int* dims, const int64_t* strides, float scale) {
+// form: B, T, Hq, Hk, D, window (1 .. T), sinks (0 .. T), then the element strides of batch, position and head of q, k, v (and dO in
+// the backward pass); channels are adjacent.  A size beyond 32 bits reads as -1, which no check passes.
+static SwParams sw_params(const int64_t* form, bool strides, float scale) {
+  auto size = [&](int i) { return form[i] > 0x7fffffff ? -1 : (int)form[i]; };
   SwParams p{};
-  p.B = dims[0]; p.T = dims[1]; p.Hq = dims[2]; p.Hk = dims[3]; p.D = dims[4]; p.window = dims[5]; p.sinks = dims[6];
-  p.sq = {strides[0], strides[1], strides[2]};
-  p.sk = {strides[3], strides[4], strides[5]};
-  p.sv = {strides[6], strides[7], strides[8]};
+  p.B = size(0); p.T = size(1); p.Hq = size(2); p.Hk = size(3); p.D = size(4); p.window = size(5); p.sinks = size(6);
+  if (strides) {
+    p.sq = {form[7], form[8], form[9]};
+    p.sk = {form[10], form[11], form[12]};
+    p.sv = {form[13], form[14], form[15]};
+  }
   p.scale = scale;
   return p;
 }
@@ -254,11 +259,10 @@ using namespace mxb;
 
 MXB_EXPORT int mxb_sldwin_max_dim(void) { return kSwMaxD; }
 
-// dims: B, T, Hq, Hk, D, window (1 .. T), sinks (0 .. T).  strides: batch, position and head of q, k, v (and dO), in elements;
-// channels are adjacent.  lse: [B, Hq, T] floats (forward: may be null when no backward pass follows).
+// lse: [B, Hq, T] floats (may be null when no backward pass follows).
 MXB_EXPORT int mxb_sldwin_forward(int dtype, const void* q, const void* k, const void* v, const int* valid, void* out, float* lse,
-                                  const int* dims, const int64_t* strides, float scale, int* error_flag, void* stream) {
-  SwParams p = sw_params(dims, strides, scale);
+                                  const int64_t* form, float scale, int* error_flag, void* stream) {
+  SwParams p = sw_params(form, true, scale);
   p.q = q; p.k = k; p.v = v; p.valid = valid; p.out = out; p.lse = lse;
   if (!sw_shape_ok(p)) return -2;
   cudaStream_t st = (cudaStream_t)stream;
@@ -276,11 +280,11 @@ MXB_EXPORT int mxb_sldwin_forward(int dtype, const void* q, const void* k, const
 // mxb_sldwin_backward_parts floats of workspace (may be null when that is 0).
 MXB_EXPORT int mxb_sldwin_backward(int dtype, const void* q, const void* k, const void* v, const int* valid, const void* o,
                                    const void* dout, const float* lse, float* delta, float* parts, void* dq, void* dk, void* dv,
-                                   const int* dims, const int64_t* strides, float scale, int* error_flag, void* stream) {
-  SwParams p = sw_params(dims, strides, scale);
+                                   const int64_t* form, float scale, int* error_flag, void* stream) {
+  SwParams p = sw_params(form, true, scale);
   p.q = q; p.k = k; p.v = v; p.valid = valid; p.o = o; p.dout = dout; p.lse = const_cast<float*>(lse); p.delta = delta;
   p.dq = dq; p.dk = dk; p.dv = dv;
-  p.sdo = {strides[9], strides[10], strides[11]};
+  p.sdo = {form[16], form[17], form[18]};
   if (!sw_shape_ok(p)) return -2;
   cudaStream_t st = (cudaStream_t)stream;
   if (tc_takes(p, dtype) && tc_layout_ok(dout, p.sdo, p.B, p.T, p.Hq)) {
@@ -294,9 +298,8 @@ MXB_EXPORT int mxb_sldwin_backward(int dtype, const void* q, const void* k, cons
 }
 
 // Floats of workspace for sums that come in parts (0 for shapes that only the general kernels take).
-MXB_EXPORT int64_t mxb_sldwin_backward_parts(int dtype, const int* dims) {
-  const int64_t none[12] = {0};
-  const SwParams p = sw_params(dims, none, 1.f);
+MXB_EXPORT int64_t mxb_sldwin_backward_parts(int dtype, const int64_t* form) {
+  const SwParams p = sw_params(form, false, 1.f);
   if (!sw_shape_ok(p) || (p.D != 64 && p.D != 128) || (dtype != kF16 && dtype != kBF16)) return 0;
   return dkv_part_floats(p);
 }

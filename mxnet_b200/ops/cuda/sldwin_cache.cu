@@ -374,13 +374,15 @@ static int step_tc(const StepParams& p, cudaStream_t st) {
 
 using namespace mxb;
 
-// dims: B, T, H, D, C, sinks (0 .. C - 1).  strides: batch, position, head of k, v, key cache, value cache, in elements.
-MXB_EXPORT int mxb_cache_fill(int dtype, const void* k, const void* v, void* kc, void* vc, const int* valid, const int* dims,
-                              const int64_t* s, void* stream) {
+// form: B, T, H, D, C, sinks (0 .. C - 1), then the element strides of batch, position and head of k, v, key cache and value cache.
+MXB_EXPORT int mxb_cache_fill(int dtype, const void* k, const void* v, void* kc, void* vc, const int* valid, const int64_t* form,
+                              void* stream) {
   if (dtype < kF32 || dtype > kBF16) return -1;
   FillParams p{};
   p.k = k; p.v = v; p.kc = kc; p.vc = vc; p.valid = valid;
-  p.B = dims[0]; p.T = dims[1]; p.H = dims[2]; p.D = dims[3]; p.C = dims[4]; p.sinks = dims[5];
+  for (int i = 0; i < 6; ++i) if (form[i] < 0 || form[i] > 0x7fffffff) return -2;
+  p.B = (int)form[0]; p.T = (int)form[1]; p.H = (int)form[2]; p.D = (int)form[3]; p.C = (int)form[4]; p.sinks = (int)form[5];
+  const int64_t* s = form + 6;
   p.sk = {s[0], s[1], s[2]}; p.sv = {s[3], s[4], s[5]}; p.skc = {s[6], s[7], s[8]}; p.svc = {s[9], s[10], s[11]};
   if (p.B < 1 || p.B > 65535 || p.T < 1 || p.H < 1 || p.D < 1 || p.sinks < 0 || p.C <= p.sinks) return -2;
   if ((int64_t)p.H * p.D > (1 << 30)) return -2;
@@ -403,12 +405,15 @@ MXB_EXPORT int mxb_cache_fill(int dtype, const void* k, const void* v, void* kc,
   return (int)cudaGetLastError();
 }
 
-// dims: B, Hq, Hk, D, C, window (1 .. C - sinks), sinks.  strides: batch, row, head of the key and the value cache.
+// form: B, Hq, Hk, D, C, window (1 .. C - sinks), sinks, then the element strides of batch, row and head of the key and the value cache.
 MXB_EXPORT int mxb_sldwin_step(int dtype, const void* q, const void* k, const void* v, void* kc, void* vc, const int64_t* pos, void* out,
-                               const int* dims, const int64_t* s, float scale, void* stream) {
+                               const int64_t* form, float scale, void* stream) {
   StepParams p{};
   p.q = q; p.k = k; p.v = v; p.kc = kc; p.vc = vc; p.pos = pos; p.out = out;
-  p.B = dims[0]; p.Hq = dims[1]; p.Hk = dims[2]; p.D = dims[3]; p.C = dims[4]; p.window = dims[5]; p.sinks = dims[6];
+  for (int i = 0; i < 7; ++i) if (form[i] < 0 || form[i] > 0x7fffffff) return -2;
+  p.B = (int)form[0]; p.Hq = (int)form[1]; p.Hk = (int)form[2]; p.D = (int)form[3]; p.C = (int)form[4]; p.window = (int)form[5];
+  p.sinks = (int)form[6];
+  const int64_t* s = form + 7;
   p.skc = {s[0], s[1], s[2]}; p.svc = {s[3], s[4], s[5]};
   p.scale = scale;
   if (p.B < 1 || p.Hk < 1 || p.Hq < p.Hk || p.Hq % p.Hk || p.D < 1 || p.D > kStepMaxD || p.sinks < 0 || p.C <= p.sinks ||

@@ -8,8 +8,7 @@ from torch.autograd.function import once_differentiable
 from . import lib, count_launch, check
 from ._util import DT, address, on_device, raw_stream
 
-_DIMS7, _DIMS6 = C.c_int * 7, C.c_int * 6
-_S6, _S12 = C.c_int64 * 6, C.c_int64 * 12
+_I13, _I16, _I18, _I19 = C.c_int64 * 13, C.c_int64 * 16, C.c_int64 * 18, C.c_int64 * 19      # sizes, then strides
 
 
 _report = []          # a word of pinned host memory that the kernels set when a wait inside them ran out, and its reader
@@ -47,11 +46,11 @@ def _forward(q, k, v, valid, window, sinks, scale, keep):
     dtype, dev = q.dtype, q.device
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev) if keep else None
-    dims = _DIMS7(B, T, Hq, k.shape[2], D, window, sinks)
-    strides = _S12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    (q0, q1, q2, _), (k0, k1, k2, _), (v0, v1, v2, _) = q.stride(), k.stride(), v.stride()
+    form = _I16(B, T, Hq, k.shape[2], D, window, sinks, q0, q1, q2, k0, k1, k2, v0, v1, v2)
     with on_device(q):
         check(lib().mxb_sldwin_forward(DT[dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), address(valid), out.data_ptr(), address(lse),
-                                       dims, strides, scale, _error_word(), raw_stream(q)), 'sldwin_attention')
+                                       form, scale, _error_word(), raw_stream(q)), 'sldwin_attention')
     count_launch(1)
     return out, lse
 
@@ -76,18 +75,18 @@ class _SldwinAttention(torch.autograd.Function):
         dq = torch.empty_like(q, memory_format=torch.contiguous_format)
         dk = torch.empty_like(k, memory_format=torch.contiguous_format)
         dv = torch.empty_like(v, memory_format=torch.contiguous_format)
-        dims = _DIMS7(B, T, Hq, kshape[2], D, window, sinks)
-        strides = _S12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *dout.stride()[:3])
+        (q0, q1, q2, _), (k0, k1, k2, _), (v0, v1, v2, _), (g0, g1, g2, _) = q.stride(), k.stride(), v.stride(), dout.stride()
+        form = _I19(B, T, Hq, kshape[2], D, window, sinks, q0, q1, q2, k0, k1, k2, v0, v1, v2, g0, g1, g2)
         L, code = lib(), DT[dtype]
         # workspace: rowsum(dO * O) and the largest |dO| of each query tile, then key gradients that several blocks sum up
         rows = (B * Hq * (T + (T + 127) // 128) + 3) // 4 * 4
-        parts = L.mxb_sldwin_backward_parts(code, dims)
+        parts = L.mxb_sldwin_backward_parts(code, form)
         work = torch.empty(rows + parts, dtype=torch.float32, device=dev)
         at = work.data_ptr()
         with on_device(q):
             check(L.mxb_sldwin_backward(code, q.data_ptr(), k.data_ptr(), v.data_ptr(), address(valid), out.data_ptr(), dout.data_ptr(),
                                         lse.data_ptr(), at, at + 4 * rows if parts else 0, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                        dims, strides, scale, _error_word(), raw_stream(q)), 'sldwin_attention backward')
+                                        form, scale, _error_word(), raw_stream(q)), 'sldwin_attention backward')
         count_launch(3 if parts else 2)
         return dq, dk, dv, None, None, None, None
 
@@ -115,11 +114,11 @@ def cache_fill(k, v, key_cache, value_cache, valid, sinks):
     k, v = _rows(k), _rows(v)
     if valid is not None:
         valid = _int32(valid)
-    dims = _DIMS6(B, T, H, D, key_cache.shape[1], sinks)
-    strides = _S12(*k.stride()[:3], *v.stride()[:3], *key_cache.stride()[:3], *value_cache.stride()[:3])
+    (k0, k1, k2, _), (v0, v1, v2, _), (a0, a1, a2, _), (b0, b1, b2, _) = k.stride(), v.stride(), key_cache.stride(), value_cache.stride()
+    form = _I18(B, T, H, D, key_cache.shape[1], sinks, k0, k1, k2, v0, v1, v2, a0, a1, a2, b0, b1, b2)
     with on_device(k):
         check(lib().mxb_cache_fill(DT[k.dtype], k.data_ptr(), v.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), address(valid),
-                                   dims, strides, raw_stream(k)), 'sldwin_cache_fill')
+                                   form, raw_stream(k)), 'sldwin_cache_fill')
     count_launch(1)
 
 
@@ -133,10 +132,10 @@ def attention_step(q, k, v, key_cache, value_cache, positions, window, sinks, sc
     if positions.dtype != torch.int64 or not positions.is_contiguous():
         positions = positions.to(torch.int64).contiguous()
     out = torch.empty_like(q)
-    dims = _DIMS7(B, Hq, k.shape[1], D, key_cache.shape[1], window, sinks)
-    strides = _S6(*key_cache.stride()[:3], *value_cache.stride()[:3])
+    (a0, a1, a2, _), (b0, b1, b2, _) = key_cache.stride(), value_cache.stride()
+    form = _I13(B, Hq, k.shape[1], D, key_cache.shape[1], window, sinks, a0, a1, a2, b0, b1, b2)
     with on_device(q):
         check(lib().mxb_sldwin_step(DT[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-                                    positions.data_ptr(), out.data_ptr(), dims, strides, scale, raw_stream(q)), 'sldwin_attention_step')
+                                    positions.data_ptr(), out.data_ptr(), form, scale, raw_stream(q)), 'sldwin_attention_step')
     count_launch(1)
     return out

@@ -12,6 +12,7 @@ import math
 import torch
 
 from .registry import register
+from .cuda import logprob_ops, rotary_ops, sldwin_ops
 from .. import env
 from ..base import MXNetError
 
@@ -28,13 +29,11 @@ def _kernels(t):
     return t.is_cuda and t.dtype in _KERNEL_TYPES and t.numel() > 0 and env.get('MXNET_B200_KERNELS')
 
 
-def _alike(first, *others):
+def _alike(first, second, third):
     """Floating-point arrays of one type on one device."""
-    t, dev = first.dtype, first.device
-    for o in others:
-        if o.dtype is not t or o.device != dev:
-            return False
-    return t.is_floating_point
+    t, dev = first.dtype, first.get_device()
+    return t is second.dtype and t is third.dtype and dev == second.get_device() and dev == third.get_device() and t.is_floating_point and \
+        (dev >= 0 or first.device == second.device == third.device)
 
 
 def _plain(t):
@@ -108,13 +107,11 @@ def rotary_inv_freq(dim=64, base=10000.0, scaling='none', factor=1.0, original_l
 
 
 def _rotary_fits(data, positions, inv_freq):
-    if data.dim() != 4:
-        return False
-    B, T, _, D = data.shape
-    at = positions.shape
-    return data.is_floating_point() and (at == (T,) or at == (B, T)) and inv_freq.dim() == 1 and 1 <= inv_freq.shape[0] <= D // 2 and \
-        inv_freq.is_floating_point() and not positions.is_complex() and positions.dtype != torch.bool and \
-        positions.device == data.device and inv_freq.device == data.device
+    n, at, dev = data.shape, positions.shape, data.get_device()
+    return len(n) == 4 and data.is_floating_point() and (at == n[:2] or at == n[1:2]) and inv_freq.dim() == 1 and \
+        1 <= inv_freq.shape[0] <= n[3] // 2 and inv_freq.is_floating_point() and not positions.is_complex() and \
+        positions.dtype is not torch.bool and positions.get_device() == dev and inv_freq.get_device() == dev and \
+        (dev >= 0 or positions.device == data.device == inv_freq.device)
 
 
 def _rotary_refuse(name, data, positions, inv_freq):
@@ -146,7 +143,6 @@ def rotary_embedding(data, positions=None, inv_freq=None, interleaved=False, sca
     B, T, H, D = data.shape
     positions, inv_freq, scale = _plain(positions), _plain(inv_freq), float(scale)
     if _kernels(data) and D <= 1024 and H <= 4096 and B * T < (1 << 30):
-        from .cuda import rotary_ops
         return rotary_ops.rotary_embedding(data, positions, inv_freq, 1 if interleaved else 0, scale)
     R = 2 * inv_freq.shape[0]
     x = _work(data)
@@ -173,11 +169,9 @@ def _window_args(name, window, sinks, scale, D):
 
 
 def _heads_fit(query, key, value, axes):
-    if query.dim() != axes or key.dim() != axes:
-        return False
     qs, ks = query.shape, key.shape
-    return qs[:-2] == ks[:-2] and qs[-1] == ks[-1] and ks == value.shape and ks[-2] >= 1 and qs[-2] % ks[-2] == 0 and qs[-1] >= 1 and \
-        _alike(query, key, value)
+    return len(qs) == axes and len(ks) == axes and ks == value.shape and qs[0] == ks[0] and (axes == 3 or qs[1] == ks[1]) and \
+        qs[-1] == ks[-1] >= 1 and ks[-2] >= 1 and qs[-2] % ks[-2] == 0 and _alike(query, key, value)
 
 
 def _heads_refuse(name, query, key, value, lead):
@@ -232,7 +226,6 @@ def sldwin_attention(query, key=None, value=None, valid_length=None, window=0, s
     window, sinks, scale = _window_args(name, window, sinks, scale, D)
     valid = _lengths(name, valid_length, B, query.device)
     if _kernels(query) and D <= 256 and T <= (1 << 30):
-        from .cuda import sldwin_ops
         # a window of T sees everything, and more sinks than T are T
         return sldwin_ops.attention(query, key, value, valid, min(window, T) or T, min(sinks, T), scale)
     if query.numel() == 0:
@@ -312,7 +305,6 @@ def sldwin_cache_fill(key, value=None, key_cache=None, value_cache=None, valid_l
     if key.numel() == 0:
         return key_cache, value_cache
     if _kernels(key) and B <= 65535:
-        from .cuda import sldwin_ops
         sldwin_ops.cache_fill(key, value, key_cache, value_cache, valid, sinks)
         _written(key_cache, value_cache)
         return key_cache, value_cache
@@ -360,7 +352,6 @@ def sldwin_attention_step(query, key=None, value=None, key_cache=None, value_cac
     ring = key_cache.shape[1] - sinks
     window = min(window, ring) or ring
     if _kernels(query) and D <= 256:
-        from .cuda import sldwin_ops
         out = sldwin_ops.attention_step(query, key, value, key_cache, value_cache, positions, window, sinks, scale)
         _written(key_cache, value_cache)
         return out
@@ -417,7 +408,6 @@ def token_log_probs(logits, tokens=None, topk=0, ignore_label=-1):
     if tok.dtype != torch.int64:
         tok = tok.long()
     if _kernels(logits) and V < (1 << 31) - 1024:
-        from .cuda import logprob_ops
         res = logprob_ops.token_log_probs(x.contiguous(), tok.contiguous(), k, ignore)
     else:
         res = _token_log_probs(_work(x), tok, k, ignore)
