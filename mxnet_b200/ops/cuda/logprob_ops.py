@@ -10,7 +10,7 @@ def _forward(x, tokens, k, ignore, keep):
     rows, cols = x.shape
     dev = x.device
     lp = torch.empty(rows, dtype=torch.float32, device=dev)
-    ent = torch.empty(rows, dtype=torch.float32, device=dev)
+    ent = torch.empty_like(lp)
     top_lp = torch.empty((rows, k), dtype=torch.float32, device=dev) if k else None
     top_id = torch.empty((rows, k), dtype=torch.int64, device=dev) if k else None
     stat = torch.empty((rows, 3), dtype=torch.float32, device=dev) if keep else None

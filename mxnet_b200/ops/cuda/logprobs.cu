@@ -224,7 +224,7 @@ template <> __device__ __forceinline__ uint64_t lp_remote<uint64_t>(const uint64
 }
 __device__ __forceinline__ void lp_cluster_sync() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 512, kLpMaxShare = 8;
 constexpr int kLpBatch = 4;              // vectors of a thread on their way at once
 
 template <typename T>
@@ -420,12 +420,28 @@ logprob_fwd_kernel(const LogProbParams p) {
     if (p.share > 1) lp_cluster_sync();
     else __syncthreads();
     if (rank == 0 && warp == 0) {
+      // every remote word is asked for before the first is used: a trip to another CTA takes about a microsecond
       RowStat all = part_stat;
       uint64_t list = best[0][lane];
-      for (int c = 1; c < p.share; ++c) {
-        all = rs_merge(all, {lp_remote(&part_stat.m, c), lp_remote(&part_stat.r, c), lp_remote(&part_stat.w, c)});
-        if (p.k) list = warp_merge_desc(list, lp_remote(&best[0][lane], c));
+      if (p.share > 1) {
+        uint64_t other[kLpMaxShare - 1];
+        if (p.k) {
+#pragma unroll
+          for (int c = 1; c < kLpMaxShare; ++c) other[c - 1] = c < p.share ? lp_remote(&best[0][lane], c) : 0;
+        }
+        all = {-INFINITY, 0.f, 0.f};
+        if (lane < p.share) all = {lp_remote(&part_stat.m, lane), lp_remote(&part_stat.r, lane), lp_remote(&part_stat.w, lane)};
+#pragma unroll
+        for (int o = 1; o < kLpMaxShare; o <<= 1)
+          all = rs_merge(all, {__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.r, o), __shfl_xor_sync(0xffffffffu, all.w, o)});
+        if (p.k) {
+#pragma unroll
+          for (int c = 1; c < kLpMaxShare; ++c) if (c < p.share) list = warp_merge_desc(list, other[c - 1]);
+        }
       }
+      all.m = __shfl_sync(0xffffffffu, all.m, 0);
+      all.r = __shfl_sync(0xffffffffu, all.r, 0);
+      all.w = __shfl_sync(0xffffffffu, all.w, 0);
       const bool empty = all.m == -INFINITY;                      // nothing is possible: every log probability is -inf
       const float lt = log1pf(all.r);
       if (lane == 0) {
@@ -532,7 +548,7 @@ static int logprob_forward(LogProbParams p, cudaStream_t st) {
   // Rows are shared while that fills no more than two CTAs on every SM and leaves each CTA 16 KB (a part with less has too little
   // to read for the joins it causes).
   p.share = 1;
-  while (p.share < 8 && p.rows * p.share * 2 <= 2 * sm_count() && (int64_t)p.cols * sizeof(T) / (p.share * 2) >= 16384) p.share <<= 1;
+  while (p.share < kLpMaxShare && p.rows * p.share * 2 <= 2 * sm_count() && (int64_t)p.cols * sizeof(T) / (p.share * 2) >= 16384) p.share <<= 1;
   p.part = p.share == 1 ? p.cols : ((p.cols + p.share - 1) / p.share + 63) / 64 * 64;
   const int64_t cap = (int64_t)sm_count() * 64;
   const int64_t rows = p.rows < cap ? p.rows : cap;

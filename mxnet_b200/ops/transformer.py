@@ -375,6 +375,16 @@ def sldwin_attention_step(query, key=None, value=None, key_cache=None, value_cac
 # ------------------------------------------------------------------------------------------
 # scored tokens
 # ------------------------------------------------------------------------------------------
+def _log_probs_refuse(name, logits, tokens, k):
+    _need(logits.dim() >= 1 and logits.is_floating_point(), '%s: logits must be floating-point (..., V), got %s of %s', name,
+          tuple(logits.shape), logits.dtype)
+    V, lead = logits.shape[-1], tuple(logits.shape[:-1])
+    _need(tuple(tokens.shape) == lead, '%s: tokens must be %s, got %s', name, lead, tuple(tokens.shape))
+    _need(V >= 1, '%s: logits have no entries', name)
+    _need(0 <= k <= min(V, _MAX_TOP), '%s: topk must be between 0 and %d, got %d', name, min(V, _MAX_TOP), k)
+    raise MXNetError('%s: tokens are on %s, expected %s' % (name, tokens.device, logits.device))
+
+
 @register('_contrib_token_log_probs', '_npx_token_log_probs', inputs=('logits', 'tokens'),
           nout=lambda attrs: 4 if int(attrs.get('topk', 0) or 0) else 2, defaults={'topk': 0, 'ignore_label': -1})
 def token_log_probs(logits, tokens=None, topk=0, ignore_label=-1):
@@ -391,16 +401,15 @@ def token_log_probs(logits, tokens=None, topk=0, ignore_label=-1):
     Differentiable in ``logits`` through log_prob, entropy and top_log_prob.  On a GPU one kernel reads the logits once for all
     outputs and one writes the gradient; probabilities are not stored."""
     name = 'token_log_probs'
-    _need(tokens is not None, '%s: logits and tokens are required', name)
-    _need(logits.dim() >= 1 and logits.is_floating_point(), '%s: logits must be floating-point (..., V), got %s of %s', name,
-          logits.shape, logits.dtype)
+    if tokens is None or type(topk) is not int or type(ignore_label) is not int:
+        _need(tokens is not None, '%s: logits and tokens are required', name)
+        topk, ignore_label = _whole(name, 'topk', topk or 0), _whole(name, 'ignore_label', ignore_label)
+    k, ignore = topk, ignore_label
     shape = logits.shape
+    if not (len(shape) >= 1 and logits.is_floating_point() and tokens.shape == shape[:-1] and shape[-1] >= 1 and
+            0 <= k <= min(shape[-1], _MAX_TOP) and tokens.device == logits.device):
+        _log_probs_refuse(name, logits, tokens, k)
     V, lead = shape[-1], shape[:-1]
-    _need(tokens.shape == lead, '%s: tokens must be %s, got %s', name, tuple(lead), tuple(tokens.shape))
-    _need(tokens.device == logits.device, '%s: tokens are on %s, expected %s', name, tokens.device, logits.device)
-    k, ignore = _whole(name, 'topk', topk or 0), _whole(name, 'ignore_label', ignore_label)
-    _need(V >= 1, '%s: logits have no entries', name)
-    _need(0 <= k <= min(V, _MAX_TOP), '%s: topk must be between 0 and %d, got %d', name, min(V, _MAX_TOP), k)
     flat = len(shape) == 2
     tok, x = _plain(tokens), logits
     if not flat:
@@ -408,7 +417,7 @@ def token_log_probs(logits, tokens=None, topk=0, ignore_label=-1):
     if tok.dtype != torch.int64:
         tok = tok.long()
     if _kernels(logits) and V < (1 << 31) - 1024:
-        res = logprob_ops.token_log_probs(x.contiguous(), tok.contiguous(), k, ignore)
+        res = logprob_ops.token_log_probs(x if x.is_contiguous() else x.contiguous(), tok.contiguous(), k, ignore)
     else:
         res = _token_log_probs(_work(x), tok, k, ignore)
     return res if flat else tuple(r.reshape(lead if i < 2 else lead + (k,)) for i, r in enumerate(res))
