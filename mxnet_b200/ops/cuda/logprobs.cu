@@ -480,6 +480,7 @@ struct LogProbGradParams {
   int64_t ignore;
 };
 
+constexpr int kLpGradThreads = 512, kLpGradBatch = 4;          // vectors of a thread on their way at once
 template <typename T>
 __global__ void __launch_bounds__(512)
 logprob_bwd_kernel(const LogProbGradParams p) {
@@ -511,12 +512,20 @@ logprob_bwd_kernel(const LogProbGradParams p) {
         const int c = cut.loose_index(tid);
         dx[c] = Cvt<T>::from_f(grad(Cvt<T>::to_f(x[c]), c));
       }
-      for (int i = tid; i < cut.vecs; i += blockDim.x) {
-        const Vec16<T> a = ld16(x + cut.head + (int64_t)i * V);
-        Vec16<T> o;
+      for (int i0 = tid; i0 < cut.vecs; i0 += blockDim.x * kLpGradBatch) {
+        uint4 a[kLpGradBatch];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o.v[j] = Cvt<T>::from_f(grad(Cvt<T>::to_f(a.v[j]), 0));
-        st16(dx + cut.head + (int64_t)i * V, o);
+        for (int u = 0; u < kLpGradBatch; ++u)
+          if (i0 + u * (int)blockDim.x < cut.vecs) a[u] = __ldcs(reinterpret_cast<const uint4*>(x + cut.head) + i0 + u * (int)blockDim.x);
+#pragma unroll
+        for (int u = 0; u < kLpGradBatch; ++u) {
+          if (i0 + u * (int)blockDim.x >= cut.vecs) break;
+          const Vec16<T>& in = *reinterpret_cast<const Vec16<T>*>(&a[u]);
+          Vec16<T> o;
+#pragma unroll
+          for (int j = 0; j < V; ++j) o.v[j] = Cvt<T>::from_f(grad(Cvt<T>::to_f(in.v[j]), 0));
+          __stcs(reinterpret_cast<uint4*>(dx + cut.head) + i0 + u * (int)blockDim.x, *reinterpret_cast<const uint4*>(&o));
+        }
       }
     } else {
       for (int c = tid; c < p.cols; c += blockDim.x) dx[c] = Cvt<T>::from_f(grad(Cvt<T>::to_f(x[c]), c));
@@ -591,9 +600,9 @@ MXB_EXPORT int mxb_logprob_backward(int dtype, const void* x, void* dx, const in
   cudaStream_t st = (cudaStream_t)stream;
   const int64_t cap = (int64_t)sm_count() * 64;
   const unsigned grid = (unsigned)(rows < cap ? rows : cap);
-  if (dtype == kF32) logprob_bwd_kernel<float><<<grid, lp_threads(cols, 4, kLpThreads), 0, st>>>(p);
-  else if (dtype == kF16) logprob_bwd_kernel<__half><<<grid, lp_threads(cols, 2, kLpThreads), 0, st>>>(p);
-  else if (dtype == kBF16) logprob_bwd_kernel<__nv_bfloat16><<<grid, lp_threads(cols, 2, kLpThreads), 0, st>>>(p);
+  if (dtype == kF32) logprob_bwd_kernel<float><<<grid, lp_threads(cols, 4, kLpGradThreads), 0, st>>>(p);
+  else if (dtype == kF16) logprob_bwd_kernel<__half><<<grid, lp_threads(cols, 2, kLpGradThreads), 0, st>>>(p);
+  else if (dtype == kBF16) logprob_bwd_kernel<__nv_bfloat16><<<grid, lp_threads(cols, 2, kLpGradThreads), 0, st>>>(p);
   else return -1;
   return (int)cudaGetLastError();
 }

@@ -52,6 +52,15 @@ def test_rotary(dtype, interleaved, B, T, H, D, R):
     oracle.check(x.grad, back, rotary_bound(g, back, dtype), 'grad')
 
 
+def test_rotary_of_the_widest_heads():
+    x = randn(1, 9700, 1, 1024, dtype=torch.bfloat16)             # many tokens for each block, the largest table
+    pos, freq = torch.arange(9700, device=dev()), torch.rand(512, device=dev()) ** 4
+    got = op('rotary_embedding')(x, pos, freq)
+    at = torch.cat([torch.arange(40), torch.arange(4000, 4040), torch.arange(9660, 9700)])
+    want = oracle.rotary(x[:, at].cpu(), pos[at].cpu(), freq.cpu())
+    oracle.check(got[:, at], want, rotary_bound(x[:, at], want, torch.bfloat16))
+
+
 @pytest.mark.parametrize('pos_dtype', [torch.int32, torch.int64, torch.float32, torch.float64, torch.int16])
 @pytest.mark.parametrize('freq_dtype', [torch.float32, torch.float64])
 def test_rotary_takes_views_and_number_types(pos_dtype, freq_dtype):
