@@ -162,6 +162,30 @@ __device__ __forceinline__ void tc_accumulate(uint32_t tmem_d, uint32_t tmem_p, 
     umma_ts(tmem_d, tmem_p + k / kSteps * 16 * kSteps + k % kSteps * 8, v + (uint64_t)k * 128u, idesc, k > 0 ? 1u : carry);
 }
 
+// The start of a CTA: the loading warp has set up the barriers and goes on at once, the others meet behind the TMEM allocation.
+template <int kThreads>
+__device__ __forceinline__ void tc_start_loader() {
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  fence_async_smem();
+  __syncwarp();
+  asm volatile("bar.arrive 0, %0;" ::"n"(kThreads) : "memory");
+}
+template <int kThreads>
+__device__ __forceinline__ uint32_t tc_start(uint32_t* slot, bool alloc) {
+  if (alloc) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  asm volatile("bar.sync 0, %0;" ::"n"(kThreads) : "memory");
+  tc_fence_after();
+  return warp_uniform(*slot);
+}
+// `count` rows of `row` 16-byte words become zeros, `pitch` words from one to the next (a whole CTA).
+__device__ __forceinline__ void tc_zero_rows(void* dst, int count, int row, int64_t pitch) {
+  for (int e = threadIdx.x; e < count * row; e += blockDim.x) static_cast<uint4*>(dst)[e / row * pitch + e % row] = make_uint4(0, 0, 0, 0);
+}
+
 __device__ __forceinline__ void tc_finish(uint32_t tmem_base, uint32_t cols, int warp, int alloc_warp, volatile int* abort_flag, int* error_flag) {
   tc_fence_before();
   __syncthreads();
@@ -174,12 +198,6 @@ __device__ __forceinline__ void tc_finish(uint32_t tmem_base, uint32_t cols, int
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(cols) : "memory");
   }
 }
-__device__ __forceinline__ uint32_t tc_alloc(uint32_t* slot, uint32_t cols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  return 0;
-}
-
 // ------------------------------------------------------------------------------------------------ forward
 // Warps 0-3 and 4-7: the softmax of query tiles 0 and 1, one thread for each row; warp 8: MMA issue and TMEM; warp 9: TMA;
 // warps 10 and 11 complete the warpgroup that gives its registers to the others.
@@ -244,20 +262,27 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int ntiles = hi < lo ? 0 : ns + hi - lo + 1;
   auto key_tile = [&](int j) { return j < ns ? j : lo + (j - ns); };
 
-  if (threadIdx.x == 0) {
+  if (ntiles == 0) {                                              // rows behind the sequence
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&q_full[s], 1); mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1);
-      mbar_init(&s_full[s], 1); mbar_init(&p_half[s], 4); mbar_init(&p_full[s], 4);
+      const int q0 = qa + s * qstep, h = h0 + s * hstep, rows = min(kTcRows, p.T - q0);
+      if (rows <= 0 || (s == 1 && !qstep && !hstep)) continue;
+      tc_zero_rows(static_cast<T*>(p.out) + (((int64_t)b * p.T + q0) * p.Hq + h) * D, rows, D / 8, (int64_t)p.Hq * D / 8);
+      if (p.lse) for (int e = threadIdx.x; e < rows; e += kFwdThreads) p.lse[((int64_t)b * p.Hq + h) * p.T + q0 + e] = INFINITY;
     }
-    mbar_init(o_full, 1); mbar_init(patch, 1); mbar_init(drain, 1);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    return;
   }
-  if (warp == 8) tc_alloc(tmem_slot, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = warp_uniform(*tmem_slot);
+  uint32_t tmem = 0;
+  if (warp == 9) {
+    if (lane == 0) {
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(&q_full[s], 1); mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1);
+        mbar_init(&s_full[s], 1); mbar_init(&p_half[s], 4); mbar_init(&p_full[s], 4);
+      }
+      mbar_init(o_full, 1); mbar_init(patch, 1); mbar_init(drain, 1);
+      *abort_flag = 0;
+    }
+    tc_start_loader<kFwdThreads>();
+  } else tmem = tc_start<kFwdThreads>(tmem_slot, warp == 8);
 
   if (warp == 9) {
     // ---------------------------------------------------------------- loads

@@ -57,6 +57,7 @@ __device__ __forceinline__ void bwd_probs(uint32_t (&x)[32], const float* lse, f
 // TMEM columns: S of even tiles | S of odd tiles | dP (128 each) | dQ (D).  dS lies over the S it comes from: each part of the
 // columns over its own.
 constexpr int kBwdThreads = 576, kBwdMma = 16, kBwdTma = 17;
+constexpr int kDkvThreads = 608, kDkvStat = 18;           // one warp more: log-sum-exps and deltas of the query rows
 template <int D> struct DqSmem {
   static constexpr uint32_t tile = (D / 64) * kTcHalf;
   static constexpr int kst = 3, vst = 2;
@@ -90,19 +91,24 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const int ntiles = r.count();
   auto key_tile = [&](int j) { return j < r.ns ? j : r.lo + (j - r.ns); };
 
-  if (threadIdx.x == 0) {
-    mbar_init(qg_full, 1);
-    for (int s = 0; s < L::kst; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
-    for (int s = 0; s < L::vst; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
-    mbar_init(sd_full, 1); mbar_init(dp_empty, 16); mbar_init(ds_full, 16); mbar_init(done, 1); mbar_init(patch, 1); mbar_init(drain, 1);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  if (ntiles == 0) {                                              // rows behind the sequence
+    const int rows = min(kTcRows, p.T - q0);
+    tc_zero_rows(static_cast<T*>(p.dq) + (((int64_t)b * p.T + q0) * p.Hq + h) * D, rows, D / 8, (int64_t)p.Hq * D / 8);
+    for (int e = threadIdx.x; e < rows; e += kBwdThreads) p.delta[((int64_t)b * p.Hq + h) * p.T + q0 + e] = 0.f;
+    if (BwdRange<T>::scaled && threadIdx.x == 0) p.gmax[((int64_t)b * p.Hq + h) * tiles + qt] = 0.f;
+    return;
   }
-  if (warp == kBwdMma) tc_alloc(tmem_slot, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = warp_uniform(*tmem_slot);
+  uint32_t tmem = 0;
+  if (warp == kBwdTma) {
+    if (lane == 0) {
+      mbar_init(qg_full, 1);
+      for (int s = 0; s < L::kst; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
+      for (int s = 0; s < L::vst; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+      mbar_init(sd_full, 1); mbar_init(dp_empty, 16); mbar_init(ds_full, 16); mbar_init(done, 1); mbar_init(patch, 1); mbar_init(drain, 1);
+      *abort_flag = 0;
+    }
+    tc_start_loader<kBwdThreads>();
+  } else tmem = tc_start<kBwdThreads>(tmem_slot, warp == kBwdMma);
   constexpr uint32_t kDp = 256, kDq = 384;
 
   if (warp == kBwdTma) {
@@ -337,7 +343,7 @@ template <int D> struct DkvSmem {
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(kDkvThreads, 1)
 sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g, const TcParams p,
                  const DkvSplit sp, int bf16) {
@@ -373,20 +379,30 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int per_head = max(0, qhi - qlo + 1);
   const int nit = k0 < n ? per_head * heads : 0;
 
-  if (threadIdx.x == 0) {
-    mbar_init(kv_full, 1);
-    for (int s = 0; s < L::qst; ++s) { mbar_init(&q_full[s], 1); mbar_init(&q_empty[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&g_full[s], 1); mbar_init(&g_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], 16); }
-    mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_ready, 16); mbar_init(ds_ready, 16); mbar_init(done, 1); mbar_init(patch, 1);
-    mbar_init(drain, 1);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  if (nit == 0) {                                                 // keys behind the sequence, or queries that a short one does not have
+    if (kt < sp.part_tiles) {
+      float* sum = far ? dkv_far_part(sp, (int64_t)p.B * p.Hk, hs, chunk, bh, kt, D) : dkv_near_part(sp, (int64_t)p.B * p.Hk, hs, bh, kt, D);
+      tc_zero_rows(sum, 2 * kTcRows, D / 4, D / 4);
+    } else {
+      const int64_t at = (((int64_t)b * p.T + k0) * p.Hk + hk) * D;
+      const int rows = min(kTcRows, p.T - k0);
+      tc_zero_rows(static_cast<T*>(p.dk) + at, rows, D / 8, (int64_t)p.Hk * D / 8);
+      tc_zero_rows(static_cast<T*>(p.dv) + at, rows, D / 8, (int64_t)p.Hk * D / 8);
+    }
+    return;
   }
-  if (warp == kBwdMma) tc_alloc(tmem_slot, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = warp_uniform(*tmem_slot);
+  uint32_t tmem = 0;
+  if (warp == kBwdTma) {
+    if (lane == 0) {
+      mbar_init(kv_full, 1);
+      for (int s = 0; s < L::qst; ++s) { mbar_init(&q_full[s], 1); mbar_init(&q_empty[s], 1); }
+      for (int s = 0; s < 2; ++s) { mbar_init(&g_full[s], 1); mbar_init(&g_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], 16); }
+      mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_ready, 16); mbar_init(ds_ready, 16); mbar_init(done, 1); mbar_init(patch, 1);
+      mbar_init(drain, 1);
+      *abort_flag = 0;
+    }
+    tc_start_loader<kDkvThreads>();
+  } else tmem = tc_start<kDkvThreads>(tmem_slot, warp == kBwdMma);
   constexpr uint32_t kDp = 128, kDv = 256, kDk = 256 + D;
 
   if (warp == kBwdTma) {
@@ -399,15 +415,6 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       bool ok = true;
       int nq = 0, ng = 0;
       uint32_t patched = 0;
-      float f = BwdRange<T>::unshift;
-      if (BwdRange<T>::scaled) {
-        float big = 0.f;
-        for (int e = lane; e < nit; e += 32)
-          big = fmaxf(big, p.gmax[((int64_t)b * p.Hq + h_first + e / per_head) * sp.tiles + qlo + e % per_head]);
-        const float up = bwd_factor(warp_max(big));
-        f *= up;
-        if (lane == 0) s_factor[0] = up;
-      }
       for (int it = 0; it < nit && ok; ++it) {
         const int h = h_first + it / per_head, q0 = (qlo + it % per_head) * kTcRows;
         const int sq = it % L::qst, sg = it % L::gst;
@@ -416,39 +423,23 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (it >= L::qst && !(ok = mbar_wait_warp(&q_empty[sq], (uint32_t)(it / L::qst + 1) & 1u))) break;
         if (lane == 0) {
           uint64_t* bar = ends ? patch : &q_full[sq];
-          mbar_expect_tx(bar, L::tile);
+          mbar_expect_tx(bar, ends ? 2 * L::tile : L::tile);
           tc_load_tile<D>(tq, &map_q, h, q0, b, bar);
         }
         nq = ends ? it : it + 1;
-        if (ends) {
-          if (!(ok = mbar_wait_warp(patch, patched++ & 1u))) break;
-          tc_clear_rows<D>(tq, n - q0);
-          if (lane == 0) mbar_arrive(&q_full[sq]);
-        }
         if (it >= L::gst && !(ok = mbar_wait_warp(&g_empty[sg], (uint32_t)(it / L::gst + 1) & 1u))) break;
         if (lane == 0) {
           uint64_t* bar = ends ? patch : &g_full[sg];
-          mbar_expect_tx(bar, L::tile);
+          if (!ends) mbar_expect_tx(bar, L::tile);
           tc_load_tile<D>(tg, &map_g, h, q0, b, bar);
         }
         ng = ends ? it : it + 1;
         if (ends) {
           if (!(ok = mbar_wait_warp(patch, patched++ & 1u))) break;
+          tc_clear_rows<D>(tq, n - q0);
           tc_clear_rows<D>(tg, n - q0);
-          if (lane == 0) mbar_arrive(&g_full[sg]);
+          if (lane == 0) { mbar_arrive(&q_full[sq]); mbar_arrive(&g_full[sg]); }
         }
-        // log-sum-exp and delta of the tile's rows; a row that is not there gets +inf: probability 0
-        if (it >= 2 && !(ok = mbar_wait_warp(&st_empty[it & 1], (uint32_t)(it / 2 + 1) & 1u))) break;
-        const int64_t at = ((int64_t)b * p.Hq + h) * p.T + q0;
-        float* st = s_stat + (it & 1) * 256;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int c = lane + 32 * e;
-          st[c] = q0 + c < n ? BwdRange<T>::shift - p.lse[at + c] : -INFINITY;
-          st[128 + c] = q0 + c < n ? -p.delta[at + c] * f : 0.f;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&st_full[it & 1]);
       }
       if (!ok) {
         *abort_flag = 1;
@@ -459,6 +450,33 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
       }
     }
+  } else if (warp == kDkvStat) {
+    bool ok = true;
+    float f = BwdRange<T>::unshift;
+    if (BwdRange<T>::scaled) {
+      float big = 0.f;
+      for (int e = lane; e < nit; e += 32)
+        big = fmaxf(big, p.gmax[((int64_t)b * p.Hq + h_first + e / per_head) * sp.tiles + qlo + e % per_head]);
+      const float up = bwd_factor(warp_max(big));
+      f *= up;
+      if (lane == 0) s_factor[0] = up;
+    }
+    for (int it = 0; it < nit && ok; ++it) {
+      const int h = h_first + it / per_head, q0 = (qlo + it % per_head) * kTcRows;
+      // log-sum-exp and delta of the tile's rows; a row that is not there gets +inf: probability 0
+      if (it >= 2 && !(ok = mbar_wait_warp(&st_empty[it & 1], (uint32_t)(it / 2 + 1) & 1u))) break;
+      const int64_t at = ((int64_t)b * p.Hq + h) * p.T + q0;
+      float* st = s_stat + (it & 1) * 256;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = lane + 32 * e;
+        st[c] = q0 + c < n ? BwdRange<T>::shift - p.lse[at + c] : -INFINITY;
+        st[128 + c] = q0 + c < n ? -p.delta[at + c] * f : 0.f;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&st_full[it & 1]);
+    }
+    if (!ok) *abort_flag = 1;
   } else if (warp == kBwdMma) {
     if (nit > 0) {
       const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
@@ -647,11 +665,12 @@ static DkvSplit dkv_split(const SwParams& p) {
     s.sink_tiles = (p.sinks + kTcRows - 1) / kTcRows;
     s.far_chunks = (far + s.near_span) / (s.near_span + 1);
   }
-  // fewer CTAs than two for each SM: the heads of a group are walked side by side instead of one after another
+  // Fewer CTAs than SMs: the heads of a group are walked side by side instead of one after another (with a threshold of two for
+  // each SM the sums in parts cost more than the fuller device gives: 2 x 4096, 16 heads over 4, window 1024: 316 us against 288).
   const int group = p.Hq / p.Hk;
   s.hsplit = 1;
   for (int k = 1; k <= group; ++k)
-    if (group % k == 0) { s.hsplit = k; if ((int64_t)p.B * p.Hk * s.tiles * k >= 2 * sm_count()) break; }
+    if (group % k == 0) { s.hsplit = k; if ((int64_t)p.B * p.Hk * s.tiles * k >= sm_count()) break; }
   s.part_tiles = s.hsplit > 1 ? s.tiles : s.sink_tiles;
   s.items = p.B * p.Hk * s.hsplit;
   return s;
@@ -685,7 +704,7 @@ static int tc_backward(const SwParams& p, float* parts, int bf16, int* error_fla
   sw_dq_tc_kernel<T, D><<<(unsigned)gq, kBwdThreads, DqSmem<D>::total, st>>>(mq, mk, mv, mg, t, bf16);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
-  sw_dkv_tc_kernel<T, D><<<(unsigned)gk, kBwdThreads, DkvSmem<D>::total, st>>>(mq, mk, mv, mg, t, s, bf16);
+  sw_dkv_tc_kernel<T, D><<<(unsigned)gk, kDkvThreads, DkvSmem<D>::total, st>>>(mq, mk, mv, mg, t, s, bf16);
   e = cudaGetLastError();
   if (e != cudaSuccess || !s.part_tiles) return (int)e;
   sw_dkv_join_kernel<T, D><<<dim3((unsigned)(s.part_tiles * p.B * p.Hk), 2 * kTcRows * D / 8 / 256), 256, 0, st>>>(t, s);
