@@ -54,23 +54,30 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {      // a NaN stays
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
-// 2^x on the fp32 pipes, for x <= 2^6: n + f with f in [-1/2, 1/2], 2^f by the degree-4 polynomial of least relative error (3e-6,
-// far below the half step of P's type), n added to the exponent.  Arguments are cut at -126.
+// 2^x on the fp32 pipes, for x <= 2^6: n + f with f in [-1/2, 1/2], 2^f by the degree-4 polynomial of least relative error with
+// 2^0 = 1 (2.8e-6, far below the half step of P's type), n added to the exponent.  Arguments are cut at -127, where the bits of 1
+// become those of 0: what is hidden weighs nothing, however large its value.  A NaN becomes the largest number, which is
+// infinite in half types.
 constexpr float kRoundMagic = 12582912.f;                 // 1.5 * 2^23: adding it rounds to a whole number in the low bits
 __device__ __forceinline__ f32x2 exp2_poly(float a, float b) {
-  const f32x2 x = pack_f2(fmaxf(a, -126.f), fmaxf(b, -126.f)), magic = pack_f2(kRoundMagic, kRoundMagic);
+  const f32x2 x = pack_f2(max2(a, -127.f), max2(b, -127.f)), magic = pack_f2(kRoundMagic, kRoundMagic);
   const f32x2 n = add_f2(x, magic);
   const f32x2 f = add_f2(x, mul_f2(add_f2(n, pack_f2(-kRoundMagic, -kRoundMagic)), pack_f2(-1.f, -1.f)));
-  f32x2 y = fma_f2(f, pack_f2(0.009570102f, 0.009570102f), pack_f2(0.055917863f, 0.055917863f));
-  y = fma_f2(y, f, pack_f2(0.24024744f, 0.24024744f));
-  y = fma_f2(y, f, pack_f2(0.6931218f, 0.6931218f));
-  y = fma_f2(y, f, pack_f2(0.9999993f, 0.9999993f));
+  f32x2 y = fma_f2(f, pack_f2(0.009582844f, 0.009582844f), pack_f2(0.055906426f, 0.055906426f));
+  y = fma_f2(y, f, pack_f2(0.24024099f, 0.24024099f));
+  y = fma_f2(y, f, pack_f2(0.69312418f, 0.69312418f));
+  y = fma_f2(y, f, pack_f2(1.f, 1.f));
   float y0, y1, n0, n1;
   unpack_f2(y, y0, y1);
   unpack_f2(n, n0, n1);
@@ -214,10 +221,9 @@ template <int D> struct FwdSmem {
 // maximum may lag behind by 8 (2^14 in all, far from the type's largest) before the output is rescaled.
 constexpr float kPShift = 6.f, kMaxLag = 8.f;
 constexpr int kPolyPairs = 2;
-constexpr float kNoWeight = 1e-30f;       // a row that sees anything has weights from 2^6 / 2^8 up: below this it has none
 
 // 32 columns of a row: P = 2^(score sc + off), its sums, and its values in the operand type.  Of every 8 pairs kPolyPairs go
-// through the polynomial (the MUFU pipe alone takes 1024 cycles for a tile); there a hidden key gets 2^-126 in place of 0.
+// through the polynomial (the MUFU pipe alone takes 1024 cycles for a tile).
 template <typename T>
 __device__ __forceinline__ void tc_weigh(const uint32_t* x, f32x2 sc2, f32x2 off2, f32x2 (&part)[2], uint32_t (&pk)[16]) {
 #pragma unroll
@@ -430,10 +436,10 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < 128; c += 2) mx[c >> 1 & 3] = max3(mx[c >> 1 & 3], __uint_as_float(x[c]), __uint_as_float(x[c + 1]));
-      const float mt = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc);
-      const bool move = mt > m + kMaxLag || m == -INFINITY;
+      const float mt = max2(m, max3(max2(mx[0], mx[1]), mx[2], mx[3]) * sc);
+      const bool move = !(mt <= m + kMaxLag) || m == -INFINITY;
       if (__any_sync(0xffffffffu, move)) {
-        const float to_m = move ? mt : m;
+        const float to_m = move ? (mt < INFINITY ? mt : NAN) : m;            // a score of NaN or +inf makes the row NaN
         const float alpha = move ? (to_m == -INFINITY ? 0.f : ex2(m - to_m)) : 1.f;
         m = to_m;
         l *= alpha;
@@ -474,7 +480,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     tc_fence_after();
     if (ok) {
       const bool live = i < n && r.count() > 0;
-      const float inv = live ? (l > kNoWeight || l != l ? 1.f / l : 0.f) : 0.f;
+      const float inv = live && l != 0.f ? 1.f / l : 0.f;
       T* orow = static_cast<T*>(p.out) + (((int64_t)b * p.T + i) * p.Hq + h) * D;
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 32) {
@@ -494,7 +500,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           }
         }
       }
-      if (i < p.T && p.lse) p.lse[((int64_t)b * p.Hq + h) * p.T + i] = live && (l > kNoWeight || l != l) ? m + log2f(l) - kPShift : INFINITY;
+      if (i < p.T && p.lse) p.lse[((int64_t)b * p.Hq + h) * p.T + i] = live && l != 0.f ? m + log2f(l) - kPShift : INFINITY;
     }
   }
   tc_finish(tmem, 512, warp, 8, abort_flag, p.error_flag);
