@@ -104,8 +104,8 @@ def _int32(valid):
     """Lengths as the kernels read them (real ones are cut, values beyond 32 bits stay beyond every length)."""
     if valid.dtype == torch.int32 and valid.is_contiguous():
         return valid
-    if not valid.is_floating_point():
-        valid = valid.long()                                      # narrow and unsigned types do not hold the bounds below
+    # narrow and unsigned types do not hold the bounds below
+    valid = valid.double() if valid.is_floating_point() else valid.long()
     return valid.clamp(-1, (1 << 31) - 128).to(torch.int32).contiguous()
 
 

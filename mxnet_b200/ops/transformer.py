@@ -49,7 +49,7 @@ def _same(name, first, **others):
 
 
 def _whole(name, what, v):
-    _need(isinstance(v, int) and not isinstance(v, bool) or (isinstance(v, float) and v == int(v)), '%s: %s must be a whole number, got %r',
+    _need(isinstance(v, int) and not isinstance(v, bool) or (isinstance(v, float) and v.is_integer()), '%s: %s must be a whole number, got %r',
           name, what, v)
     return int(v)
 
@@ -198,6 +198,11 @@ def _lengths(name, valid_length, B, device):
     return valid_length
 
 
+def _cut(valid, T):
+    """Lengths as whole numbers from 0 to T (real ones are cut)."""
+    return (valid.double() if valid.is_floating_point() else valid.long()).clamp(0, T).long()
+
+
 def _grouped_softmax(score, seen):
     """Probabilities of ``score`` over the keys that are seen; a row that sees none gets zeros."""
     score = score.masked_fill(~seen, -math.inf)
@@ -214,8 +219,11 @@ def sldwin_attention(query, key=None, value=None, valid_length=None, window=0, s
 
     ``query``: (B, T, Hq, D); ``key``, ``value``: (B, T, Hk, D), Hq a multiple of Hk (query heads ``h * Hk // Hq`` share a key
     head); any strides over B, T and H.  Query i sees key j when ``j <= i`` and ``i - j < window`` or ``j < sinks``; ``window=0``
-    sees every ``j <= i``.  ``valid_length``: (B,) numbers of tokens (clipped to 0 .. T); the rows behind them take no part - what
-    they hold does not matter - and their outputs and gradients are 0.  ``scale`` defaults to ``1 / sqrt(D)``.
+    sees every ``j <= i``.  ``valid_length``: (B,) numbers of tokens (cut to whole ones in 0 .. T); the rows behind them take no
+    part - what they hold does not matter - and their outputs and gradients are 0.  ``scale`` defaults to ``1 / sqrt(D)``.
+
+    A query whose largest score is NaN or +inf gets NaN, one with nothing but -inf gets 0.  A value that is not finite may make
+    rows of its sequence NaN that do not see it (0 times infinity).
 
     Returns (B, T, Hq, D); differentiable in query, key and value.  The (T, T) scores are not stored on the GPU."""
     name = 'sldwin_attention'
@@ -240,7 +248,7 @@ def sldwin_attention(query, key=None, value=None, valid_length=None, window=0, s
         seen = seen & ((gap < window) | (i < sinks)[None, :])
     seen = seen.expand(B, 1, 1, T, T)
     if valid is not None:
-        there = i[None, :] < valid[:, None]
+        there = i[None, :] < _cut(valid, T)[:, None]
         seen = seen & there[:, None, None, :, None]
         gone = ~there[:, None, None, :, None]
         q, k, v = q.masked_fill(gone, 0.0), k.masked_fill(gone, 0.0), v.masked_fill(gone, 0.0)
@@ -310,7 +318,7 @@ def sldwin_cache_fill(key, value=None, key_cache=None, value_cache=None, valid_l
         return key_cache, value_cache
     C = key_cache.shape[1]
     at = torch.arange(T, device=key.device).expand(B, T)
-    n = (valid.long().clamp(0, T) if valid is not None else at.new_full((B,), T))[:, None]
+    n = (_cut(valid, T) if valid is not None else at.new_full((B,), T))[:, None]
     # the position that ends up in each row: the last one that falls on it
     row = torch.arange(C, device=key.device).expand(B, C)
     held = torch.where(row < sinks, row, n - 1 - torch.remainder(n - 1 - row, C - sinks))

@@ -140,6 +140,47 @@ def test_lengths_of_any_number_type(dtype):
     assert torch.equal(*caches)
 
 
+@pytest.mark.parametrize('dtype', HALF)
+def test_lengths_of_half_types(dtype):
+    q, k, v = (randn(3, 140, 2, 64, dtype=torch.float16) for _ in range(3))
+    lengths = torch.tensor([-math.inf, 97, math.inf], device=dev()).to(dtype)
+    want = op('sldwin_attention')(q, k, v, torch.tensor([0, 97, 140], dtype=torch.int32, device=dev()), window=33)
+    assert torch.equal(op('sldwin_attention')(q, k, v, lengths, window=33), want)
+
+
+@pytest.mark.parametrize('dtype', HALF)
+@pytest.mark.parametrize('D', [64, 128, 72])
+@pytest.mark.parametrize('j', [0, 1, 5, 130, 131, 191])
+def test_attention_with_keys_that_are_not_finite(dtype, D, j):
+    """A key of NaN makes the rows NaN that see it, one that scores -inf weighs nothing, one that scores +inf makes rows NaN; the
+    other rows keep their bits.  Hidden values weigh nothing however large they are."""
+    T, window = 300, 140
+    q, k, v = (randn(1, T, h, D, dtype=dtype) for h in (2, 1, 1))
+    q[..., 0] = q[..., 0].abs() + 0.25
+    i = torch.arange(T, device=dev())
+    sees = (i >= j) & (i - j < window)
+    base = op('sldwin_attention')(q, k, v, window=window)
+    large = v.clone()
+    large[:, j] = torch.finfo(dtype).max
+    got = op('sldwin_attention')(q, k, large, window=window)
+    assert torch.equal(got[:, ~sees], base[:, ~sees])
+    for x in (math.nan, math.inf):
+        bad = k.clone()
+        bad[:, j, :, 0] = x
+        got = op('sldwin_attention')(q, bad, v, window=window)
+        assert torch.equal(got[:, ~sees], base[:, ~sees]) and bool(torch.isnan(got[:, sees]).all()), x
+    bad = k.clone()
+    bad[:, j, :, 0] = -math.inf
+    got = op('sldwin_attention')(q, bad, v, window=window)
+    mask = (oracle.visible(T, window, 0) & (i.cpu() != j)[None, :])[None, None]
+    P = (torch.einsum('bihd,bjgd->bhij', q.double(), k.double()).cpu() / math.sqrt(D)).masked_fill(~mask, -math.inf).softmax(-1).nan_to_num(nan=0.0)
+    V = v.double().cpu()[:, :, 0]
+    want = torch.einsum('bhij,bjd->bihd', P, V)
+    half = oracle.half(dtype)
+    bound = (half + oracle.FP32) * torch.einsum('bhij,bjd->bihd', P, V.abs()) + half * want.abs() + oracle.least(dtype)
+    oracle.check(got, want, bound, 'out')
+
+
 def test_a_reported_time_out_is_raised_by_the_next_call():
     from mxnet_b200.ops.cuda import sldwin_ops
     q = randn(1, 20, 1, 64, dtype=torch.float16)

@@ -300,6 +300,27 @@ def test_log_probs_refuse(x, tok, attrs):
         nd.contrib.token_log_probs(arr(x), *([arr(tok)] if tok is not None else []), **attrs)
 
 
+@pytest.mark.parametrize('bad', [math.inf, -math.inf, math.nan])
+def test_sizes_that_are_no_numbers_are_refused(bad):
+    a = {k: nd.NDArray(v) for k, v in _attention_args().items()}
+    for size in ('window', 'sinks'):
+        with pytest.raises(MXNetError):
+            nd.contrib.sldwin_attention(**a, **{size: bad})
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32, torch.float64])
+def test_real_lengths_are_cut(dtype):
+    q, k, v = (randn(4, 9, 2, 4) for _ in range(3))
+    lengths = torch.tensor([-math.inf, 2.5, 7.0, math.inf]).to(dtype)
+    whole = torch.tensor([0, 2, 7, 9])
+    got, want = (nd.contrib.sldwin_attention(arr(q), arr(k), arr(v), arr(n), window=3)._data for n in (lengths, whole))
+    assert torch.equal(got, want)
+    caches = [torch.zeros(2, 4, 5, 2, 4, dtype=torch.float64) for _ in range(2)]
+    for c, n in zip(caches, (lengths, whole)):
+        nd.contrib.sldwin_cache_fill(arr(k), arr(v), arr(c[0]), arr(c[1]), arr(n), sinks=1)
+    assert torch.equal(*caches)
+
+
 # ------------------------------------------------------------------------------------------------- front ends, empty
 def test_empty_arrays():
     z = lambda *s: arr(torch.zeros(*s))   # noqa: E731
