@@ -316,12 +316,12 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 // ------------------------------------------------------------------------------------------------ dK, dV
 // A CTA owns 128 keys of one key head and walks (query head, query tile): the heads of its part of the group, the tiles whose
 // windows reach its keys.  A key tile that holds sinks is seen by all later queries as well: those far tiles go to CTAs of
-// their own in chunks as long as a window, and where keys are few the heads of a group are split over CTAs; such parts are
+// their own in chunks, and where keys are few the heads of a group are split over CTAs; such parts are
 // written in fp32 and added in a fixed order by a last small kernel.
 // TMEM columns: S^T | dP^T (128 each) | dV | dK (D each); P^T over S^T, dS^T over dP^T, each part of the columns over its own.
 struct DkvSplit {
   int tiles, near_span;                  // query tiles kt .. kt + near_span reach a key tile by their windows
-  int sink_tiles, far_chunks;            // far CTAs: sink_tiles x far_chunks of near_span + 1 query tiles
+  int sink_tiles, far_chunks, far_len;   // far CTAs: sink_tiles x far_chunks, of far_len query tiles
   int hsplit;                            // parts of a head group
   int part_tiles;                        // key tiles whose sums come in parts: the first part_tiles
   int items;                             // B * Hk * hsplit
@@ -374,8 +374,8 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int n = warp_uniform(tc_valid(p, b));
   const int k0 = kt * kTcRows;
   const int last_tile = n > 0 ? (n - 1) / kTcRows : -1;
-  const int qlo = far ? kt + sp.near_span + 1 + chunk * (sp.near_span + 1) : kt;
-  const int qhi = min(last_tile, qlo + sp.near_span);
+  const int qlo = far ? kt + sp.near_span + 1 + chunk * sp.far_len : kt;
+  const int qhi = min(last_tile, far ? qlo + sp.far_len - 1 : qlo + sp.near_span);
   const int per_head = max(0, qhi - qlo + 1);
   const int nit = k0 < n ? per_head * heads : 0;
 
@@ -661,18 +661,23 @@ static DkvSplit dkv_split(const SwParams& p) {
   s.near_span = (int)(((int64_t)kTcRows - 2 + p.window) / kTcRows);
   if (s.near_span > s.tiles - 1) s.near_span = s.tiles - 1;
   const int far = s.tiles - 1 - s.near_span;             // query tiles behind the windows of the first key tile
-  if (far > 0 && p.sinks > 0) {
-    s.sink_tiles = (p.sinks + kTcRows - 1) / kTcRows;
-    s.far_chunks = (far + s.near_span) / (s.near_span + 1);
-  }
   // Fewer CTAs than SMs: the heads of a group are walked side by side instead of one after another (with a threshold of two for
   // each SM the sums in parts cost more than the fuller device gives: 2 x 4096, 16 heads over 4, window 1024: 316 us against 288).
   const int group = p.Hq / p.Hk;
   s.hsplit = 1;
   for (int k = 1; k <= group; ++k)
     if (group % k == 0) { s.hsplit = k; if ((int64_t)p.B * p.Hk * s.tiles * k >= sm_count()) break; }
-  s.part_tiles = s.hsplit > 1 ? s.tiles : s.sink_tiles;
   s.items = p.B * p.Hk * s.hsplit;
+  if (far > 0 && p.sinks > 0) {
+    // Chunks as long as a window, twice as long while there are more of them than SMs: each writes 2 x 128 x D sums that are read
+    // again.  1 x 32768, 16 heads over 4 of 128, window 128: backward 672 us with chunks of a window, 595 so; 8 x 4096, 12 over 4 of
+    // 64: 380 and 343; up to two CTAs for each SM: 620 and 360.
+    s.sink_tiles = (p.sinks + kTcRows - 1) / kTcRows;
+    s.far_len = s.near_span + 1;
+    while (s.far_len < far && (int64_t)s.items * s.sink_tiles * ((far + s.far_len - 1) / s.far_len) > sm_count()) s.far_len *= 2;
+    s.far_chunks = (far + s.far_len - 1) / s.far_len;
+  }
+  s.part_tiles = s.hsplit > 1 ? s.tiles : s.sink_tiles;
   return s;
 }
 

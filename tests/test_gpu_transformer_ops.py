@@ -124,6 +124,15 @@ def test_attention_ragged_and_what_lies_behind(dtype, D, window, sinks):
             assert not bool(b.masked_select(behind.expand_as(b)).any())
 
 
+@pytest.mark.parametrize('dtype', HALF)
+@pytest.mark.parametrize('B,T,Hq,Hk,D,sinks', [(60, 900, 1, 1, 64, 130), (20, 1300, 4, 4, 128, 4), (160, 600, 2, 1, 64, 1)])
+def test_attention_with_sinks_seen_by_many_later_tiles(dtype, B, T, Hq, Hk, D, sinks):
+    valid = torch.randint(0, T + 1, (B,), device=dev(), dtype=torch.int32)
+    valid[:2] = T
+    q, k, v, g = (randn(B, T, h, D, dtype=dtype) for h in (Hq, Hk, Hk, Hq))
+    check_attention(q, k, v, valid, 64, sinks, g)
+
+
 @pytest.mark.parametrize('dtype', [torch.uint8, torch.int16, torch.int64, torch.float32, torch.float64])
 def test_lengths_of_any_number_type(dtype):
     q, k, v = (randn(3, 140, 2, 64, dtype=torch.float16) for _ in range(3))
