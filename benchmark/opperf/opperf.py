@@ -212,6 +212,56 @@ def case_rnn(ctx, dtype, small, mode='lstm', bidirectional=False):
     return dict(inputs=[x, params], fn=fn, fwd_flops=fl, bwd_flops=2 * fl)
 
 
+def case_rotary(ctx, dtype, small):
+    b, t = (1, 2048) if small else (8, 2048)
+    x = _rand((b, t, 20, 128), ctx, dtype)
+    pos, freq = nd.arange(t, ctx=ctx), nd.contrib.rotary_inv_freq(dim=128, ctx=ctx)
+    nb = x.size * _esize(dtype)
+    return dict(inputs=[x], fn=lambda x: nd.contrib.rotary_embedding(x, pos, freq), fwd_bytes=2 * nb, bwd_bytes=2 * nb)
+
+
+def case_sldwin_attention(ctx, dtype, small, b=2, t=4096, heads=16, kv_heads=4, dim=128, window=1024, sinks=4):
+    b, t = (1, 2048) if small else (b, t)
+    q, k, v = (_rand((b, t, h, dim), ctx, dtype) for h in (heads, kv_heads, kv_heads))
+    near = min(window or t, t)
+    pairs = near * (near + 1) // 2 + (t - near) * near + sum(min(sinks, max(0, i + 1 - near)) for i in range(t))
+    fl = 4.0 * b * heads * dim * pairs
+
+    def fn(q, k, v):
+        return nd.contrib.sldwin_attention(q, k, v, window=window, sinks=sinks)
+    return dict(inputs=[q, k, v], fn=fn, fwd_flops=fl, bwd_flops=2 * fl)
+
+
+def _cache_pair(ctx, dtype, shape):
+    return _rand(shape, ctx, dtype), _rand(shape, ctx, dtype)
+
+
+def case_sldwin_cache_fill(ctx, dtype, small):
+    b, t, c = (4, 6000, 4096) if small else (16, 6000, 4096)
+    k, v = _cache_pair(ctx, dtype, (b, t, 8, 128))
+    kc, vc = _cache_pair(ctx, dtype, (b, c, 8, 128))
+    return dict(inputs=[k, v], fn=lambda k, v: nd.contrib.sldwin_cache_fill(k, v, kc, vc, sinks=4), no_backward=True,
+                fwd_bytes=4 * kc.size * _esize(dtype))
+
+
+def case_sldwin_step(ctx, dtype, small):
+    b, c = (16, 4100) if small else (64, 4100)
+    q = _rand((b, 32, 128), ctx, dtype)
+    k, v = _cache_pair(ctx, dtype, (b, 8, 128))
+    kc, vc = _cache_pair(ctx, dtype, (b, c, 8, 128))
+    pos = nd.arange(5000, 5000 + b, ctx=ctx)
+    return dict(inputs=[q, k, v], fn=lambda q, k, v: nd.contrib.sldwin_attention_step(q, k, v, kc, vc, pos, window=4096, sinks=4),
+                no_backward=True, fwd_bytes=2 * kc.size * _esize(dtype))
+
+
+def case_token_log_probs(ctx, dtype, small):
+    rows, v = (1024, 33278) if small else (4096, 33278)
+    x = _rand((rows, v), ctx, dtype)
+    tok = nd.NDArray._from_tensor(torch.randint(0, v, (rows,), device=ctx.torch_device), ctx)
+    nb = x.size * _esize(dtype)
+    return dict(inputs=[x], fn=lambda x: nd.contrib.token_log_probs(x, tok)[0], fwd_bytes=nb, bwd_bytes=2 * nb)
+
+
 CASES = {
     'csr_dot_dense': case_csr_dot,
     'csr_dot_dense_library': lambda c, d, s: case_csr_dot(c, d, s, library=True),
@@ -236,6 +286,13 @@ CASES = {
     'fused_self_attention': case_attention,
     'fused_self_attention_t256': lambda c, d, s: case_attention(c, d, s, t=256),
     'fused_self_attention_t512': lambda c, d, s: case_attention(c, d, s, t=512, heads=16),
+    'rotary_embedding': case_rotary,
+    'sldwin_attention': case_sldwin_attention,
+    'sldwin_attention_causal': lambda c, d, s: case_sldwin_attention(c, d, s, b=16, t=512, heads=12, kv_heads=12, dim=64, window=0, sinks=0),
+    'sldwin_attention_prompt': lambda c, d, s: case_sldwin_attention(c, d, s, b=1, t=8192, heads=32, kv_heads=8, window=2048),
+    'sldwin_cache_fill': case_sldwin_cache_fill,
+    'sldwin_attention_step': case_sldwin_step,
+    'token_log_probs': case_token_log_probs,
     'elemwise_add': case_add,
     'GELU': case_gelu,
     'dropout_add': case_dropout_add,

@@ -14,6 +14,9 @@
 // of threads whose maximum reaches it (k of them, more with ties) are read a second time; a warp keeps its 32 best as one
 // sorted entry for each lane.  Equal logits rank by the lower index.
 // Few rows: a cluster of CTAs shares a row and joins over distributed shared memory.
+//
+// 4096 x 33278 bf16: forward 62 to 68 us for 273 MB (4.0 to 4.4 TB/s; bound by instructions: 70 % of the issue slots), backward 93 us for 545 MB (5.9 TB/s of the 6.4 a copy reaches).  24 x 131072 fp32 with
+// 20 alternatives: 16 us for 12.6 MB, a chain of joins.
 #include "common.cuh"
 
 namespace mxb {

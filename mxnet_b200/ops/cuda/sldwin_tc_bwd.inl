@@ -2,9 +2,15 @@
 //
 // Two kernels, each the owner of what it accumulates, so that no result depends on the order of anything: dQ by query tiles
 // (S, dP and dS K: three products per pair of tiles) and dK, dV by key tiles (S^T, dP^T, P^T dO, dS^T Q: four).  The scores
-// are formed twice; sharing them would need sums of dQ across CTAs in memory.  In both, two warpgroups share each tile of
-// scores (64 columns each), so that their exponentials take less time than the products and the tensor cores set the pace.
-
+// are formed twice; sharing them would need sums of dQ across CTAs in memory.  In both, four warpgroups share each tile of
+// scores (32 columns each: a thread holds its scores and their gradients in registers), so that the exponentials of a tile take
+// less time than its products.
+//
+// What bounds it: a step of the dK, dV walk takes 2700 cycles, of which the four products need 2048 at the tensor cores' full rate
+// (512 for 128 x 128 x 128) and the chain scores, probabilities, next scores the rest; then the start and the end of each CTA, with
+// one CTA on an SM (shared memory and TMEM are full).
+// 2 x 4096, 16 heads over 4 of 128, window 1024, 4 sinks, bf16: dQ 134 us (tensor pipe active 42 %), dK and dV 147 us (61 %).
+// 16 x 512 padded, 12 heads of 64, fp16: 35 and 41 us, a chain of one to four tiles in each CTA (tensor pipe 10 %).
 //
 // Range in fp16: probabilities enter the dV product 2^14 times their value (at most 2^14, digits kept down to 2^-28), and dS is
 // formed from dO scaled by the power of two that brings the largest dO of the CTA's tiles into [8, 16): neither small
@@ -661,12 +667,16 @@ static DkvSplit dkv_split(const SwParams& p) {
   s.near_span = (int)(((int64_t)kTcRows - 2 + p.window) / kTcRows);
   if (s.near_span > s.tiles - 1) s.near_span = s.tiles - 1;
   const int far = s.tiles - 1 - s.near_span;             // query tiles behind the windows of the first key tile
-  // Fewer CTAs than SMs: the heads of a group are walked side by side instead of one after another (with a threshold of two for
-  // each SM the sums in parts cost more than the fuller device gives: 2 x 4096, 16 heads over 4, window 1024: 316 us against 288).
+  // Fewer CTAs than SMs: the heads of a group are walked side by side instead of one after another.  The sums in parts cost more
+  // than a device that is filled better gives once half the SMs have a CTA (16 heads over 4 of 128, window 1024, whole backward
+  // pass: 1 x 4096 tokens, 128 CTAs, 164 us, two parts 175 us; 1 x 2048, 64 CTAs, two parts 94 us, four 106 us, one 116 us),
+  // unless windows cut hardly any walk short: there the first keys' walks are long and the others fill in (1 x 4096, 8 heads
+  // over 1 of 128, no window, 32 CTAs: one part 435 us, two 261, four 173, eight 137).
   const int group = p.Hq / p.Hk;
+  const int64_t enough = 4 * (int64_t)s.near_span >= 3 * (int64_t)s.tiles ? sm_count() : sm_count() / 2;
   s.hsplit = 1;
   for (int k = 1; k <= group; ++k)
-    if (group % k == 0) { s.hsplit = k; if ((int64_t)p.B * p.Hk * s.tiles * k >= sm_count()) break; }
+    if (group % k == 0) { s.hsplit = k; if ((int64_t)p.B * p.Hk * s.tiles * k >= enough) break; }
   s.items = p.B * p.Hk * s.hsplit;
   if (far > 0 && p.sinks > 0) {
     // Chunks as long as a window, twice as long while there are more of them than SMs: each writes 2 x 128 x D sums that are read
