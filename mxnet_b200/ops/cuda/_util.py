@@ -1,5 +1,8 @@
 """Helpers shared by the kernel wrappers."""
+import functools
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import lib, ptr, stream_ptr, count_launch, check
 
@@ -63,6 +66,17 @@ def raw_stream(t):
 def address(t):
     """Address of a tensor's data for a launcher (0 = no tensor)."""
     return 0 if t is None else t.data_ptr()
+
+
+def once(backward):
+    """``backward`` of a Function whose gradient has no gradient: one that is asked for raises.  Without ``create_graph`` nothing
+    can ask, and the guard (9 us of host time) stays out."""
+    guarded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 class _Here(object):

@@ -1,9 +1,8 @@
 """Log probabilities of tokens, entropy and top alternatives on the sm_100a kernels (``logprobs.cu``)."""
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import lib, count_launch, check
-from ._util import DT, address, on_device, raw_stream
+from ._util import DT, address, on_device, once, raw_stream
 
 
 def _forward(x, tokens, k, ignore, keep):
@@ -34,7 +33,7 @@ class _TokenLogProbs(torch.autograd.Function):
         return lp, ent, top_lp, top_id
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, g_lp, g_ent, g_top=None, _=None):
         x, tokens, stat, top_id = ctx.saved_tensors
         k, ignore = ctx.args

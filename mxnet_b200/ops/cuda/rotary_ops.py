@@ -1,9 +1,8 @@
 """Rotary position embedding on the sm_100a kernel (``rotary.cu``)."""
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import lib, count_launch, check
-from ._util import DT, on_device, raw_stream
+from ._util import DT, on_device, once, raw_stream
 
 _POS = {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int64: 3}
 
@@ -32,7 +31,7 @@ class _Rotary(torch.autograd.Function):
         return _run(x, positions, inv_freq, interleaved, scale, 0)
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dy):
         positions, inv_freq = ctx.saved_tensors
         if dy.stride(3) != 1:

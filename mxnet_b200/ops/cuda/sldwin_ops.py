@@ -3,10 +3,9 @@ key/value cache with the attention of single tokens over it (``sldwin_cache.cu``
 import ctypes as C
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import lib, count_launch, check
-from ._util import DT, address, on_device, raw_stream
+from ._util import DT, address, on_device, once, raw_stream
 
 _I13, _I16, _I18, _I19 = C.c_int64 * 13, C.c_int64 * 16, C.c_int64 * 18, C.c_int64 * 19      # sizes, then strides
 
@@ -64,7 +63,7 @@ class _SldwinAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dout):
         q, k, v, valid, out, lse = ctx.saved_tensors
         window, sinks, scale = ctx.args

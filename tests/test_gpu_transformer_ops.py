@@ -190,6 +190,20 @@ def test_attention_with_keys_that_are_not_finite(dtype, D, j):
     oracle.check(got, want, bound, 'out')
 
 
+def test_second_derivatives_are_refused():
+    x = randn(2, 5, 3, 64, dtype=torch.float16)
+    pos, freq = torch.arange(5, device=dev()), torch.rand(4, device=dev())
+    tok = torch.zeros(10, dtype=torch.int64, device=dev())
+    for f in (lambda a: op('rotary_embedding')(a, pos, freq), lambda a: op('sldwin_attention')(a, a, a),
+              lambda a: op('token_log_probs')(a.reshape(10, -1), tok)[0]):
+        a = x.clone().requires_grad_(True)
+        first, = torch.autograd.grad(f(a).float().square().sum(), a)
+        again, = torch.autograd.grad(f(a).float().square().sum(), a, create_graph=True)
+        assert torch.equal(first, again)
+        with pytest.raises(RuntimeError, match='once_differentiable'):
+            again.float().sum().backward()
+
+
 def test_a_reported_time_out_is_raised_by_the_next_call():
     from mxnet_b200.ops.cuda import sldwin_ops
     q = randn(1, 20, 1, 64, dtype=torch.float16)

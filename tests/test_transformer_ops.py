@@ -347,3 +347,30 @@ def test_symbols_infer_shapes_and_run():
     s = mx.sym.contrib.token_log_probs(x, t, topk=2)
     assert len(s.list_outputs()) == 4
     assert s.infer_shape(x=(3, 7), t=(3,))[1] == [(3,), (3,), (3, 2), (3, 2)]
+
+
+def test_gradient_passes_of_odd_heads():
+    """Head gradients of another shape and arrays outside of the graph are refused, no heads at all are no pass; several heads
+    and second derivatives are what they were."""
+    x = nd.array([[1.0, 2.0], [3.0, 4.0]])
+    x.attach_grad()
+    with autograd.record():
+        y = x * x
+    autograd.backward([])
+    with pytest.raises(Exception):
+        autograd.backward([y], [nd.ones((3, 2))])
+    with autograd.record():
+        y = x * x
+    autograd.backward([y], [nd.ones((2, 2))])
+    assert x.grad.asnumpy().tolist() == [[2, 4], [6, 8]]
+    with autograd.record():
+        y, z = x * x, 3 * x
+    g = autograd.grad([y, z], [x], [nd.ones((2, 2)) * 2, nd.ones((2, 2))])[0]
+    assert g.asnumpy().tolist() == [[7, 11], [15, 19]]
+    with autograd.record():
+        y = x * x * x
+        first = autograd.grad(y, x, create_graph=True, retain_graph=True)
+        second = autograd.grad(first, x)
+    assert second.asnumpy().tolist() == [[6, 12], [18, 24]]
+    with pytest.raises(Exception):                       # an array outside of the graph
+        autograd.grad([nd.ones((2, 2))], [x])
