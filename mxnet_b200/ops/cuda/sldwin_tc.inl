@@ -177,10 +177,10 @@ __device__ __forceinline__ void tc_start_loader() {
   __syncwarp();
   asm volatile("bar.arrive 0, %0;" ::"n"(kThreads) : "memory");
 }
-template <int kThreads>
+template <int kThreads, int kCols = 512>
 __device__ __forceinline__ uint32_t tc_start(uint32_t* slot, bool alloc) {
   if (alloc) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
@@ -216,11 +216,16 @@ __device__ __forceinline__ void tc_finish(uint32_t tmem_base, uint32_t cols, int
 // for a tile that only holds sinks gains 3 % at windows of 128 and costs 3 % everywhere else: the branch breaks up the
 // exponentials.
 // TMEM columns: S0 | S1 (128 each; P over the first 64 of its S), O0 | O1 (D each).
-constexpr int kFwdThreads = 384;         // launched with 168 registers each: 2 x 128 x 224 + 128 x 56 of the 64512
+// With one tile (kTiles 1, heads of 64) a CTA takes half an SM and the turns are taken by two CTAs.
 constexpr int kFwdStages = 2;
-template <int D> struct FwdSmem {
+template <int D, int kTiles> struct FwdForm {
+  static constexpr int threads = 128 * kTiles + 128, per_sm = kTiles == 1 ? 2 : 1;
+  // registers: launched with 168 each, 2 x 128 x 224 + 128 x 56 of the 64512; with one tile 128 each, 128 x 200 + 128 x 56 of 32768
+  static constexpr int row_regs = kTiles == 1 ? 200 : 224, other_regs = 56;
+  static constexpr uint32_t tmem_o = 128 * kTiles, tmem_cols = kTiles == 1 ? 256 : 512;
+  static constexpr int mma = 4 * kTiles, tma = mma + 1;            // warps
   static constexpr uint32_t tile = (D / 64) * kTcHalf;
-  static constexpr uint32_t q = 0, k = 2 * tile, v = k + kFwdStages * tile, bars = v + kFwdStages * tile;
+  static constexpr uint32_t q = 0, k = kTiles * tile, v = k + kFwdStages * tile, bars = v + kFwdStages * tile;
   static constexpr uint32_t total = bars + 256 + 1024;
 };
 // P is kept 2^6 times its value, so that in fp16 a weight keeps its digits down to 2^-20 of the row's largest; the running
@@ -245,11 +250,11 @@ __device__ __forceinline__ void tc_weigh(const uint32_t* x, f32x2 sc2, f32x2 off
   }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+template <typename T, int D, int kTiles>
+__global__ void __launch_bounds__(128 * kTiles + 128, kTiles == 1 ? 2 : 1)
 sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const TcParams p, int bf16) {
-  typedef FwdSmem<D> L;
+  typedef FwdForm<D, kTiles> L;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
@@ -261,13 +266,14 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 
   // the last tiles of causal attention are the longest: they start first
   const int tiles = p.T / kTcRows + (p.T % kTcRows ? 1 : 0);
-  const int qblocks = p.qpair ? tiles : (tiles + 1) / 2;
+  const bool pair = kTiles == 2 && p.qpair;
+  const int qblocks = pair || kTiles == 1 ? tiles : (tiles + 1) / 2;
   const int qb = qblocks - 1 - (int)(blockIdx.x / p.items), item = blockIdx.x % p.items;
-  const int hcount = p.qpair ? p.Hq / 2 : p.Hq;
-  const int b = item / hcount, h0 = (item % hcount) * (p.qpair ? 2 : 1), hk = h0 / (p.Hq / p.Hk);
+  const int hcount = pair ? p.Hq / 2 : p.Hq;
+  const int b = item / hcount, h0 = (item % hcount) * (pair ? 2 : 1), hk = h0 / (p.Hq / p.Hk);
   const int n = warp_uniform(tc_valid(p, b));
-  const int qa = p.qpair ? qb * kTcRows : qb * 2 * kTcRows;
-  const int qstep = p.qpair ? 0 : kTcRows, hstep = p.qpair ? 1 : 0;
+  const int qa = pair || kTiles == 1 ? qb * kTcRows : qb * 2 * kTcRows;
+  const int qstep = pair || kTiles == 1 ? 0 : kTcRows, hstep = pair ? 1 : 0;
   const KeyRange r0(qa, n, p.window, p.sinks), r1(qa + qstep, n, p.window, p.sinks);
   // the union of both: sinks, then [lo of the first, hi of the second]
   const int hi = max(r0.hi, r1.hi), lo = r0.lo, ns = max(r0.ns, min(r1.ns, lo));
@@ -275,16 +281,16 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   auto key_tile = [&](int j) { return j < ns ? j : lo + (j - ns); };
 
   if (ntiles == 0) {                                              // rows behind the sequence
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < kTiles; ++s) {
       const int q0 = qa + s * qstep, h = h0 + s * hstep, rows = min(kTcRows, p.T - q0);
       if (rows <= 0 || (s == 1 && !qstep && !hstep)) continue;
       tc_zero_rows(static_cast<T*>(p.out) + (((int64_t)b * p.T + q0) * p.Hq + h) * D, rows, D / 8, (int64_t)p.Hq * D / 8);
-      if (p.lse) for (int e = threadIdx.x; e < rows; e += kFwdThreads) p.lse[((int64_t)b * p.Hq + h) * p.T + q0 + e] = INFINITY;
+      if (p.lse) for (int e = threadIdx.x; e < rows; e += L::threads) p.lse[((int64_t)b * p.Hq + h) * p.T + q0 + e] = INFINITY;
     }
     return;
   }
   uint32_t tmem = 0;
-  if (warp == 9) {
+  if (warp == L::tma) {
     if (lane == 0) {
       for (int s = 0; s < 2; ++s) {
         mbar_init(&q_full[s], 1); mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1);
@@ -293,15 +299,15 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       mbar_init(o_full, 1); mbar_init(patch, 1); mbar_init(drain, 1);
       *abort_flag = 0;
     }
-    tc_start_loader<kFwdThreads>();
-  } else tmem = tc_start<kFwdThreads>(tmem_slot, warp == 8);
+    tc_start_loader<L::threads>();
+  } else tmem = tc_start<L::threads, L::tmem_cols>(tmem_slot, warp == L::mma);
 
-  if (warp == 9) {
+  if (warp == L::tma) {
     // ---------------------------------------------------------------- loads
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::other_regs));
     if (ntiles > 0) {
       if (lane == 0) {
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < kTiles; ++s) {
           if ((s ? r1 : r0).count() == 0) continue;
           mbar_expect_tx(&q_full[s], L::tile);
           tc_load_tile<D>(smem + L::q + s * L::tile, &map_q, h0 + s * hstep, qa + s * qstep, b, &q_full[s]);
@@ -338,16 +344,16 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (lane == 0) {
           // no copy may still be under way when the CTA's shared memory is given back
           for (int s = 0; s < 2; ++s) {
-            if ((s ? r1 : r0).count()) mbar_wait(&q_full[s], 0);
+            if (s < kTiles && (s ? r1 : r0).count()) mbar_wait(&q_full[s], 0);
             if (nk > s) mbar_wait(&k_full[s], (uint32_t)((nk - 1 - s) / kFwdStages) & 1u);
             if (nv > s) mbar_wait(&v_full[s], (uint32_t)((nv - 1 - s) / kFwdStages) & 1u);
           }
         }
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == L::mma) {
     // ---------------------------------------------------------------- products
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::other_regs));
     if (ntiles > 0) {
       const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
       const uint64_t dq = make_desc(smem_u32(smem + L::q)), dk = make_desc(smem_u32(smem + L::k)),
@@ -355,7 +361,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       constexpr uint64_t step = L::tile >> 4;
       bool ok = true;
       uint32_t pphase = 0, started = 0;                           // bit s: of query tile s
-      for (int s = 0; s < 2 && ok; ++s) {
+      for (int s = 0; s < kTiles && ok; ++s) {
         const KeyRange& r = s ? r1 : r0;
         if (r.count() == 0) continue;
         ok = mbar_wait_warp(&q_full[s], 0);
@@ -372,16 +378,16 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const uint32_t ph = (uint32_t)(j / kFwdStages) & 1u, pn = (uint32_t)((j + 1) / kFwdStages) & 1u;
         ok = mbar_wait_warp(&v_full[st], ph);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < kTiles; ++s) {
           const KeyRange& r = s ? r1 : r0;
           if (ok && r.has(kt)) {
             ok = mbar_wait_warp(&p_half[s], pphase >> s & 1u);
             tc_fence_after();
-            if (ok && elect_one()) tc_accumulate<8, 0, 4>(tmem + 256 + D * s, tmem + 128 * s, dv + st * step, id_o, started >> s & 1u);
+            if (ok && elect_one()) tc_accumulate<8, 0, 4>(tmem + L::tmem_o + D * s, tmem + 128 * s, dv + st * step, id_o, started >> s & 1u);
             ok = ok && mbar_wait_warp(&p_full[s], pphase >> s & 1u);
             pphase ^= 1u << s;
             tc_fence_after();
-            if (ok && elect_one()) tc_accumulate<8, 4, 8>(tmem + 256 + D * s, tmem + 128 * s, dv + st * step, id_o, 1u);
+            if (ok && elect_one()) tc_accumulate<8, 4, 8>(tmem + L::tmem_o + D * s, tmem + 128 * s, dv + st * step, id_o, 1u);
             started |= 1u << s;
           }
           if (ok && next >= 0 && r.has(next)) {
@@ -401,17 +407,17 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (elect_one()) umma_commit(ok ? o_full : drain);
       if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
     }
-  } else if (warp >= 10) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  } else if (warp > L::tma) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::other_regs));
   } else {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::row_regs));
     const int s = warp >> 2, quad = warp & 3;
     const int row = quad * 32 + lane;
     const int q0 = qa + s * qstep, i = q0 + row, h = h0 + s * hstep;
     const KeyRange r = s ? r1 : r0;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-    const uint32_t ts = tmem + 128 * s + lane_off, to = tmem + 256 + D * s + lane_off;
+    const uint32_t ts = tmem + 128 * s + lane_off, to = tmem + L::tmem_o + D * s + lane_off;
     const float sc = p.scale * kSwLog2e;
     float m = -INFINITY, l = 0.f;
     uint32_t phase = 0;
@@ -509,7 +515,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (i < p.T && p.lse) p.lse[((int64_t)b * p.Hq + h) * p.T + i] = live && l != 0.f ? m + log2f(l) - kPShift : INFINITY;
     }
   }
-  tc_finish(tmem, 512, warp, 8, abort_flag, p.error_flag);
+  tc_finish(tmem, L::tmem_cols, warp, L::mma, abort_flag, p.error_flag);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -549,6 +555,20 @@ static TcParams tc_params(const SwParams& p, int* error_flag) {
   return t;
 }
 
+template <typename T, int D, int kTiles>
+static int tc_forward_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, TcParams& t, int bf16, cudaStream_t st) {
+  typedef FwdForm<D, kTiles> L;
+  t.qpair = kTiles == 2 && (t.Hq / t.Hk) % 2 == 0;      // two heads over the same keys and the same rows, where heads come in pairs
+  t.items = t.B * (t.qpair ? t.Hq / 2 : t.Hq);
+  const int64_t tiles = (t.T + kTcRows - 1) / kTcRows;
+  const int64_t grid = (t.qpair || kTiles == 1 ? tiles : (tiles + 1) / 2) * t.items;
+  if (grid > 0x7fffffff) return -2;
+  static unsigned long long seen = 0;
+  if (first_on_device(&seen)) cudaFuncSetAttribute(sw_fwd_tc_kernel<T, D, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::total);
+  sw_fwd_tc_kernel<T, D, kTiles><<<(unsigned)grid, L::threads, L::total, st>>>(mq, mk, mv, t, bf16);
+  return (int)cudaGetLastError();
+}
+
 template <typename T, int D>
 static int tc_forward(const SwParams& p, int bf16, int* error_flag, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
@@ -557,13 +577,9 @@ static int tc_forward(const SwParams& p, int bf16, int* error_flag, cudaStream_t
   if (!rc) rc = tc_map(&mv, p.v, bf16, p.B, p.T, p.Hk, D, p.sv);
   if (rc) return rc;
   TcParams t = tc_params(p, error_flag);
-  t.qpair = (p.Hq / p.Hk) % 2 == 0;      // two heads over the same keys and the same rows, where heads come in pairs
-  t.items = p.B * (t.qpair ? p.Hq / 2 : p.Hq);
-  const int64_t tiles = (p.T + kTcRows - 1) / kTcRows;
-  const int64_t grid = (t.qpair ? tiles : (tiles + 1) / 2) * t.items;
-  if (grid > 0x7fffffff) return -2;
-  static unsigned long long seen = 0;
-  if (first_on_device(&seen)) cudaFuncSetAttribute(sw_fwd_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdSmem<D>::total);
-  sw_fwd_tc_kernel<T, D><<<(unsigned)grid, kFwdThreads, FwdSmem<D>::total, st>>>(mq, mk, mv, t, bf16);
-  return (int)cudaGetLastError();
+  // Heads of 64: one query tile to a CTA and two CTAs on an SM while walks are short and their starts and ends count (64 x 128, 12
+  // heads: 24 us against 39; 16 x 512: 33 and 38; 4 x 4096, 16 over 4, window 128: 75 and 82; 8 x 2048, 12 heads, no window: 114
+  // and 116); for long walks two tiles that share their keys (4 x 4096, 16 over 4, no window: 218 us against 238).
+  if (D == 64 && p.window <= 2048) return tc_forward_launch<T, 64, 1>(mq, mk, mv, t, bf16, st);
+  return tc_forward_launch<T, D, 2>(mq, mk, mv, t, bf16, st);
 }

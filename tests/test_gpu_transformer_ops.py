@@ -125,6 +125,13 @@ def test_attention_ragged_and_what_lies_behind(dtype, D, window, sinks):
 
 
 @pytest.mark.parametrize('dtype', HALF)
+@pytest.mark.parametrize('Hq,Hk,window,sinks', [(2, 1, 0, 0), (1, 1, 2049, 3), (3, 3, 2048, 130)])
+def test_attention_long_walks_of_small_heads(dtype, Hq, Hk, window, sinks):
+    q, k, v, g = (randn(1, 2500, h, 64, dtype=dtype) for h in (Hq, Hk, Hk, Hq))
+    check_attention(q, k, v, torch.tensor([2390], dtype=torch.int32, device=dev()), window, sinks, g)
+
+
+@pytest.mark.parametrize('dtype', HALF)
 @pytest.mark.parametrize('B,T,Hq,Hk,D,sinks', [(60, 900, 1, 1, 64, 130), (20, 1300, 4, 4, 128, 4), (160, 600, 2, 1, 64, 1)])
 def test_attention_with_sinks_seen_by_many_later_tiles(dtype, B, T, Hq, Hk, D, sinks):
     valid = torch.randint(0, T + 1, (B,), device=dev(), dtype=torch.int32)
