@@ -131,12 +131,12 @@ __device__ __forceinline__ void tc_load_tile(uint8_t* dst, const CUtensorMap* ma
 #pragma unroll
   for (int c = 0; c < D / 64; ++c) tma_load_4d(dst + c * kTcHalf, map, c * 64, h, t, b, bar);
 }
-// Rows [from, 128) of a tile become zeros (a whole warp): what lies behind a sequence must not reach a sum, not even times 0.
-template <int D>
+// Rows [from, kRows) of a tile become zeros (a whole warp): what lies behind a sequence must not reach a sum, not even times 0.
+template <int D, int kRows = kTcRows>
 __device__ __forceinline__ void tc_clear_rows(uint8_t* tile, int from) {
   const int lane = threadIdx.x & 31;
   for (int c = 0; c < D / 64; ++c)
-    for (uint32_t o = (uint32_t)from * 128u + lane * 16u; o < kTcHalf; o += 512u)
+    for (uint32_t o = (uint32_t)from * 128u + lane * 16u; o < kRows * 128u; o += 512u)
       *reinterpret_cast<uint4*>(tile + c * kTcHalf + o) = make_uint4(0, 0, 0, 0);
   fence_async_smem();
   __syncwarp();
@@ -519,14 +519,14 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// 4-D tensor map over [B, T, H, D] with element strides; box = 64 channels x 1 head x 128 positions.
-static int tc_map(CUtensorMap* map, const void* base, int bf16, int B, int T, int H, int D, SwStride s) {
+// 4-D tensor map over [B, T, H, D] with element strides; box = 64 channels x 1 head x `rows` positions.
+static int tc_map(CUtensorMap* map, const void* base, int bf16, int B, int T, int H, int D, SwStride s, int rows = kTcRows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return -10;
   auto bytes = [&](int64_t stride, int size) { return size == 1 ? (cuuint64_t)D * 2 : (cuuint64_t)stride * 2; };   // an axis of one entry is never walked
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T, (cuuint64_t)B};
   cuuint64_t strides[3] = {bytes(s.h, H), bytes(s.t, T), bytes(s.b, B)};
-  cuuint32_t box[4] = {64, 1, (cuuint32_t)kTcRows, 1};
+  cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult rc = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
                          dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

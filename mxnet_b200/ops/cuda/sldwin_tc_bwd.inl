@@ -63,7 +63,6 @@ __device__ __forceinline__ void bwd_probs(uint32_t (&x)[32], const float* lse, f
 // TMEM columns: S of even tiles | S of odd tiles | dP (128 each) | dQ (D).  dS lies over the S it comes from: each part of the
 // columns over its own.
 constexpr int kBwdThreads = 576, kBwdMma = 16, kBwdTma = 17;
-constexpr int kDkvThreads = 608, kDkvStat = 18;           // one warp more: log-sum-exps and deltas of the query rows
 template <int D> struct DqSmem {
   static constexpr uint32_t tile = (D / 64) * kTcHalf;
   static constexpr int kst = 3, vst = 2;
@@ -341,21 +340,25 @@ __device__ __forceinline__ float* dkv_far_part(const DkvSplit& s, int64_t bh_all
   return s.parts + ((near + (((int64_t)hs * s.far_chunks + chunk) * bh_all + bh) * s.sink_tiles + kt) * 2) * kTcRows * D;
 }
 
-template <int D> struct DkvSmem {
-  static constexpr uint32_t tile = (D / 64) * kTcHalf;
+// kQ: query rows of a step.  With 64 of them heads of 64 fit twice on an SM (shared memory, 256 TMEM columns, 352 threads).
+template <int D, int kQ> struct DkvForm {
+  static_assert(kQ == 128 || D == 64, "");
+  static constexpr int parts = kQ / 32, rows_warps = 4 * parts, mma = rows_warps, tma = mma + 1, stats = mma + 2, threads = 32 * (mma + 3);
+  static constexpr uint32_t tmem_dp = kQ, tmem_dv = 2 * kQ, tmem_dk = 2 * kQ + D, tmem_cols = kQ == 64 ? 256 : 512;
+  static constexpr uint32_t tile = (D / 64) * kTcHalf, qtile = tile * kQ / 128;
   static constexpr int qst = 3, gst = 2;
-  static constexpr uint32_t k = 0, v = tile, q = 2 * tile, g = q + qst * tile, stat = g + gst * tile, bars = stat + 2048;
+  static constexpr uint32_t k = 0, v = tile, q = 2 * tile, g = q + qst * qtile, stat = g + gst * qtile, bars = stat + 2048;
   static constexpr uint32_t total = bars + 256;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kDkvThreads, 1)
+template <typename T, int D, int kQ>
+__global__ void __launch_bounds__(32 * (kQ / 8 + 3), kQ == 64 ? 2 : 1)
 sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g, const TcParams p,
                  const DkvSplit sp, int bf16) {
-  typedef DkvSmem<D> L;
+  typedef DkvForm<D, kQ> L;
   extern __shared__ __align__(1024) uint8_t smem[];
-  float* s_stat = reinterpret_cast<float*>(smem + L::stat);        // [2 stages][-lse 128 | -delta 128]
+  float* s_stat = reinterpret_cast<float*>(smem + L::stat);        // [2 stages][-lse kQ | -delta kQ]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
   uint64_t *kv_full = bars, *q_full = bars + 1, *q_empty = bars + 4, *g_full = bars + 7, *g_empty = bars + 9, *st_full = bars + 11,
            *st_empty = bars + 13, *s_full = bars + 15, *dp_full = bars + 16, *p_ready = bars + 17, *ds_ready = bars + 18, *done = bars + 19,
@@ -379,9 +382,10 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int chunk = far ? unit / sp.sink_tiles : 0;
   const int n = warp_uniform(tc_valid(p, b));
   const int k0 = kt * kTcRows;
-  const int last_tile = n > 0 ? (n - 1) / kTcRows : -1;
-  const int qlo = far ? kt + sp.near_span + 1 + chunk * sp.far_len : kt;
-  const int qhi = min(last_tile, far ? qlo + sp.far_len - 1 : qlo + sp.near_span);
+  const int last_q = n > 0 ? (n - 1) / kQ : -1;                    // in steps of kQ queries
+  const int from_tile = far ? kt + sp.near_span + 1 + chunk * sp.far_len : kt;
+  const int qlo = from_tile * (kTcRows / kQ);
+  const int qhi = (int)min((int64_t)last_q, ((int64_t)from_tile + (far ? sp.far_len : sp.near_span + 1)) * (kTcRows / kQ) - 1);
   const int per_head = max(0, qhi - qlo + 1);
   const int nit = k0 < n ? per_head * heads : 0;
 
@@ -398,20 +402,19 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     return;
   }
   uint32_t tmem = 0;
-  if (warp == kBwdTma) {
+  if (warp == L::tma) {
     if (lane == 0) {
       mbar_init(kv_full, 1);
       for (int s = 0; s < L::qst; ++s) { mbar_init(&q_full[s], 1); mbar_init(&q_empty[s], 1); }
-      for (int s = 0; s < 2; ++s) { mbar_init(&g_full[s], 1); mbar_init(&g_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], 16); }
-      mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_ready, 16); mbar_init(ds_ready, 16); mbar_init(done, 1); mbar_init(patch, 1);
+      for (int s = 0; s < 2; ++s) { mbar_init(&g_full[s], 1); mbar_init(&g_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], L::rows_warps); }
+      mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_ready, L::rows_warps); mbar_init(ds_ready, L::rows_warps); mbar_init(done, 1); mbar_init(patch, 1);
       mbar_init(drain, 1);
       *abort_flag = 0;
     }
-    tc_start_loader<kDkvThreads>();
-  } else tmem = tc_start<kDkvThreads>(tmem_slot, warp == kBwdMma);
-  constexpr uint32_t kDp = 128, kDv = 256, kDk = 256 + D;
+    tc_start_loader<L::threads>();
+  } else tmem = tc_start<L::threads, L::tmem_cols>(tmem_slot, warp == L::mma);
 
-  if (warp == kBwdTma) {
+  if (warp == L::tma) {
     if (nit > 0) {
       if (lane == 0) {
         mbar_expect_tx(kv_full, 2 * L::tile);
@@ -422,28 +425,28 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       int nq = 0, ng = 0;
       uint32_t patched = 0;
       for (int it = 0; it < nit && ok; ++it) {
-        const int h = h_first + it / per_head, q0 = (qlo + it % per_head) * kTcRows;
+        const int h = h_first + it / per_head, q0 = (qlo + it % per_head) * kQ;
         const int sq = it % L::qst, sg = it % L::gst;
-        const bool ends = q0 + kTcRows > n && n < p.T;            // the sequence ends inside this tile
-        uint8_t *tq = smem + L::q + sq * L::tile, *tg = smem + L::g + sg * L::tile;
+        const bool ends = q0 + kQ > n && n < p.T;            // the sequence ends inside this tile
+        uint8_t *tq = smem + L::q + sq * L::qtile, *tg = smem + L::g + sg * L::qtile;
         if (it >= L::qst && !(ok = mbar_wait_warp(&q_empty[sq], (uint32_t)(it / L::qst + 1) & 1u))) break;
         if (lane == 0) {
           uint64_t* bar = ends ? patch : &q_full[sq];
-          mbar_expect_tx(bar, ends ? 2 * L::tile : L::tile);
+          mbar_expect_tx(bar, ends ? 2 * L::qtile : L::qtile);
           tc_load_tile<D>(tq, &map_q, h, q0, b, bar);
         }
         nq = ends ? it : it + 1;
         if (it >= L::gst && !(ok = mbar_wait_warp(&g_empty[sg], (uint32_t)(it / L::gst + 1) & 1u))) break;
         if (lane == 0) {
           uint64_t* bar = ends ? patch : &g_full[sg];
-          if (!ends) mbar_expect_tx(bar, L::tile);
+          if (!ends) mbar_expect_tx(bar, L::qtile);
           tc_load_tile<D>(tg, &map_g, h, q0, b, bar);
         }
         ng = ends ? it : it + 1;
         if (ends) {
           if (!(ok = mbar_wait_warp(patch, patched++ & 1u))) break;
-          tc_clear_rows<D>(tq, n - q0);
-          tc_clear_rows<D>(tg, n - q0);
+          tc_clear_rows<D, kQ>(tq, n - q0);
+          tc_clear_rows<D, kQ>(tg, n - q0);
           if (lane == 0) { mbar_arrive(&q_full[sq]); mbar_arrive(&g_full[sg]); }
         }
       }
@@ -456,40 +459,40 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
       }
     }
-  } else if (warp == kDkvStat) {
+  } else if (warp == L::stats) {
     bool ok = true;
     float f = BwdRange<T>::unshift;
     if (BwdRange<T>::scaled) {
       float big = 0.f;
       for (int e = lane; e < nit; e += 32)
-        big = fmaxf(big, p.gmax[((int64_t)b * p.Hq + h_first + e / per_head) * sp.tiles + qlo + e % per_head]);
+        big = fmaxf(big, p.gmax[((int64_t)b * p.Hq + h_first + e / per_head) * sp.tiles + (qlo + e % per_head) / (kTcRows / kQ)]);
       const float up = bwd_factor(warp_max(big));
       f *= up;
       if (lane == 0) s_factor[0] = up;
     }
     for (int it = 0; it < nit && ok; ++it) {
-      const int h = h_first + it / per_head, q0 = (qlo + it % per_head) * kTcRows;
+      const int h = h_first + it / per_head, q0 = (qlo + it % per_head) * kQ;
       // log-sum-exp and delta of the tile's rows; a row that is not there gets +inf: probability 0
       if (it >= 2 && !(ok = mbar_wait_warp(&st_empty[it & 1], (uint32_t)(it / 2 + 1) & 1u))) break;
       const int64_t at = ((int64_t)b * p.Hq + h) * p.T + q0;
-      float* st = s_stat + (it & 1) * 256;
+      float* st = s_stat + (it & 1) * 2 * kQ;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < kQ / 32; ++e) {
         const int c = lane + 32 * e;
         st[c] = q0 + c < n ? BwdRange<T>::shift - p.lse[at + c] : -INFINITY;
-        st[128 + c] = q0 + c < n ? -p.delta[at + c] * f : 0.f;
+        st[kQ + c] = q0 + c < n ? -p.delta[at + c] * f : 0.f;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&st_full[it & 1]);
     }
     if (!ok) *abort_flag = 1;
-  } else if (warp == kBwdMma) {
+  } else if (warp == L::mma) {
     if (nit > 0) {
-      const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
+      const uint32_t id_s = make_idesc(bf16, kQ, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
       const uint64_t dk = make_desc(smem_u32(smem + L::k)), dv = make_desc(smem_u32(smem + L::v)), dq = make_desc(smem_u32(smem + L::q)),
                      dg = make_desc(smem_u32(smem + L::g)), dqm = make_desc_mn(smem_u32(smem + L::q), kTcHalf),
                      dgm = make_desc_mn(smem_u32(smem + L::g), kTcHalf);
-      constexpr uint64_t step = L::tile >> 4;
+      constexpr uint64_t step = L::qtile >> 4;
       bool ok = mbar_wait_warp(kv_full, 0);
       auto scores = [&](int it) {
         ok = mbar_wait_warp(&q_full[it % L::qst], (uint32_t)(it / L::qst) & 1u);
@@ -499,7 +502,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       auto dprobs = [&](int it) {
         ok = mbar_wait_warp(&g_full[it % L::gst], (uint32_t)(it / L::gst) & 1u);
         tc_fence_after();
-        if (ok && elect_one()) { tc_scores<D>(tmem + kDp, dv, dg + (it % L::gst) * step, id_s); umma_commit(dp_full); }
+        if (ok && elect_one()) { tc_scores<D>(tmem + L::tmem_dp, dv, dg + (it % L::gst) * step, id_s); umma_commit(dp_full); }
       };
       if (ok) scores(0);
       if (ok) dprobs(0);
@@ -508,7 +511,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          tc_accumulate<2>(tmem + kDv, tmem, dgm + (it % L::gst) * step, id_o, it > 0 ? 1u : 0u);
+          tc_accumulate<2, 0, kQ / 16>(tmem + L::tmem_dv, tmem, dgm + (it % L::gst) * step, id_o, it > 0 ? 1u : 0u);
           umma_commit(&g_empty[it % L::gst]);                     // dP of this tile was issued before: dO is done with
         }
         if (it + 1 < nit) scores(it + 1);
@@ -517,7 +520,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          tc_accumulate<2>(tmem + kDk, tmem + kDp, dqm + (it % L::qst) * step, id_o, it > 0 ? 1u : 0u);
+          tc_accumulate<2, 0, kQ / 16>(tmem + L::tmem_dk, tmem + L::tmem_dp, dqm + (it % L::qst) * step, id_o, it > 0 ? 1u : 0u);
           umma_commit(&q_empty[it % L::qst]);
         }
         if (it + 1 < nit) dprobs(it + 1);
@@ -529,20 +532,20 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const int part = warp >> 2, quad = warp & 3;
     const int row = quad * 32 + lane, j = k0 + row;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-    const uint32_t ts = tmem + 32 * part + lane_off, td = tmem + kDp + 32 * part + lane_off;
+    const uint32_t ts = tmem + 32 * part + lane_off, td = tmem + L::tmem_dp + 32 * part + lane_off;
     const float sc = p.scale * kSwLog2e;
     float f = 1.f;                                                // of dO in dS
     bool ok = true;
     for (int it = 0; it < nit; ++it) {
-      const int q0 = (qlo + it % per_head) * kTcRows;
-      const float* st = s_stat + (it & 1) * 256 + 32 * part;
+      const int q0 = (qlo + it % per_head) * kQ;
+      const float* st = s_stat + (it & 1) * 2 * kQ + 32 * part;
       ok = mbar_wait_warp(&st_full[it & 1], (uint32_t)(it / 2) & 1u) && mbar_wait_warp(s_full, (uint32_t)it & 1u);
       if (!ok) break;
       tc_fence_after();
       uint32_t x[32], y[32];
       tmem_ld32(ts, x);
       tmem_wait_ld32(x);
-      const bool whole = k0 + kTcRows - 1 <= q0 && (q0 + kTcRows - 1 - k0 < p.window || k0 + kTcRows <= p.sinks);
+      const bool whole = k0 + kTcRows - 1 <= q0 && (q0 + kQ - 1 - k0 < p.window || k0 + kTcRows <= p.sinks);
       bwd_probs(x, st, sc);
       if (!whole) {
         // query i = base + c sees key j when c >= j - base, and c < j - base + window or j is a sink
@@ -572,7 +575,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tmem_wait_ld32(y);
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
-        const float2 d2 = *reinterpret_cast<const float2*>(st + 128 + c);
+        const float2 d2 = *reinterpret_cast<const float2*>(st + kQ + c);
         const f32x2 dp = pack_f2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), nd = pack_f2(d2.x, d2.y);
         float a, b;
         unpack_f2(mul_f2(pack_f2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), BwdRange<T>::scaled ? fma_f2(dp, fu2, nd) : add_f2(dp, nd)), a, b);
@@ -588,10 +591,11 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (!ok) *abort_flag = 1;
     tc_fence_after();
     if (ok) {
-      // parts 0 and 1 write the halves of dK, parts 2 and 3 those of dV
-      const int which = part >> 1, from = (part & 1) * (D / 2);
+      // the first half of the parts writes dK, each an equal share of the channels, the second dV
+      constexpr int kEach = L::parts / 2, kWide = D / kEach;
+      const int which = part / kEach, from = part % kEach * kWide;
       const float mul = which == 0 ? p.scale / f : BwdRange<T>::unshift;
-      const uint32_t acc = tmem + (which == 0 ? kDk : kDv) + from + lane_off;
+      const uint32_t acc = tmem + (which == 0 ? L::tmem_dk : L::tmem_dv) + from + lane_off;
       const bool parts = kt < sp.part_tiles;
       const bool live = j < n && nit > 0;
       float* sum = nullptr;
@@ -601,7 +605,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
       T* dst = static_cast<T*>(which == 0 ? p.dk : p.dv) + (((int64_t)b * p.T + j) * p.Hk + hk) * D + from;
 #pragma unroll 1
-      for (int c0 = 0; c0 < D / 2; c0 += 32) {
+      for (int c0 = 0; c0 < kWide; c0 += 32) {
         uint32_t o[32];
         if (nit > 0) { tmem_ld32(acc + c0, o); tmem_wait_ld32(o); }
         if (parts) {
@@ -628,7 +632,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
     }
   }
-  tc_finish(tmem, 512, warp, kBwdMma, abort_flag, p.error_flag);
+  tc_finish(tmem, L::tmem_cols, warp, L::mma, abort_flag, p.error_flag);
 }
 
 // dK and dV of the key tiles that came in parts: blockIdx.x = (sample and key head, key tile), blockIdx.y a stretch of the tile.
@@ -696,6 +700,21 @@ static int64_t dkv_part_floats(const SwParams& p) {
   return ((int64_t)s.hsplit * p.B * p.Hk * s.part_tiles + (int64_t)s.hsplit * s.far_chunks * p.B * p.Hk * s.sink_tiles) * 2 * kTcRows * p.D;
 }
 
+template <typename T, int D, int kQ>
+static int dkv_launch(const SwParams& p, const TcParams& t, const DkvSplit& s, unsigned grid, int bf16, cudaStream_t st) {
+  typedef DkvForm<D, kQ> L;
+  CUtensorMap mq, mk, mv, mg;
+  int rc = tc_map(&mq, p.q, bf16, p.B, p.T, p.Hq, D, p.sq, kQ);
+  if (!rc) rc = tc_map(&mk, p.k, bf16, p.B, p.T, p.Hk, D, p.sk);
+  if (!rc) rc = tc_map(&mv, p.v, bf16, p.B, p.T, p.Hk, D, p.sv);
+  if (!rc) rc = tc_map(&mg, p.dout, bf16, p.B, p.T, p.Hq, D, p.sdo, kQ);
+  if (rc) return rc;
+  static unsigned long long seen = 0;
+  if (first_on_device(&seen)) cudaFuncSetAttribute(sw_dkv_tc_kernel<T, D, kQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::total);
+  sw_dkv_tc_kernel<T, D, kQ><<<grid, L::threads, L::total, st>>>(mq, mk, mv, mg, t, s, bf16);
+  return (int)cudaGetLastError();
+}
+
 template <typename T, int D>
 static int tc_backward(const SwParams& p, float* parts, int bf16, int* error_flag, cudaStream_t st) {
   CUtensorMap mq, mk, mv, mg;
@@ -712,16 +731,14 @@ static int tc_backward(const SwParams& p, float* parts, int bf16, int* error_fla
   const int64_t gq = (int64_t)s.tiles * t.items, gk = ((int64_t)s.tiles + (int64_t)s.sink_tiles * s.far_chunks) * s.items;
   if (gq > 0x7fffffff || gk > 0x7fffffff) return -2;
   static unsigned long long seen = 0;
-  if (first_on_device(&seen)) {
-    cudaFuncSetAttribute(sw_dq_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DqSmem<D>::total);
-    cudaFuncSetAttribute(sw_dkv_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DkvSmem<D>::total);
-  }
+  if (first_on_device(&seen)) cudaFuncSetAttribute(sw_dq_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DqSmem<D>::total);
   sw_dq_tc_kernel<T, D><<<(unsigned)gq, kBwdThreads, DqSmem<D>::total, st>>>(mq, mk, mv, mg, t, bf16);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
-  sw_dkv_tc_kernel<T, D><<<(unsigned)gk, kDkvThreads, DkvSmem<D>::total, st>>>(mq, mk, mv, mg, t, s, bf16);
-  e = cudaGetLastError();
-  if (e != cudaSuccess || !s.part_tiles) return (int)e;
+  // Heads of 64: steps of 64 queries, two CTAs on an SM, where there are CTAs for both (whole backward pass, 12 heads: 64 x 128 85 us
+  // against 99, 16 x 512 102 and 116, 8 x 2048 303 and 335; 1 x 1024, 96 CTAs, 44 and 40).
+  const int code = D == 64 && gk > sm_count() ? dkv_launch<T, 64, 64>(p, t, s, (unsigned)gk, bf16, st) : dkv_launch<T, D, 128>(p, t, s, (unsigned)gk, bf16, st);
+  if (code || !s.part_tiles) return code;
   sw_dkv_join_kernel<T, D><<<dim3((unsigned)(s.part_tiles * p.B * p.Hk), 2 * kTcRows * D / 8 / 256), 256, 0, st>>>(t, s);
   return (int)cudaGetLastError();
 }

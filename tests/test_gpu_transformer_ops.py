@@ -125,6 +125,20 @@ def test_attention_ragged_and_what_lies_behind(dtype, D, window, sinks):
 
 
 @pytest.mark.parametrize('dtype', HALF)
+@pytest.mark.parametrize('Hq,Hk,window,sinks', [(3, 3, 0, 0), (4, 2, 70, 3), (3, 3, 129, 65)])
+def test_attention_of_many_short_sequences(dtype, Hq, Hk, window, sinks):
+    T = 520
+    valid = torch.tensor([0, 1, 2, 63, 64, 65, 66, 127, 128, 129, 191, 192, 193, 256, 257, 383, 385, 449, 513, T, T + 1, 300, 320, 500],
+                         dtype=torch.int32, device=dev())
+    q, k, v, g = (randn(24, T, h, 64, dtype=dtype) for h in (Hq, Hk, Hk, Hq))
+    got = check_attention(q, k, v, valid, window, sinks, g)
+    behind = (torch.arange(T, device=dev())[None] >= valid[:, None])[:, :, None, None]
+    for fill in (math.nan, math.inf):
+        again = run_attention(*(t.masked_fill(behind, fill) for t in (q, k, v)), valid, window, sinks, g.masked_fill(behind, fill))
+        assert all(torch.equal(a, b) for a, b in zip(got, again)), fill
+
+
+@pytest.mark.parametrize('dtype', HALF)
 @pytest.mark.parametrize('Hq,Hk,window,sinks', [(2, 1, 0, 0), (1, 1, 2049, 3), (3, 3, 2048, 130)])
 def test_attention_long_walks_of_small_heads(dtype, Hq, Hk, window, sinks):
     q, k, v, g = (randn(1, 2500, h, 64, dtype=dtype) for h in (Hq, Hk, Hk, Hq))
