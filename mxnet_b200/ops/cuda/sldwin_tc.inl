@@ -105,20 +105,22 @@ __device__ __forceinline__ int tc_valid(const TcParams& p, int b) {
   return n < 0 ? 0 : (n > p.T ? p.T : n);
 }
 
-// Key tiles that queries [q0, q0 + 128) of a sequence of n tokens see: the first `ns` tiles (sinks) and tiles [lo, hi].
-struct KeyRange {
+// Tiles of kKeys keys that queries [q0, q0 + 128) of a sequence of n tokens see: the first `ns` (sinks) and those from lo to hi.
+template <int kKeys>
+struct KeyTiles {
   int ns, lo, hi;
-  __device__ __forceinline__ KeyRange(int q0, int n, int window, int sinks) {
+  __device__ __forceinline__ KeyTiles(int q0, int n, int window, int sinks) {
     const int last = min(q0 + kTcRows, n) - 1;           // last query that is there
     if (last < q0) { ns = 0; lo = 0; hi = -1; return; }
-    hi = last / kTcRows;
+    hi = last / kKeys;
     const int64_t first = (int64_t)q0 - window + 1;
-    lo = first <= 0 ? 0 : (int)(first / kTcRows);
-    ns = min((min(sinks, last + 1) + kTcRows - 1) / kTcRows, lo);
+    lo = first <= 0 ? 0 : (int)(first / kKeys);
+    ns = min((min(sinks, last + 1) + kKeys - 1) / kKeys, lo);
   }
   __device__ __forceinline__ bool has(int kt) const { return kt <= hi && (kt >= lo || kt < ns); }
   __device__ __forceinline__ int count() const { return hi < lo ? 0 : ns + hi - lo + 1; }
 };
+typedef KeyTiles<kTcRows> KeyRange;
 
 // Bits of 32 neighbouring keys that a query sees: keys up to `hi`, of them those behind `gone` and those up to `sink` (indexes
 // relative to the first of the 32).

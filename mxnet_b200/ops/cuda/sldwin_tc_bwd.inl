@@ -10,7 +10,8 @@
 // (512 for 128 x 128 x 128) and the chain scores, probabilities, next scores the rest; then the start and the end of each CTA, with
 // one CTA on an SM (shared memory and TMEM are full).
 // 2 x 4096, 16 heads over 4 of 128, window 1024, 4 sinks, bf16: dQ 134 us (tensor pipe active 42 %), dK and dV 147 us (61 %).
-// 16 x 512 padded, 12 heads of 64, fp16: 35 and 41 us, a chain of one to four tiles in each CTA (tensor pipe 10 %).
+// Heads of 64 fit twice on an SM in steps of 64, so that one CTA's start and end run under the other's walk: 16 x 512 padded,
+// 12 heads, fp16: 25 and 32 us instead of 35 and 41.
 //
 // Range in fp16: probabilities enter the dV product 2^14 times their value (at most 2^14, digits kept down to 2^-28), and dS is
 // formed from dO scaled by the power of two that brings the largest dO of the CTA's tiles into [8, 16): neither small
@@ -62,21 +63,26 @@ __device__ __forceinline__ void bwd_probs(uint32_t (&x)[32], const float* lse, f
 // ------------------------------------------------------------------------------------------------ dQ
 // TMEM columns: S of even tiles | S of odd tiles | dP (128 each) | dQ (D).  dS lies over the S it comes from: each part of the
 // columns over its own.
-constexpr int kBwdThreads = 576, kBwdMma = 16, kBwdTma = 17;
-template <int D> struct DqSmem {
-  static constexpr uint32_t tile = (D / 64) * kTcHalf;
+// kKeys: keys of a step.  With 64 of them heads of 64 fit twice on an SM (shared memory, 256 TMEM columns, 320 threads).
+template <int D, int kKeys> struct DqForm {
+  static_assert(kKeys == 128 || D == 64, "");
+  static constexpr int parts = kKeys / 32, rows_warps = 4 * parts, mma = rows_warps, tma = mma + 1, threads = 32 * (mma + 2);
+  static constexpr uint32_t tmem_dp = 2 * kKeys, tmem_dq = 3 * kKeys, tmem_cols = kKeys == 64 ? 256 : 512;
+  static constexpr uint32_t tile = (D / 64) * kTcHalf, ktile = tile * kKeys / 128;
   static constexpr int kst = 3, vst = 2;
-  static constexpr uint32_t q = 0, g = tile, k = 2 * tile, v = k + kst * tile, delta = v + vst * tile, bars = delta + 1024;
+  // delta: [128], then the warps' largest |dO|; sums: [parts][128], with steps of 128 keys in a stage that two steps leave unused
+  static constexpr uint32_t q = 0, g = tile, k = 2 * tile, v = k + kst * ktile, delta = v + vst * ktile,
+                            sums = kKeys == 64 ? delta + 1024 : k + 2 * ktile, bars = kKeys == 64 ? sums + parts * 512 : delta + 1024;
   static constexpr uint32_t total = bars + 256;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+template <typename T, int D, int kKeys>
+__global__ void __launch_bounds__(32 * (kKeys / 8 + 2), kKeys == 64 ? 2 : 1)
 sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g, const TcParams p, int bf16) {
-  typedef DqSmem<D> L;
+  typedef DqForm<D, kKeys> L;
   extern __shared__ __align__(1024) uint8_t smem[];
-  float* s_delta = reinterpret_cast<float*>(smem + L::delta);      // [128], then the warps' largest |dO|
+  float* s_delta = reinterpret_cast<float*>(smem + L::delta);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
   uint64_t *qg_full = bars, *k_full = bars + 1, *k_empty = bars + 4, *v_full = bars + 7, *v_empty = bars + 9, *sd_full = bars + 11,
            *dp_empty = bars + 12, *ds_full = bars + 13, *done = bars + 14, *patch = bars + 15, *drain = bars + 16;
@@ -92,31 +98,37 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const int b = item / p.Hq, h = item % p.Hq, hk = h / (p.Hq / p.Hk);
   const int n = warp_uniform(tc_valid(p, b));
   const int q0 = qt * kTcRows;
-  const KeyRange r(q0, n, p.window, p.sinks);
+  const KeyTiles<kKeys> r(q0, n, p.window, p.sinks);
   const int ntiles = r.count();
-  auto key_tile = [&](int j) { return j < r.ns ? j : r.lo + (j - r.ns); };
+  // Rows that see few keys (those whose keys lie in 128 rows, the first query tile's among them) get delta from the sum of P dP
+  // instead of from the rounded output, whose rounding is not small beside dP - delta there: such a CTA walks its tiles once for
+  // the sums and once more for dQ.
+  const int ahead = ntiles <= kTcRows / kKeys ? ntiles : 0, nit = ahead + ntiles;
+  auto key_tile = [&](int it) {
+    const int j = it < ahead ? it : it - ahead;
+    return j < r.ns ? j : r.lo + (j - r.ns);
+  };
 
   if (ntiles == 0) {                                              // rows behind the sequence
     const int rows = min(kTcRows, p.T - q0);
     tc_zero_rows(static_cast<T*>(p.dq) + (((int64_t)b * p.T + q0) * p.Hq + h) * D, rows, D / 8, (int64_t)p.Hq * D / 8);
-    for (int e = threadIdx.x; e < rows; e += kBwdThreads) p.delta[((int64_t)b * p.Hq + h) * p.T + q0 + e] = 0.f;
+    for (int e = threadIdx.x; e < rows; e += L::threads) p.delta[((int64_t)b * p.Hq + h) * p.T + q0 + e] = 0.f;
     if (BwdRange<T>::scaled && threadIdx.x == 0) p.gmax[((int64_t)b * p.Hq + h) * tiles + qt] = 0.f;
     return;
   }
   uint32_t tmem = 0;
-  if (warp == kBwdTma) {
+  if (warp == L::tma) {
     if (lane == 0) {
       mbar_init(qg_full, 1);
       for (int s = 0; s < L::kst; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
       for (int s = 0; s < L::vst; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
-      mbar_init(sd_full, 1); mbar_init(dp_empty, 16); mbar_init(ds_full, 16); mbar_init(done, 1); mbar_init(patch, 1); mbar_init(drain, 1);
+      mbar_init(sd_full, 1); mbar_init(dp_empty, L::rows_warps); mbar_init(ds_full, L::rows_warps); mbar_init(done, 1); mbar_init(patch, 1); mbar_init(drain, 1);
       *abort_flag = 0;
     }
-    tc_start_loader<kBwdThreads>();
-  } else tmem = tc_start<kBwdThreads>(tmem_slot, warp == kBwdMma);
-  constexpr uint32_t kDp = 256, kDq = 384;
+    tc_start_loader<L::threads>();
+  } else tmem = tc_start<L::threads, L::tmem_cols>(tmem_slot, warp == L::mma);
 
-  if (warp == kBwdTma) {
+  if (warp == L::tma) {
     if (ntiles > 0) {
       if (lane == 0) {
         mbar_expect_tx(qg_full, 2 * L::tile);
@@ -125,26 +137,27 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
       bool ok = true;
       int nk = 0, nv = 0;
-      for (int j = 0; j < ntiles; ++j) {
+      uint32_t patched = 0;
+      for (int j = 0; j < nit; ++j) {
         const int sk = j % L::kst, sv = j % L::vst, kt = key_tile(j);
         if (j >= L::kst && !(ok = mbar_wait_warp(&k_empty[sk], (uint32_t)(j / L::kst + 1) & 1u))) break;
-        const bool ends = (kt + 1) * kTcRows > n && n < p.T;      // the sequence ends inside this tile: dS K must not meet what follows
-        uint8_t* tile = smem + L::k + sk * L::tile;
+        const bool ends = (kt + 1) * kKeys > n && n < p.T;      // the sequence ends inside this tile: dS K must not meet what follows
+        uint8_t* tile = smem + L::k + sk * L::ktile;
         if (lane == 0) {
           uint64_t* bar = ends ? patch : &k_full[sk];
-          mbar_expect_tx(bar, L::tile);
-          tc_load_tile<D>(tile, &map_k, hk, kt * kTcRows, b, bar);
+          mbar_expect_tx(bar, L::ktile);
+          tc_load_tile<D>(tile, &map_k, hk, kt * kKeys, b, bar);
         }
         nk = ends ? j : j + 1;
         if (ends) {
-          if (!(ok = mbar_wait_warp(patch, 0))) break;
-          tc_clear_rows<D>(tile, n - kt * kTcRows);
+          if (!(ok = mbar_wait_warp(patch, patched++ & 1u))) break;
+          tc_clear_rows<D, kKeys>(tile, n - kt * kKeys);
           if (lane == 0) mbar_arrive(&k_full[sk]);
         }
         if (j >= L::vst && !(ok = mbar_wait_warp(&v_empty[sv], (uint32_t)(j / L::vst + 1) & 1u))) break;
         if (lane == 0) {
-          mbar_expect_tx(&v_full[sv], L::tile);
-          tc_load_tile<D>(smem + L::v + sv * L::tile, &map_v, hk, kt * kTcRows, b, &v_full[sv]);
+          mbar_expect_tx(&v_full[sv], L::ktile);
+          tc_load_tile<D>(smem + L::v + sv * L::ktile, &map_v, hk, kt * kKeys, b, &v_full[sv]);
         }
         nv = j + 1;
       }
@@ -157,32 +170,32 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
       }
     }
-  } else if (warp == kBwdMma) {
+  } else if (warp == L::mma) {
     if (ntiles > 0) {
-      const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
+      const uint32_t id_s = make_idesc(bf16, kKeys, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
       const uint64_t dq = make_desc(smem_u32(smem + L::q)), dg = make_desc(smem_u32(smem + L::g)), dk = make_desc(smem_u32(smem + L::k)),
                      dv = make_desc(smem_u32(smem + L::v)), dkm = make_desc_mn(smem_u32(smem + L::k), kTcHalf);
-      constexpr uint64_t step = L::tile >> 4;
+      constexpr uint64_t step = L::ktile >> 4;
       bool ok = mbar_wait_warp(qg_full, 0);
       auto scores = [&](int j) {
         ok = mbar_wait_warp(&k_full[j % L::kst], (uint32_t)(j / L::kst) & 1u);
         tc_fence_after();
-        if (ok && elect_one()) tc_scores<D>(tmem + 128 * (j & 1), dq, dk + (j % L::kst) * step, id_s);
+        if (ok && elect_one()) tc_scores<D>(tmem + kKeys * (j & 1), dq, dk + (j % L::kst) * step, id_s);
       };
       auto dprobs = [&](int j) {
         ok = mbar_wait_warp(&v_full[j % L::vst], (uint32_t)(j / L::vst) & 1u);
         tc_fence_after();
         if (ok && elect_one()) {
-          tc_scores<D>(tmem + kDp, dg, dv + (j % L::vst) * step, id_s);
+          tc_scores<D>(tmem + L::tmem_dp, dg, dv + (j % L::vst) * step, id_s);
           umma_commit(sd_full);
           umma_commit(&v_empty[j % L::vst]);
         }
       };
       if (ok) scores(0);
       if (ok) dprobs(0);
-      if (ok && ntiles > 1) scores(1);
-      for (int j = 0; j < ntiles && ok; ++j) {
-        if (j + 1 < ntiles) {
+      if (ok && nit > 1) scores(1);
+      for (int j = 0; j < nit && ok; ++j) {
+        if (j + 1 < nit) {
           ok = mbar_wait_warp(dp_empty, (uint32_t)j & 1u);        // dP of this tile is in registers
           if (ok) dprobs(j + 1);
           if (!ok) break;
@@ -191,10 +204,11 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          tc_accumulate<2>(tmem + kDq, tmem + 128 * (j & 1), dkm + (j % L::kst) * step, id_o, j > 0 ? 1u : 0u);
+          if (j >= ahead)
+            tc_accumulate<2, 0, kKeys / 16>(tmem + L::tmem_dq, tmem + kKeys * (j & 1), dkm + (j % L::kst) * step, id_o, j > ahead ? 1u : 0u);
           umma_commit(&k_empty[j % L::kst]);
         }
-        if (j + 2 < ntiles) scores(j + 2);                        // over S and dS of this tile, read by the product before it
+        if (j + 2 < nit) scores(j + 2);                        // over S and dS of this tile, read by the product before it
       }
       if (elect_one()) umma_commit(ok ? done : drain);
       if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
@@ -204,12 +218,12 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const int row = quad * 32 + lane, i = q0 + row;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const bool live = i < n;
-    // delta = rowsum(dO * O) while the first products run: 8 rows for each warp, whole rows side by side in a load
-    constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+    // delta = rowsum(dO * O) while the first products run: a few rows for each warp, whole rows side by side in a load
+    constexpr int kLanes = D / 8, kRows = 32 / kLanes, kOwn = kTcRows / L::rows_warps;
     float big = 0.f;
 #pragma unroll
-    for (int r0 = 0; r0 < 8; r0 += kRows) {
-      const int rr = warp * 8 + r0 + lane / kLanes, ch = lane % kLanes * 8;
+    for (int r0 = 0; r0 < kOwn; r0 += kRows) {
+      const int rr = warp * kOwn + r0 + lane / kLanes, ch = lane % kLanes * 8;
       float dot = 0.f;
       if (q0 + rr < n) {
         const Vec16<T> a = ld16(static_cast<const T*>(p.o) + (((int64_t)b * p.T + q0 + rr) * p.Hq + h) * D + ch);
@@ -230,32 +244,31 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (lane == 0) s_delta[128 + warp] = big;
     }
     const float lse = live ? p.lse[((int64_t)b * p.Hq + h) * p.T + i] : INFINITY;
-    asm volatile("bar.sync 1, 512;" ::: "memory");
-    // Rows whose keys are all in one tile get delta from the sum of P dP instead of from the rounded output: with few keys the
-    // output's rounding is not small beside dP - delta.
-    const bool one_tile = ntiles == 1;
+    auto rows_meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * L::rows_warps) : "memory"); };
+    rows_meet();
     float delta = s_delta[row];
     float f = 1.f;
     if (BwdRange<T>::scaled) {
 #pragma unroll
-      for (int w = 0; w < 16; ++w) big = fmaxf(big, s_delta[128 + w]);
+      for (int w = 0; w < L::rows_warps; ++w) big = fmaxf(big, s_delta[128 + w]);
       if (threadIdx.x == 0) p.gmax[((int64_t)b * p.Hq + h) * tiles + qt] = big;
       f = bwd_factor(big);
     }
-    if (part == 0 && i < p.T && !one_tile) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = delta;
+    if (part == 0 && i < p.T && !ahead) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = delta;
     delta *= f;
     const float out_scale = p.scale / f;
     const float sc = p.scale * kSwLog2e;
     bool ok = true;
-    for (int j = 0; j < ntiles; ++j) {
+    float sum = 0.f;
+    for (int j = 0; j < nit; ++j) {
       const int kt = key_tile(j);
       ok = mbar_wait_warp(sd_full, (uint32_t)j & 1u);
       if (!ok) {
-        if (one_tile) asm volatile("bar.sync 1, 512;" ::: "memory");           // the warps that got through wait there
+        if (j < ahead) rows_meet();                               // the warps that got through wait there
         break;
       }
       tc_fence_after();
-      const uint32_t ts = tmem + 128 * (j & 1) + 32 * part + lane_off, td = tmem + kDp + 32 * part + lane_off;
+      const uint32_t ts = tmem + kKeys * (j & 1) + 32 * part + lane_off, td = tmem + L::tmem_dp + 32 * part + lane_off;
       uint32_t x[32], y[32];
       tmem_ld32(ts, x);
       tmem_ld32(td, y);
@@ -264,20 +277,25 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dp_empty);
-      const int k0 = kt * kTcRows;
-      const bool whole = k0 + kTcRows - 1 <= q0 && (q0 + kTcRows - 1 - k0 < p.window || k0 + kTcRows <= p.sinks);
+      const int k0 = kt * kKeys;
+      const bool whole = k0 + kKeys - 1 <= q0 && (q0 + kTcRows - 1 - k0 < p.window || k0 + kKeys <= p.sinks);
       const int base = k0 + 32 * part;
       const uint32_t seen = whole ? 0xffffffffu : tc_seen(i - base, i - p.window - base, p.sinks - 1 - base);
-      if (one_tile) {
-        float sum = 0.f;
+      if (j < ahead) {
 #pragma unroll
         for (int c = 0; c < 32; ++c) if (seen & 1u << c) sum += ex2(fmaf(__uint_as_float(x[c]), sc, -lse)) * __uint_as_float(y[c]);
-        float* s_sum = reinterpret_cast<float*>(smem + L::k + L::tile);        // [4][128] in a stage that a single tile leaves unused
-        s_sum[part * 128 + row] = sum;
-        asm volatile("bar.sync 1, 512;" ::: "memory");
-        sum = (s_sum[row] + s_sum[128 + row]) + (s_sum[256 + row] + s_sum[384 + row]);
-        if (part == 0 && i < p.T) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = live ? sum : 0.f;
-        delta = sum * f;
+        if (j == ahead - 1) {
+          float* s_sum = reinterpret_cast<float*>(smem + L::sums);
+          s_sum[part * kTcRows + row] = sum;
+          rows_meet();
+          sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < L::parts; ++w) sum += s_sum[w * kTcRows + row];
+          if (part == 0 && i < p.T) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = live ? sum : 0.f;
+          delta = sum * f;
+        }
+        if (lane == 0) mbar_arrive(ds_full);
+        continue;
       }
       bwd_ds<T>(x, y, sc, -lse, f, -delta);
       if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
@@ -299,7 +317,7 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (ok && 32 * part < D) {
       T* dst = static_cast<T*>(p.dq) + (((int64_t)b * p.T + i) * p.Hq + h) * D + 32 * part;
       uint32_t o[32];
-      if (ntiles > 0) { tmem_ld32(tmem + kDq + 32 * part + lane_off, o); tmem_wait_ld32(o); }
+      if (ntiles > 0) { tmem_ld32(tmem + L::tmem_dq + 32 * part + lane_off, o); tmem_wait_ld32(o); }
       if (i < p.T) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
@@ -315,7 +333,7 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
     }
   }
-  tc_finish(tmem, 512, warp, kBwdMma, abort_flag, p.error_flag);
+  tc_finish(tmem, L::tmem_cols, warp, L::mma, abort_flag, p.error_flag);
 }
 
 // ------------------------------------------------------------------------------------------------ dK, dV
@@ -700,6 +718,21 @@ static int64_t dkv_part_floats(const SwParams& p) {
   return ((int64_t)s.hsplit * p.B * p.Hk * s.part_tiles + (int64_t)s.hsplit * s.far_chunks * p.B * p.Hk * s.sink_tiles) * 2 * kTcRows * p.D;
 }
 
+template <typename T, int D, int kKeys>
+static int dq_launch(const SwParams& p, const TcParams& t, unsigned grid, int bf16, cudaStream_t st) {
+  typedef DqForm<D, kKeys> L;
+  CUtensorMap mq, mk, mv, mg;
+  int rc = tc_map(&mq, p.q, bf16, p.B, p.T, p.Hq, D, p.sq);
+  if (!rc) rc = tc_map(&mk, p.k, bf16, p.B, p.T, p.Hk, D, p.sk, kKeys);
+  if (!rc) rc = tc_map(&mv, p.v, bf16, p.B, p.T, p.Hk, D, p.sv, kKeys);
+  if (!rc) rc = tc_map(&mg, p.dout, bf16, p.B, p.T, p.Hq, D, p.sdo);
+  if (rc) return rc;
+  static unsigned long long seen = 0;
+  if (first_on_device(&seen)) cudaFuncSetAttribute(sw_dq_tc_kernel<T, D, kKeys>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::total);
+  sw_dq_tc_kernel<T, D, kKeys><<<grid, L::threads, L::total, st>>>(mq, mk, mv, mg, t, bf16);
+  return (int)cudaGetLastError();
+}
+
 template <typename T, int D, int kQ>
 static int dkv_launch(const SwParams& p, const TcParams& t, const DkvSplit& s, unsigned grid, int bf16, cudaStream_t st) {
   typedef DkvForm<D, kQ> L;
@@ -717,12 +750,6 @@ static int dkv_launch(const SwParams& p, const TcParams& t, const DkvSplit& s, u
 
 template <typename T, int D>
 static int tc_backward(const SwParams& p, float* parts, int bf16, int* error_flag, cudaStream_t st) {
-  CUtensorMap mq, mk, mv, mg;
-  int rc = tc_map(&mq, p.q, bf16, p.B, p.T, p.Hq, D, p.sq);
-  if (!rc) rc = tc_map(&mk, p.k, bf16, p.B, p.T, p.Hk, D, p.sk);
-  if (!rc) rc = tc_map(&mv, p.v, bf16, p.B, p.T, p.Hk, D, p.sv);
-  if (!rc) rc = tc_map(&mg, p.dout, bf16, p.B, p.T, p.Hq, D, p.sdo);
-  if (rc) return rc;
   TcParams t = tc_params(p, error_flag);
   t.items = p.B * p.Hq;
   DkvSplit s = dkv_split(p);
@@ -730,14 +757,12 @@ static int tc_backward(const SwParams& p, float* parts, int bf16, int* error_fla
   if (s.part_tiles && (!parts || (uintptr_t)parts % 16)) return -3;
   const int64_t gq = (int64_t)s.tiles * t.items, gk = ((int64_t)s.tiles + (int64_t)s.sink_tiles * s.far_chunks) * s.items;
   if (gq > 0x7fffffff || gk > 0x7fffffff) return -2;
-  static unsigned long long seen = 0;
-  if (first_on_device(&seen)) cudaFuncSetAttribute(sw_dq_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DqSmem<D>::total);
-  sw_dq_tc_kernel<T, D><<<(unsigned)gq, kBwdThreads, DqSmem<D>::total, st>>>(mq, mk, mv, mg, t, bf16);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return (int)e;
-  // Heads of 64: steps of 64 queries, two CTAs on an SM, where there are CTAs for both (whole backward pass, 12 heads: 64 x 128 85 us
-  // against 99, 16 x 512 102 and 116, 8 x 2048 303 and 335; 1 x 1024, 96 CTAs, 44 and 40).
-  const int code = D == 64 && gk > sm_count() ? dkv_launch<T, 64, 64>(p, t, s, (unsigned)gk, bf16, st) : dkv_launch<T, D, 128>(p, t, s, (unsigned)gk, bf16, st);
+  // Heads of 64: steps of 64 keys or queries and two CTAs on an SM, where there are CTAs for both.  Whole backward pass with such
+  // steps for dQ, dK and dV / for dK and dV alone / for neither: 64 x 128, 12 heads 77 / 87 / 99 us, 16 x 512 91 / 105 / 116,
+  // 8 x 2048 285 / 306 / 335, 4 x 4096, 16 over 4, window 128 188 / 226 / 234; 1 x 1024, 96 CTAs, dK and dV 44 against 40.
+  int code = D == 64 && gq > sm_count() ? dq_launch<T, 64, 64>(p, t, (unsigned)gq, bf16, st) : dq_launch<T, D, 128>(p, t, (unsigned)gq, bf16, st);
+  if (code) return code;
+  code = D == 64 && gk > sm_count() ? dkv_launch<T, 64, 64>(p, t, s, (unsigned)gk, bf16, st) : dkv_launch<T, D, 128>(p, t, s, (unsigned)gk, bf16, st);
   if (code || !s.part_tiles) return code;
   sw_dkv_join_kernel<T, D><<<dim3((unsigned)(s.part_tiles * p.B * p.Hk), 2 * kTcRows * D / 8 / 256), 256, 0, st>>>(t, s);
   return (int)cudaGetLastError();
