@@ -172,6 +172,7 @@ __device__ __forceinline__ void tc_accumulate(uint32_t tmem_d, uint32_t tmem_p, 
 }
 
 // The start of a CTA: the loading warp has set up the barriers and goes on at once, the others meet behind the TMEM allocation.
+// It may be at the end of its work before they have met, so the end meets on another barrier.
 template <int kThreads>
 __device__ __forceinline__ void tc_start_loader() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -197,7 +198,7 @@ __device__ __forceinline__ void tc_zero_rows(void* dst, int count, int row, int6
 
 __device__ __forceinline__ void tc_finish(uint32_t tmem_base, uint32_t cols, int warp, int alloc_warp, volatile int* abort_flag, int* error_flag) {
   tc_fence_before();
-  __syncthreads();
+  asm volatile("bar.sync 2, %0;" ::"r"((int)blockDim.x) : "memory");
   if (threadIdx.x == 0 && *abort_flag && error_flag) {
     *static_cast<volatile int*>(error_flag) = 1;         // host memory
     __threadfence_system();

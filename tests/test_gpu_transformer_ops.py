@@ -138,6 +138,22 @@ def test_attention_of_many_short_sequences(dtype, Hq, Hk, window, sinks):
         assert all(torch.equal(a, b) for a, b in zip(got, again)), fill
 
 
+@pytest.mark.parametrize('D', [64, 128])
+def test_attention_of_short_sequences_over_and_over(D):
+    """Short walks one after another, without a pause: the loading warp is done before the others have their TMEM."""
+    T = 512
+    valid = torch.randint(0, T + 1, (16,), device=dev(), dtype=torch.int32)
+    q, k, v, g = (randn(16, T, 12, D, dtype=torch.float16) for _ in range(4))
+    want = check_attention(q[:4], k[:4], v[:4], valid[:4], 0, 0, g[:4])
+    first = run_attention(q, k, v, valid, 0, 0, g)
+    assert all(torch.equal(a, b[:4]) for a, b in zip(want[:2], first[:2]))
+    same = torch.ones((), dtype=torch.bool, device=dev())
+    for _ in range(300):
+        for a, b in zip(first, run_attention(q, k, v, valid, 0, 0, g)):
+            same &= (a == b).all()
+    assert bool(same)
+
+
 @pytest.mark.parametrize('dtype', HALF)
 @pytest.mark.parametrize('Hq,Hk,window,sinks', [(2, 1, 0, 0), (1, 1, 2049, 3), (3, 3, 2048, 130)])
 def test_attention_long_walks_of_small_heads(dtype, Hq, Hk, window, sinks):
