@@ -198,7 +198,8 @@ __device__ __forceinline__ void tc_zero_rows(void* dst, int count, int row, int6
 
 __device__ __forceinline__ void tc_finish(uint32_t tmem_base, uint32_t cols, int warp, int alloc_warp, volatile int* abort_flag, int* error_flag) {
   tc_fence_before();
-  asm volatile("bar.sync 2, %0;" ::"r"((int)blockDim.x) : "memory");
+  __syncwarp();
+  asm volatile("barrier.sync 2, %0;" ::"r"((int)blockDim.x) : "memory");
   if (threadIdx.x == 0 && *abort_flag && error_flag) {
     *static_cast<volatile int*>(error_flag) = 1;         // host memory
     __threadfence_system();

@@ -70,9 +70,9 @@ template <int D, int kKeys> struct DqForm {
   static constexpr uint32_t tmem_dp = 2 * kKeys, tmem_dq = 3 * kKeys, tmem_cols = kKeys == 64 ? 256 : 512;
   static constexpr uint32_t tile = (D / 64) * kTcHalf, ktile = tile * kKeys / 128;
   static constexpr int kst = 3, vst = 2;
-  // delta: [128], then the warps' largest |dO|; sums: [parts][128], with steps of 128 keys in a stage that two steps leave unused
+  // delta: [128], then the warps' largest |dO|; sums: [parts][128] pairs, with steps of 128 keys in a stage that two steps leave unused
   static constexpr uint32_t q = 0, g = tile, k = 2 * tile, v = k + kst * ktile, delta = v + vst * ktile,
-                            sums = kKeys == 64 ? delta + 1024 : k + 2 * ktile, bars = kKeys == 64 ? sums + parts * 512 : delta + 1024;
+                            sums = kKeys == 64 ? delta + 1024 : k + 2 * ktile, bars = kKeys == 64 ? sums + parts * 1024 : delta + 1024;
   static constexpr uint32_t total = bars + 256;
 };
 
@@ -85,8 +85,9 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   float* s_delta = reinterpret_cast<float*>(smem + L::delta);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
   uint64_t *qg_full = bars, *k_full = bars + 1, *k_empty = bars + 4, *v_full = bars + 7, *v_empty = bars + 9, *sd_full = bars + 11,
-           *dp_empty = bars + 12, *ds_full = bars + 13, *done = bars + 14, *patch = bars + 15, *drain = bars + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+           *dp_empty = bars + 12, *ds_full = bars + 13, *done = bars + 15, *patch = bars + 16, *drain = bars + 17;
+  // ds_full: two, in turn - a warp may be done with its dS of a step before another is with the step before
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (smem_u32(smem) & 1023u) {                                    // swizzled tiles lie on 1024-byte boundaries
@@ -122,7 +123,7 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       mbar_init(qg_full, 1);
       for (int s = 0; s < L::kst; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
       for (int s = 0; s < L::vst; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
-      mbar_init(sd_full, 1); mbar_init(dp_empty, L::rows_warps); mbar_init(ds_full, L::rows_warps); mbar_init(done, 1); mbar_init(patch, 1); mbar_init(drain, 1);
+      mbar_init(sd_full, 1); mbar_init(dp_empty, L::rows_warps); mbar_init(&ds_full[0], L::rows_warps); mbar_init(&ds_full[1], L::rows_warps); mbar_init(done, 1); mbar_init(patch, 1); mbar_init(drain, 1);
       *abort_flag = 0;
     }
     tc_start_loader<L::threads>();
@@ -200,7 +201,7 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           if (ok) dprobs(j + 1);
           if (!ok) break;
         }
-        ok = mbar_wait_warp(ds_full, (uint32_t)j & 1u);
+        ok = mbar_wait_warp(&ds_full[j & 1], (uint32_t)(j >> 1) & 1u);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -244,7 +245,10 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (lane == 0) s_delta[128 + warp] = big;
     }
     const float lse = live ? p.lse[((int64_t)b * p.Hq + h) * p.T + i] : INFINITY;
-    auto rows_meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * L::rows_warps) : "memory"); };
+    auto rows_meet = [] {                                         // the lanes of a warp may come one by one
+      __syncwarp();
+      asm volatile("barrier.sync 1, %0;" ::"n"(32 * L::rows_warps) : "memory");
+    };
     rows_meet();
     float delta = s_delta[row];
     float f = 1.f;
@@ -259,7 +263,7 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const float out_scale = p.scale / f;
     const float sc = p.scale * kSwLog2e;
     bool ok = true;
-    float sum = 0.f;
+    float sum = 0.f, total = 0.f;
     for (int j = 0; j < nit; ++j) {
       const int kt = key_tile(j);
       ok = mbar_wait_warp(sd_full, (uint32_t)j & 1u);
@@ -283,18 +287,27 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const uint32_t seen = whole ? 0xffffffffu : tc_seen(i - base, i - p.window - base, p.sinks - 1 - base);
       if (j < ahead) {
 #pragma unroll
-        for (int c = 0; c < 32; ++c) if (seen & 1u << c) sum += ex2(fmaf(__uint_as_float(x[c]), sc, -lse)) * __uint_as_float(y[c]);
-        if (j == ahead - 1) {
-          float* s_sum = reinterpret_cast<float*>(smem + L::sums);
-          s_sum[part * kTcRows + row] = sum;
-          rows_meet();
-          sum = 0.f;
-#pragma unroll
-          for (int w = 0; w < L::parts; ++w) sum += s_sum[w * kTcRows + row];
-          if (part == 0 && i < p.T) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = live ? sum : 0.f;
-          delta = sum * f;
+        for (int c = 0; c < 32; ++c) {
+          const bool on = seen >> c & 1u;
+          const float pr = on ? ex2(fmaf(__uint_as_float(x[c]), sc, -lse)) : 0.f;
+          sum = fmaf(pr, on ? __uint_as_float(y[c]) : 0.f, sum);
+          total += pr;
         }
-        if (lane == 0) mbar_arrive(ds_full);
+        if (j == ahead - 1) {
+          float2* s_sum = reinterpret_cast<float2*>(smem + L::sums);
+          s_sum[part * kTcRows + row] = make_float2(sum, total);
+          rows_meet();
+          sum = total = 0.f;
+#pragma unroll
+          for (int w = 0; w < L::parts; ++w) { sum += s_sum[w * kTcRows + row].x; total += s_sum[w * kTcRows + row].y; }
+          // over the sum of the same P, which is 1 but for the rounding of the log-sum-exp: a row with one key gets that key's dP
+          delta = live && total != 0.f ? __fdiv_rn(sum, total) : 0.f;
+          if (part == 0 && i < p.T) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = delta;
+          delta *= f;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ds_full[j & 1]);
+        __syncwarp();
         continue;
       }
       bwd_ds<T>(x, y, sc, -lse, f, -delta);
@@ -309,7 +322,7 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
+      if (lane == 0) mbar_arrive(&ds_full[j & 1]);
     }
     if (ok && ntiles > 0) ok = mbar_wait_warp(done, 0);
     if (!ok) *abort_flag = 1;
