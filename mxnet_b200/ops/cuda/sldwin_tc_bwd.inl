@@ -3,15 +3,15 @@
 // Two kernels, each the owner of what it accumulates, so that no result depends on the order of anything: dQ by query tiles
 // (S, dP and dS K: three products per pair of tiles) and dK, dV by key tiles (S^T, dP^T, P^T dO, dS^T Q: four).  The scores
 // are formed twice; sharing them would need sums of dQ across CTAs in memory.  In both, four warpgroups share each tile of
-// scores (32 columns each: a thread holds its scores and their gradients in registers), so that the exponentials of a tile take
-// less time than its products.
+// scores (32 columns each: a thread holds its scores and their gradients in registers; two with steps of 64), so that the
+// exponentials of a tile take less time than its products.
 //
 // What bounds it: a step of the dK, dV walk takes 2700 cycles, of which the four products need 2048 at the tensor cores' full rate
 // (512 for 128 x 128 x 128) and the chain scores, probabilities, next scores the rest; then the start and the end of each CTA, with
-// one CTA on an SM (shared memory and TMEM are full).
+// one CTA on an SM for heads of 128 (shared memory and TMEM are full).
 // 2 x 4096, 16 heads over 4 of 128, window 1024, 4 sinks, bf16: dQ 134 us (tensor pipe active 42 %), dK and dV 147 us (61 %).
-// Heads of 64 fit twice on an SM in steps of 64, so that one CTA's start and end run under the other's walk: 16 x 512 padded,
-// 12 heads, fp16: 25 and 32 us instead of 35 and 41.
+// Heads of 64 fit twice on an SM in steps of 64, so that one CTA's start and end run under the other's walk (figures at the
+// choice of the step, tc_backward).
 //
 // Range in fp16: probabilities enter the dV product 2^14 times their value (at most 2^14, digits kept down to 2^-28), and dS is
 // formed from dO scaled by the power of two that brings the largest dO of the CTA's tiles into [8, 16): neither small
