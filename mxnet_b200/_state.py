@@ -17,6 +17,7 @@ class _State(threading.local):
         self.np_default_dtype = False
         self.opt_constraints = 0      # HybridBlock.OptConstraint flags (bit 0: AMP casts off)
         self.tracer = None          # active deferred-compute tracer (symbol/_trace.py) or None
+        self.writes = None          # list that collects the tensors operators update in place (gluon/cached_op.py) or None
         self.bulk_size = 0
         self.profiler_scope = '<unk>:'
         self.name_prefix = ''

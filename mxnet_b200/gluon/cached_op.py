@@ -10,7 +10,9 @@ buffers when ``static_alloc`` and ``static_shape`` are set on a GPU: the first c
 signature (training flag, input shapes/dtypes, parameter-storage version) runs eagerly, the second
 captures, later calls replay.  The pair is exposed to autograd as a single node (the counterpart of
 the ``_CachedOp`` / ``_backward_CachedOp`` tape node) whose inputs include every parameter, so
-gradients still land in the parameters' own buffers.  Anything that cannot be captured (host
+gradients still land in the parameters' own buffers.  Arguments are copied into static buffers, except those that the block
+updates in place (key/value caches, optimizer states): the graph reads and writes them where the caller holds them, and their
+place is part of the signature.  Anything that cannot be captured (host
 synchronisation inside ``forward``, data-dependent shapes) makes the block fall back to eager
 execution permanently, the analogue of the reference's split around incompatible operators.
 """
@@ -24,13 +26,52 @@ from .. import _state, autograd, env
 from ..ndarray.ndarray import NDArray
 
 _log = logging.getLogger('mxnet_b200.cached_op')
+_MAX_PLACED = 4          # graphs of one block that are bound to the place of an argument
+
+
+class _Uncaptured(Exception):
+    """The capture met writes to arguments (``args``: their indexes) that no eager call had shown."""
+
+
+class _Watch(object):
+    """Finds the arrays whose elements a block updates: the version counters of their tensors show what the tensor library wrote,
+    the operators' own lists (``OpDef.mutate``, ``out=``) what kernels did."""
+
+    def __init__(self, tensors):
+        self.tensors = tensors
+
+    def __enter__(self):
+        self.versions = [_version(t) for t in self.tensors]
+        self.outer, _state.state.writes = _state.state.writes, []
+        return self
+
+    def __exit__(self, *exc):
+        self.noted, _state.state.writes = _state.state.writes, self.outer
+        if self.outer is not None:
+            self.outer.extend(self.noted)
+
+    def written(self):
+        """Indexes of the arrays that were written to, and of all that share their memory."""
+        places = {_storage(t) for t in self.noted}
+        places.update(_storage(t) for t, v in zip(self.tensors, self.versions) if _version(t) != v)
+        places.discard(0)
+        return {i for i, t in enumerate(self.tensors) if _storage(t) in places}
+
+
+def _version(t):
+    return 0 if t.is_inference() else t._version
+
+
+def _storage(t):
+    return t.untyped_storage().data_ptr() if t.layout == torch.strided else 0
 
 
 class _Graphed(object):
     """Forward/backward graph pair for one call signature."""
 
-    def __init__(self, block, args, training, recording, forward=None):
+    def __init__(self, block, args, training, recording, forward=None, placed=frozenset()):
         self.block = block
+        self.placed = placed                      # arrays that the graph updates: used where they are
         self.forward = forward if forward is not None else block.forward    # a pass-rewritten graph of the block, or its code
         self.training, self.recording = training, recording
         from .block import _flatten
@@ -51,8 +92,8 @@ class _Graphed(object):
                 self.param_arrays.append(arr)
                 self.param_tensors.append(arr._data)
         self.static_in = []
-        for a in arrays:
-            t = a._data.detach().clone()
+        for i, a in enumerate(arrays):
+            t = a._data.detach() if i in placed else a._data.detach().clone()
             if recording and a._data.requires_grad:
                 t.requires_grad_(True)
             self.static_in.append(t)
@@ -83,19 +124,29 @@ class _Graphed(object):
         finally:
             if self._gc_was_enabled:
                 gc.enable()
+        # nothing here keeps the caller's arrays: a call with others of the same signature finds them in the same place
+        for i in placed:
+            self.static_in[i] = None
+        for slot in self.arg_slots:
+            self.flat_template[slot] = None
 
     def _capture(self, stream, n0, recording, dev):
         from .block import _flatten
         _kernels = self._kernels
         with torch.cuda.stream(stream):
             with torch.cuda.graph(self.fwd, pool=self.pool, stream=stream):
-                outs = self._run_forward()
+                with _Watch(list(self.static_in)) as watch:
+                    outs = self._run_forward()
+        written = watch.written()
+        if written - self.placed or (written and recording):
+            raise _Uncaptured(*sorted(written))
         self.fwd_launches = _kernels.launches() - n0     # in-tree kernels recorded in the forward graph
         self.bwd_launches = 0
         flat_out, self.out_fmt = _flatten(outs, 'output')
         self.out_is_array = [isinstance(o, NDArray) for o in flat_out]
-        self.flat_out_template = list(flat_out)
+        self.flat_out_template = [None if isinstance(o, NDArray) else o for o in flat_out]
         self.static_out = [o._data for o in flat_out if isinstance(o, NDArray)]
+        self.out_place = [self._find_place(o) for o in self.static_out]
         self.bwd = None
         if recording and self.grad_inputs and any(o.requires_grad for o in self.static_out):
             self.out_needs_grad = [o.requires_grad for o in self.static_out]
@@ -131,7 +182,26 @@ class _Graphed(object):
             self.static_gin = list(gin)
             self.bwd_launches = _kernels.launches() - n1
         torch.cuda.current_stream(dev).wait_stream(stream)
-        self.static_out_detached = [o.detach() for o in self.static_out]
+        self.static_out = [o if at is None else None for o, at in zip(self.static_out, self.out_place)]
+        self.static_out_detached = [None if o is None else o.detach() for o in self.static_out]
+
+    def _find_place(self, out):
+        """An output that lies in an updated argument: that argument's index, and the output's place in it."""
+        for i in self.placed:
+            t = self.static_in[i]
+            if _storage(out) == _storage(t):
+                return i, out.storage_offset() - t.storage_offset(), out.size(), out.stride()
+        return None
+
+    def _output(self, k, tensors):
+        at = self.out_place[k]
+        if at is None:
+            return self.static_out_detached[k]
+        i, offset, size, stride = at
+        t = tensors[i]
+        if offset == 0 and t.size() == size and t.stride() == stride:
+            return t
+        return t.as_strided(size, stride, t.storage_offset() + offset)
 
     def _run_forward(self):
         flat = list(self.flat_template)
@@ -213,10 +283,14 @@ class _Graphed(object):
         else:
             with torch.no_grad():
                 for dst, src in zip(self.static_in, tensors):
-                    dst.copy_(src)
+                    if dst is not None:
+                        dst.copy_(src)
                 self.fwd.replay()
                 self._kernels.count_launch(self.fwd_launches)
-                outs = tuple(self.static_out_detached)
+                for i in self.placed:
+                    if not tensors[i].is_inference():
+                        torch.autograd.graph.increment_version(tensors[i])
+                outs = tuple(self._output(k, tensors) for k in range(len(self.static_out)))
         flat_out, k = list(self.flat_out_template), 0
         for i, is_arr in enumerate(self.out_is_array):
             if is_arr:
@@ -234,6 +308,7 @@ class CachedOp(object):
         self.flags = dict(flags or {})
         self._seen = {}
         self._graphs = {}
+        self._written = {}       # signature -> arrays that the block updates (None: it gives the caller's array another tensor)
         self._disabled = False
 
     def _static(self):
@@ -258,6 +333,25 @@ class CachedOp(object):
                 sig.append(repr(a))
         return tuple(sig)
 
+    @staticmethod
+    def _at(sig, tensors, written):
+        """``sig`` with the places of the arrays that the block updates."""
+        return sig + tuple((i, tensors[i].data_ptr(), tensors[i].stride()) for i in sorted(written)) if written else sig
+
+    def _watched(self, eager, args, arrays, sig):
+        """An eager call that learns which of its arrays the block updates."""
+        tensors = [a._data for a in arrays]
+        with _Watch(tensors) as watch:
+            out = eager(*args)
+        if any(a._data is not t for a, t in zip(arrays, tensors)):
+            self._written[sig] = None
+        else:
+            written = watch.written()
+            known = self._written.get(sig, frozenset())
+            if written and known is not None:
+                self._written[sig] = known | written
+        return out
+
     def __call__(self, *args, graph_forward=None, graph_tag=None):
         """``graph_forward``: a callable that evaluates the block's traced graph after a graph pass (layout management);
         it replaces ``block.forward`` both in the eager runs and inside the captured graphs.  ``graph_tag`` names the pass
@@ -269,6 +363,10 @@ class CachedOp(object):
         if not self._use_graphs(arrays):
             return eager(*args)
         sig = self._signature(flat) + ((graph_tag,) if graph_forward is not None else ())
+        plain, written = sig, self._written.get(sig, frozenset())
+        if written is None or (written and _state.state.recording):
+            return eager(*args)
+        sig = self._at(plain, [a._data for a in arrays], written)
         g = self._graphs.get(sig)
         if g is not None:
             return g(args)
@@ -277,11 +375,19 @@ class CachedOp(object):
         # so that a workload whose shapes keep changing stays eager instead of collecting graphs.
         seen = self._seen.get(sig, 0)
         need = 1 if self._static() else 3
-        if seen < need or (not self._static() and len(self._graphs) >= 4):
-            self._seen[sig] = seen + 1   # warm-up runs with this signature stay eager
-            return eager(*args)
+        if seen < need or (not self._static() and len(self._graphs) >= 4) or \
+                (written and sum(1 for g in self._graphs.values() if g.placed) >= _MAX_PLACED):
+            place = [a._data for a in arrays]
+            out = self._watched(eager, args, arrays, plain)
+            now = self._written.get(plain, frozenset())
+            if now is not None:
+                self._seen[self._at(plain, place, now)] = seen + 1   # warm-up runs with this signature stay eager
+            return out
         try:
-            g = _Graphed(self.block, args, _state.state.training, _state.state.recording, forward=graph_forward)
+            g = _Graphed(self.block, args, _state.state.training, _state.state.recording, forward=graph_forward, placed=written)
+        except _Uncaptured as e:
+            self._written[plain] = written | set(e.args)
+            return eager(*args)
         except Exception as e:  # pylint: disable=broad-except
             self._disabled = True
             _log.warning('CUDA graph capture failed (%s); block %s runs eagerly', e, type(self.block).__name__,

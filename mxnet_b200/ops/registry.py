@@ -110,6 +110,15 @@ def _wrap(t, kind, ctx=None):
     return _array_classes[kind]._from_tensor(t, ctx)
 
 
+def note_writes(op, tensors):
+    """Adds the inputs that a call of ``op`` updates to the list that collects them (kernels write them without the tensor
+    library's knowledge): its ``mutate`` inputs, in training its auxiliary states too."""
+    st = _state.state
+    names = op.mutate + op.aux if st.training else op.mutate
+    if names:
+        st.writes.extend(t for name, t in zip(op.inputs, tensors) if name in names and isinstance(t, torch.Tensor))
+
+
 def invoke(op, args, attrs, out=None, kind=None):
     """Run operator ``op`` (OpDef or name) on array wrappers ``args`` with attribute dict ``attrs``.
 
@@ -169,6 +178,10 @@ def invoke(op, args, attrs, out=None, kind=None):
         if pctx is not None:
             pctx.__exit__(None, None, None)
     multi = isinstance(res, (tuple, list))
+    if st.writes is not None:
+        note_writes(op, [a._data if isinstance(a, base) else a for a in args])
+        if out is not None:
+            st.writes.extend(o._data for o in (out if isinstance(out, (list, tuple)) else [out]))
     if out is not None:
         outs = out if isinstance(out, (list, tuple)) else [out]
         ress = res if multi else [res]

@@ -147,6 +147,8 @@ def _apply_node(node, ins):
     if hook is not None and not _state.state.opt_constraints & 1:
         ins = hook(node.op.name, ins)
     res = node.op.fn(*ins, **node.attrs)
+    if _state.state.writes is not None:
+        _reg.note_writes(node.op, ins)
     return tuple(res) if isinstance(res, (tuple, list)) else (res,)
 
 
