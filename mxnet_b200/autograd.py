@@ -12,6 +12,7 @@ backward accumulates into them; ``'add'`` never clears.
 """
 from __future__ import annotations
 
+import threading
 import weakref
 
 import torch
@@ -197,14 +198,31 @@ class _Here(object):
 _HERE = _Here()
 
 
+_worked = set()                     # devices whose passes ran on the tensor library's workers
+_here = threading.local()           # .devices: those whose passes this thread ran itself
+
+
 def _calling_thread(tensors):
     """Scope of a gradient pass whose heads lie on one device: it runs on the thread that asked for it.  The tensor library's
     worker of that device would do the same work in the same order after two thread switches (30 to 200 us, as the machine
     schedules them); heads on several devices keep their workers, which run side by side."""
     first = tensors[0].device if tensors else None
     if first is not None and first.type == 'cuda' and all(t.device == first for t in tensors[1:]):
+        try:
+            _here.devices.add(first.index)
+        except AttributeError:
+            _here.devices = {first.index}
         return torch.autograd.set_multithreading_enabled(False)
+    _worked.update(t.device.index for t in tensors if t.device.type == 'cuda')
     return _HERE
+
+
+def captured_pass(device):
+    """Scope of a gradient pass of one device that a CUDA graph captures: it runs on the thread that ran the passes before it.  What
+    the libraries set up for each thread at its first GPU work (handles, workspaces) is forbidden inside a capture."""
+    if device.index in _worked and device.index not in getattr(_here, 'devices', ()):
+        return _HERE
+    return torch.autograd.set_multithreading_enabled(False)
 
 
 _run_backward = torch.autograd.Variable._execution_engine.run_backward

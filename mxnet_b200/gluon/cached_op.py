@@ -155,8 +155,9 @@ class _Graphed(object):
             n1 = _kernels.launches()
             with torch.cuda.stream(stream):
                 with torch.cuda.graph(self.bwd, pool=self.pool, stream=stream):
-                    gin = torch.autograd.grad([o for o in self.static_out if o.requires_grad], self.grad_inputs,
-                                              [g for g in self.static_gout if g is not None], allow_unused=True)
+                    with autograd.captured_pass(dev):
+                        gin = torch.autograd.grad([o for o in self.static_out if o.requires_grad], self.grad_inputs,
+                                                  [g for g in self.static_gout if g is not None], allow_unused=True)
                     # Parameter gradients are added to the parameters' gradient buffers by nodes of this graph, instead
                     # of being handed to the autograd engine, which would launch one accumulation kernel per parameter
                     # after every replay.  The buffers are kept alive here; a parameter whose buffer is replaced later

@@ -1,0 +1,56 @@
+"""The thread that a gradient pass runs on: the same for the eager passes of a device and for the one that is captured."""
+import threading
+from types import SimpleNamespace
+
+import torch
+
+from mxnet_b200 import autograd
+
+
+def on(*indexes):
+    return [SimpleNamespace(device=torch.device('cuda', i)) for i in indexes]
+
+
+def stays(scope):
+    """Whether passes inside the scope run on the calling thread."""
+    with scope:
+        return not torch._C._is_multithreading_enabled()
+
+
+def fresh(monkeypatch):
+    monkeypatch.setattr(autograd, '_worked', set())
+    monkeypatch.setattr(autograd, '_here', threading.local())
+
+
+def test_a_captured_pass_runs_where_the_eager_ones_ran(monkeypatch):
+    fresh(monkeypatch)
+    first, second = torch.device('cuda', 0), torch.device('cuda', 1)
+    assert stays(autograd.captured_pass(first))                     # no pass so far: the forward pass ran here
+    assert stays(autograd._calling_thread(on(0, 0))) and stays(autograd.captured_pass(first))
+    assert not stays(autograd._calling_thread(on(0, 1)))
+    assert stays(autograd.captured_pass(first)) and not stays(autograd.captured_pass(second))
+    seen = []
+    other = threading.Thread(target=lambda: seen.extend([stays(autograd.captured_pass(first)), stays(autograd.captured_pass(second))]))
+    other.start()
+    other.join()
+    assert seen == [False, False]                                   # that thread ran none itself
+    assert torch._C._is_multithreading_enabled()
+
+
+def test_the_setting_is_put_back_after_a_pass_that_raises():
+    class Fails(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            raise ValueError('no gradient today')
+    x = torch.ones(2, requires_grad=True)
+    for scope in (lambda: autograd.captured_pass(torch.device('cuda', 0)), lambda: autograd._calling_thread(on(0))):
+        try:
+            with scope():
+                Fails.apply(x).sum().backward()
+        except ValueError:
+            pass
+        assert torch._C._is_multithreading_enabled()
