@@ -301,6 +301,15 @@ class _Graphed(object):
         return res
 
 
+def _after_failed_capture(device):
+    """A capture that failed leaves the device's random generator in its capturing state, where it refuses to draw outside of one.
+    One that succeeds puts it back."""
+    stream = torch.cuda.Stream(device=device)
+    with torch.cuda.stream(stream):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+            torch.zeros(1, device=device)
+
+
 class CachedOp(object):
     """Per-block cache of executors keyed by call signature."""
 
@@ -391,6 +400,7 @@ class CachedOp(object):
             return eager(*args)
         except Exception as e:  # pylint: disable=broad-except
             self._disabled = True
+            _after_failed_capture(arrays[0]._data.device)
             _log.warning('CUDA graph capture failed (%s); block %s runs eagerly', e, type(self.block).__name__,
                          exc_info=bool(env.get('MXNET_CUDA_GRAPHS_VERBOSE')))
             return eager(*args)

@@ -55,3 +55,74 @@ def test_a_training_block_is_captured(how):
     run = subprocess.run([sys.executable, '-c', TRAIN, *how], cwd=root, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr[-2000:]
     assert 'graphs [(True, True)] False' in run.stdout and 'capture failed' not in run.stderr, run.stdout + run.stderr[-2000:]
+
+
+FAIL = """
+import sys
+import torch
+import mxnet_b200 as mx
+from mxnet_b200 import autograd, nd
+from mxnet_b200.gluon import HybridBlock, nn
+
+
+class Sync(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return x * 1
+
+    @staticmethod
+    def backward(ctx, g):
+        g.sum().item()
+        return g
+
+
+class Reads(HybridBlock):
+    # reads its result on the host after it has drawn, in the pass that it is told
+    def __init__(self, where):
+        super().__init__()
+        self.dense, self.where = nn.Dense(64, in_units=64), where
+
+    def forward(self, x):
+        y = nd.Dropout(self.dense(x), p=0.5)
+        if self.where == 'forward':
+            y.asnumpy()
+        elif self.where == 'backward':
+            y = nd.NDArray(Sync.apply(y._data))
+        return y
+
+
+def run(where, calls=6):
+    ctx = mx.gpu(0)
+    block = Reads(where)
+    block.initialize(ctx=ctx)
+    block.hybridize(static_alloc=True, static_shape=True)
+    x = nd.ones((64, 64), ctx=ctx)
+    shares = []
+    for _ in range(calls):
+        with autograd.record():
+            y = block(x)
+        y.backward()
+        assert block.dense.weight.grad(ctx)._data.isfinite().all()
+        shares.append(float((y._data == 0).float().mean()))
+    return block._cached_op, shares
+
+
+op, shares = run(sys.argv[1])
+assert op._disabled and not op._graphs
+# 4096 draws of 1/2: a share of zeros off by 0.05 is 6.4 standard deviations
+assert all(abs(s - 0.5) < 0.05 for s in shares) and len(set(shares)) > 1, shares
+mx.random.seed(3, ctx=mx.gpu(0))
+a = nd.random.uniform(shape=(8,), ctx=mx.gpu(0)).asnumpy()
+op, shares = run('nowhere')                 # another block is captured, its draws differ from call to call
+assert not op._disabled and len(op._graphs) == 1 and len(set(shares)) > 1, shares
+mx.random.seed(3, ctx=mx.gpu(0))
+assert (nd.random.uniform(shape=(8,), ctx=mx.gpu(0)).asnumpy() == a).all()
+print('carried on')
+"""
+
+
+@pytest.mark.parametrize('where', ['forward', 'backward'])
+def test_a_block_that_cannot_be_captured_runs_eagerly(where):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, '-c', FAIL, where], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and 'carried on' in run.stdout and 'capture failed' in run.stderr, run.stdout + run.stderr[-3000:]
