@@ -276,7 +276,7 @@ MXB_EXPORT int mxb_sldwin_forward(int dtype, const void* q, const void* k, const
   return -1;
 }
 
-// dq: [B, T, Hq, D], dk and dv: [B, T, Hk, D], contiguous; delta: [B, Hq, T + ceil(T / 128)] floats of workspace; parts:
+// dq: [B, T, Hq, D], dk and dv: [B, T, Hk, D], contiguous; delta: B (Hq (T + tiles) + Hk tiles) floats of workspace, tiles = ceil(T / 128); parts:
 // mxb_sldwin_backward_parts floats of workspace (may be null when that is 0).
 MXB_EXPORT int mxb_sldwin_backward(int dtype, const void* q, const void* k, const void* v, const int* valid, const void* o,
                                    const void* dout, const float* lse, float* delta, float* parts, void* dq, void* dk, void* dv,

@@ -77,8 +77,10 @@ class _SldwinAttention(torch.autograd.Function):
         (q0, q1, q2, _), (k0, k1, k2, _), (v0, v1, v2, _), (g0, g1, g2, _) = q.stride(), k.stride(), v.stride(), dout.stride()
         form = _I19(B, T, Hq, kshape[2], D, window, sinks, q0, q1, q2, k0, k1, k2, v0, v1, v2, g0, g1, g2)
         L, code = lib(), DT[dtype]
-        # workspace: rowsum(dO * O) and the largest |dO| of each query tile, then key gradients that several blocks sum up
-        rows = (B * Hq * (T + (T + 127) // 128) + 3) // 4 * 4
+        # workspace: rowsum(dO * O), the largest |dO| of each query tile and |V| of each key tile, then key gradients that several
+        # blocks sum up
+        tiles = (T + 127) // 128
+        rows = (B * (Hq * (T + tiles) + kshape[2] * tiles) + 3) // 4 * 4
         parts = L.mxb_sldwin_backward_parts(code, form)
         work = torch.empty(rows + parts, dtype=torch.float32, device=dev)
         at = work.data_ptr()
@@ -86,7 +88,7 @@ class _SldwinAttention(torch.autograd.Function):
             check(L.mxb_sldwin_backward(code, q.data_ptr(), k.data_ptr(), v.data_ptr(), address(valid), out.data_ptr(), dout.data_ptr(),
                                         lse.data_ptr(), at, at + 4 * rows if parts else 0, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                         form, scale, _error_word(), raw_stream(q)), 'sldwin_attention backward')
-        count_launch(3 if parts else 2)
+        count_launch(2 + (parts > 0) + (dtype is torch.float16 and D in (64, 128) and 0 < scale < 1e30))
         return dq, dk, dv, None, None, None, None
 
 

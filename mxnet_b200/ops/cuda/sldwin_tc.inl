@@ -93,6 +93,7 @@ struct TcParams {
   float* lse;                            // [B, Hq, T]
   float* delta;                          // [B, Hq, T], behind it gmax
   float* gmax;                           // [B, Hq, tiles]: largest |dO| of each query tile (fp16)
+  float* vmax;                           // [B, Hk, tiles]: largest |V| of each key tile (fp16)
   int B, T, Hq, Hk, window, sinks;
   int qpair;                             // 1: the two tiles of a CTA are two query heads, 0: two consecutive query tiles
   int items;                             // (sample, head or head pair) combinations
@@ -555,6 +556,7 @@ static TcParams tc_params(const SwParams& p, int* error_flag) {
   TcParams t{};
   t.valid = p.valid; t.o = p.o; t.dout = p.dout; t.sdo = p.sdo; t.out = p.out; t.dq = p.dq; t.dk = p.dk; t.dv = p.dv;
   t.lse = p.lse; t.delta = p.delta; t.gmax = p.delta + (int64_t)p.B * p.Hq * p.T;
+  t.vmax = t.gmax + (int64_t)p.B * p.Hq * ((p.T + kTcRows - 1) / kTcRows);
   t.B = p.B; t.T = p.T; t.Hq = p.Hq; t.Hk = p.Hk; t.window = p.window; t.sinks = p.sinks; t.scale = p.scale; t.error_flag = error_flag;
   return t;
 }

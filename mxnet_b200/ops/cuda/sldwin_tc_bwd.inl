@@ -14,13 +14,43 @@
 // choice of the step, tc_backward).
 //
 // Range in fp16: probabilities enter the dV product 2^14 times their value (at most 2^14, digits kept down to 2^-28), and dS is
-// formed from dO scaled by the power of two that brings the largest dO of the CTA's tiles into [8, 16): neither small
-// gradients nor a loss scale push it out of the type's range.  Both factors leave with the fp32 sums.  bf16 needs neither.
+// formed from dO scaled by a power of two f.  f brings the largest dO of the CTA's tiles into [8, 16), so that neither small
+// gradients nor a loss scale push dS out of the type's range, and gives way where the values V are large: with M the largest
+// |f dP| <= D * 16 * max |V|, a row's delta is a mean of its dP, so |f dS| = P |f dP - f delta| <= 2 P (1 - P) M <= M / 2, and f is
+// halved until M < 2^16 (dS up to 2^15, half the type's range).  Values up to 32 (heads of 128) or 64 leave f as it is; larger ones
+// take as many of the lowest digits of dS as they add at its top.  Both factors leave with the fp32 sums.  bf16 needs neither.
 template <typename T> struct BwdRange { static constexpr bool scaled = false; static constexpr float shift = 0.f, unshift = 1.f; };
 template <> struct BwdRange<__half> { static constexpr bool scaled = true; static constexpr float shift = 14.f, unshift = 1.f / 16384.f; };
-__device__ __forceinline__ float bwd_factor(float amax) {          // 2^(3 - e) for amax in [2^e, 2^(e + 1))
-  const int e = (int)((__float_as_uint(amax) >> 23) & 255u) - 127;
-  return e < -30 || e > 16 ? 1.f : __uint_as_float((uint32_t)(127 + 3 - e) << 23);
+__device__ __forceinline__ int float_exponent(float a) { return (int)((__float_as_uint(a) >> 23) & 255u) - 127; }      // a in [2^e, 2^(e + 1))
+template <int D>
+__device__ __forceinline__ float bwd_factor(float gmax, float vmax) {
+  const int e = float_exponent(gmax), over = min(float_exponent(vmax), 15) - (D == 128 ? 4 : 5);
+  return e < -30 || e > 16 ? 1.f : __uint_as_float((uint32_t)(127 + 3 - e - max(over, 0)) << 23);
+}
+
+// Largest |V| of each tile of 128 keys that are there (fp16 alone): blockIdx.x = (sample, key head, tile).  A pass over V ahead of
+// the two kernels; a bound from row sums in the forward pass would cost every call without gradients too.
+template <typename T, int D>
+__global__ void __launch_bounds__(256)
+sw_vmax_kernel(const TcParams p, const T* v, SwStride sv, int tiles) {
+  __shared__ float red[8];
+  const int kt = blockIdx.x % tiles, bh = blockIdx.x / tiles, b = bh / p.Hk, hk = bh % p.Hk;
+  const int rows = min(kTcRows, tc_valid(p, b) - kt * kTcRows);
+  const T* at = v + b * sv.b + (int64_t)kt * kTcRows * sv.t + hk * sv.h;
+  float big = 0.f;
+  for (int e = threadIdx.x; e < rows * (D / 8); e += 256) {
+    const Vec16<T> x = ld16(at + (int64_t)(e / (D / 8)) * sv.t + e % (D / 8) * 8);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) big = fmaxf(big, fabsf(Cvt<T>::to_f(x.v[c])));
+  }
+  big = warp_max(big);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = big;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) big = fmaxf(big, red[w]);
+    p.vmax[blockIdx.x] = big;
+  }
 }
 
 // Of every 8 pairs of exponentials kBwdPoly go through the polynomial.  What belongs to hidden keys is replaced by 0 afterwards.
@@ -256,7 +286,12 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
       for (int w = 0; w < L::rows_warps; ++w) big = fmaxf(big, s_delta[128 + w]);
       if (threadIdx.x == 0) p.gmax[((int64_t)b * p.Hq + h) * tiles + qt] = big;
-      f = bwd_factor(big);
+      // values of all tiles of 128 keys that the walk touches: the sinks', then the windows'
+      const float* vmax = p.vmax + ((int64_t)b * p.Hk + hk) * tiles;
+      const int from = r.lo * kKeys / kTcRows, to = r.hi * kKeys / kTcRows, front = min((r.ns * kKeys + kTcRows - 1) / kTcRows, from);
+      float vbig = 0.f;
+      for (int e = lane; e < front + to - from + 1; e += 32) vbig = fmaxf(vbig, vmax[e < front ? e : from + e - front]);
+      f = bwd_factor<D>(big, warp_max(vbig));
     }
     if (part == 0 && i < p.T && !ahead) p.delta[((int64_t)b * p.Hq + h) * p.T + i] = delta;
     delta *= f;
@@ -497,7 +532,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       float big = 0.f;
       for (int e = lane; e < nit; e += 32)
         big = fmaxf(big, p.gmax[((int64_t)b * p.Hq + h_first + e / per_head) * sp.tiles + (qlo + e % per_head) / (kTcRows / kQ)]);
-      const float up = bwd_factor(warp_max(big));
+      const float up = bwd_factor<D>(warp_max(big), p.vmax[((int64_t)b * p.Hk + hk) * sp.tiles + kt]);
       f *= up;
       if (lane == 0) s_factor[0] = up;
     }
@@ -773,6 +808,11 @@ static int tc_backward(const SwParams& p, float* parts, int bf16, int* error_fla
   // Heads of 64: steps of 64 keys or queries and two CTAs on an SM, where there are CTAs for both.  Whole backward pass with such
   // steps for dQ, dK and dV / for dK and dV alone / for neither: 64 x 128, 12 heads 77 / 87 / 99 us, 16 x 512 91 / 105 / 116,
   // 8 x 2048 285 / 306 / 335, 4 x 4096, 16 over 4, window 128 188 / 226 / 234; 1 x 1024, 96 CTAs, dK and dV 44 against 40.
+  if constexpr (BwdRange<T>::scaled) {
+    sw_vmax_kernel<T, D><<<(unsigned)(s.tiles * p.B * p.Hk), 256, 0, st>>>(t, static_cast<const T*>(p.v), p.sv, s.tiles);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return (int)e;
+  }
   int code = D == 64 && gq > sm_count() ? dq_launch<T, 64, 64>(p, t, (unsigned)gq, bf16, st) : dq_launch<T, D, 128>(p, t, (unsigned)gq, bf16, st);
   if (code) return code;
   code = D == 64 && gk > sm_count() ? dkv_launch<T, 64, 64>(p, t, s, (unsigned)gk, bf16, st) : dkv_launch<T, D, 128>(p, t, s, (unsigned)gk, bf16, st);
