@@ -496,7 +496,7 @@ logprob_bwd_kernel(const LogProbGradParams p) {
     const int64_t t = p.tokens[row];
     float gl = p.g_lp ? p.g_lp[row] : 0.f;
     if (t == p.ignore) gl = 0.f;
-    else if (t < 0 || t >= p.cols) gl = NAN;
+    else if (t < 0 || t >= p.cols) gl = gl == 0.f ? 0.f : NAN;   // no such token: only a gradient that asks about it is NaN
     const float h = p.g_ent ? p.g_ent[row] : 0.f;
     float G = gl;
     if (p.g_top) for (int j = 0; j < p.k; ++j) G += p.g_top[row * p.k + j];

@@ -403,7 +403,7 @@ def token_log_probs(logits, tokens=None, topk=0, ignore_label=-1):
     lower token number, as int64.  Results are fp32 (fp64 for fp64 logits).
 
     A token equal to ``ignore_label`` is padding: its log probability is 0 and no gradient flows through it.  Any other token
-    outside 0 .. V - 1 gives NaN.  Tokens with a logit of -inf are ruled out; where all are, every log probability is -inf,
+    outside 0 .. V - 1 gives NaN, and a NaN gradient of the row where its log probability has a gradient other than 0.  Tokens with a logit of -inf are ruled out; where all are, every log probability is -inf,
     the entropy 0 and the gradient 0.  A NaN or +inf in a row makes its results NaN (``top_token`` then lists NaN first).
 
     Differentiable in ``logits`` through log_prob, entropy and top_log_prob.  On a GPU one kernel reads the logits once for all
@@ -431,6 +431,24 @@ def token_log_probs(logits, tokens=None, topk=0, ignore_label=-1):
     return res if flat else tuple(r.reshape(lead if i < 2 else lead + (k,)) for i, r in enumerate(res))
 
 
+class _NoSuchToken(torch.autograd.Function):
+    """NaN where a token is not ``known``; so is its gradient where one is asked for, but in rows in which nothing is possible."""
+    @staticmethod
+    def forward(ctx, x, known, empty):
+        ctx.save_for_backward(known, empty)
+        ctx.known = known
+        return x.masked_fill(~known, math.nan)
+
+    @staticmethod
+    def backward(ctx, g):
+        known, empty = ctx.saved_tensors
+        return torch.where(known, g, torch.zeros_like(g).masked_fill((g != 0) & ~empty, math.nan)), None, None
+
+    @staticmethod
+    def jvp(ctx, dx, *_):
+        return dx.masked_fill(~ctx.known, math.nan)
+
+
 def _token_log_probs(x, tok, k, ignore):
     V = x.shape[1]
     bad = (torch.isnan(x) | (x == math.inf)).any(-1, keepdim=True)
@@ -452,7 +470,7 @@ def _token_log_probs(x, tok, k, ignore):
     entropy = (log_total - (p * shifted.masked_fill(out, 0.0)).sum(-1, keepdim=True) + nan).masked_fill(empty, 0.0).squeeze(-1)
     known = (tok >= 0) & (tok < V)
     chosen = logp.gather(-1, tok.clamp(0, V - 1)[:, None]).squeeze(-1)
-    chosen = torch.where(known, chosen, torch.full_like(chosen, math.nan))
+    chosen = _NoSuchToken.apply(chosen, known, empty.squeeze(-1))
     chosen = torch.where(empty.squeeze(-1) & known, torch.full_like(chosen, -math.inf), chosen)
     chosen = torch.where(tok == ignore, torch.zeros_like(chosen), chosen)
     if not k:
