@@ -99,7 +99,7 @@ def rotary_inv_freq(dim=64, base=10000.0, scaling='none', factor=1.0, original_l
 
         def pair(turns):                         # the (real-valued) pair that makes that many turns over the original length
             return dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
-        lo, hi = max(0, math.floor(pair(fast_turns))), min(dim // 2 - 1, math.ceil(pair(slow_turns)))
+        lo, hi = max(0, math.floor(pair(fast_turns))), min(dim - 1, math.ceil(pair(slow_turns)))     # the ramp may end behind the last pair
         ramp = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 1e-3))) for i in range(dim // 2)]
         f = [x * (1 - r) + x / factor * r for x, r in zip(f, ramp)]
     dev = (ctx if ctx is not None else current_device()).torch_device
