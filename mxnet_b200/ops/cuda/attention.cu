@@ -484,13 +484,13 @@ MXB_EXPORT int mxb_attn_forward(int dtype, const void* qkv, const float* mask, v
   p.seed = seed; p.error_flag = error_flag;
   cudaStream_t st = (cudaStream_t)stream;
   static unsigned long long attr_seen = 0;
-  if (first_on_device(&attr_seen)) {
+  if (auto first = first_on_device(&attr_seen)) {
     cudaFuncSetAttribute(attn_fwd_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFwdSmem);
     cudaFuncSetAttribute(attn_fwd_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFwdSmem);
   }
   if (T > kAttT) {
     static unsigned long long long_seen = 0;
-    if (first_on_device(&long_seen)) {
+    if (auto first = first_on_device(&long_seen)) {
       cudaFuncSetAttribute(attn_fwd_long_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFwdLongSmem);
       cudaFuncSetAttribute(attn_fwd_long_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFwdLongSmem);
     }
@@ -528,14 +528,14 @@ MXB_EXPORT int mxb_attn_backward(int dtype, const void* qkv, const float* mask, 
   p.seed = seed; p.error_flag = error_flag;
   cudaStream_t st = (cudaStream_t)stream;
   static unsigned long long attr_seen = 0;
-  if (first_on_device(&attr_seen)) {
+  if (auto first = first_on_device(&attr_seen)) {
     cudaFuncSetAttribute(attn_bwd_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdSmem);
     cudaFuncSetAttribute(attn_bwd_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdSmem);
   }
   if (T > kAttT) {
     if (!workspace || ((uintptr_t)workspace % 16)) return -3;
     static unsigned long long long_seen = 0;
-    if (first_on_device(&long_seen)) {
+    if (auto first = first_on_device(&long_seen)) {
       cudaFuncSetAttribute(attn_bwd_long_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdLongSmem);
       cudaFuncSetAttribute(attn_bwd_long_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdLongSmem);
     }

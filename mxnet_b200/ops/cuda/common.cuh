@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include "device_setup.h"
 
 #define MXB_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -136,15 +137,19 @@ __device__ __forceinline__ void fd_divmod(uint32_t x, const FastDiv& f, uint32_t
   *r = x - *q * f.d;
 }
 
-// True the first time it is called on the current device for the bit set `seen` (one per call site): kernel function
-// attributes such as the dynamic shared-memory limit belong to a device, and one process may drive several.
-inline bool first_on_device(unsigned long long* seen) {
+// The setup of a call site on the current device; see FirstOnDevice.
+inline FirstOnDevice first_on_device(unsigned long long* seen) {
   int dev = 0;
   cudaGetDevice(&dev);
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (*seen & bit) return false;
-  *seen |= bit;
-  return true;
+  return FirstOnDevice(seen, dev);
+}
+
+// Dynamic shared memory of a kernel; the code of a refusal, which is not left behind for the next launch's check.
+template <typename K>
+inline int allow_smem(K kernel, int bytes) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) cudaGetLastError();
+  return (int)e;
 }
 
 inline int sm_count() {

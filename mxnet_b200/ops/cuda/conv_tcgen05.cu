@@ -524,7 +524,7 @@ static int launch_conv(const CUtensorMap& mx, const CUtensorMap& mw, const CUten
                        float* stats, ConvGeom g, int* error_flag, cudaStream_t st) {
   using Cfg = ConvCfg<BN>;
   static unsigned long long attr_seen = 0;
-  if (first_on_device(&attr_seen)) {
+  if (auto first = first_on_device(&attr_seen)) {
     cudaError_t rc = cudaFuncSetAttribute(conv_igemm_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
     if (rc != cudaSuccess) return (int)rc;
   }
@@ -888,7 +888,7 @@ static int launch_wgrad(const CUtensorMap& mdy, const CUtensorMap& mx, float* dW
                         cudaStream_t st) {
   using Cfg = ConvCfg<BN>;
   static unsigned long long attr_seen = 0;
-  if (first_on_device(&attr_seen)) {
+  if (auto first = first_on_device(&attr_seen)) {
     cudaError_t rc = cudaFuncSetAttribute(conv_wgrad_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
     if (rc != cudaSuccess) return (int)rc;
   }

@@ -243,7 +243,7 @@ static int launch_i8(const CUtensorMap& ma, const CUtensorMap& mb, const CUtenso
                      int* error_flag, cudaStream_t st) {
   using Cfg = I8Cfg<BN>;
   static unsigned long long attr_seen = 0;
-  if (first_on_device(&attr_seen)) {
+  if (auto first = first_on_device(&attr_seen)) {
     cudaError_t rc = cudaFuncSetAttribute(gemm_i8_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
     if (rc != cudaSuccess) return (int)rc;
   }

@@ -741,7 +741,7 @@ static int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUten
                        int b3d, int* error_flag, cudaStream_t st, int batch = 1, long long stride_d = 0) {
   using Cfg = TileCfg<BN>;
   static unsigned long long attr_seen = 0;
-  if (first_on_device(&attr_seen)) {
+  if (auto first = first_on_device(&attr_seen)) {
     cudaError_t rc = cudaFuncSetAttribute(gemm_tn_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
     if (rc != cudaSuccess) return (int)rc;
   }

@@ -68,9 +68,9 @@ static int tc_make_map(CUtensorMap* map, const void* base, int dtype, int64_t ro
 template <typename K>
 static int tc_launch(K kernel, unsigned long long* seen, int grid, size_t smem, cudaStream_t st, const CUtensorMap& m0,
                      const CUtensorMap& m1, const LstmTcParams& p) {
-  if (first_on_device(seen)) {
+  if (auto first = first_on_device(seen)) {
     cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTcSmemMax - 64);   // later shapes need more
-    if (rc != cudaSuccess) return (int)rc;
+    if (first.take((int)rc)) return (int)rc;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -90,9 +90,9 @@ static int tc_launch(K kernel, unsigned long long* seen, int grid, size_t smem, 
 template <typename K>
 static int tc_launch_cluster(K kernel, unsigned long long* seen, int grid, size_t smem, cudaStream_t st, const CUtensorMap& m0,
                              const CUtensorMap& m1, const LstmTcParams& p) {
-  if (first_on_device(seen)) {
+  if (auto first = first_on_device(seen)) {
     cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTcSmemMax - 64);
-    if (rc != cudaSuccess) return (int)rc;
+    if (first.take((int)rc)) return (int)rc;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -249,9 +249,9 @@ static GruPlan gru_plan(int dtype, int B, int H) {
 template <typename K>
 static int gru_launch(K kernel, unsigned long long* seen, int grid, size_t smem, int cluster, cudaStream_t st, const CUtensorMap& m0,
                       const CUtensorMap& m1, const GruTcParams& p) {
-  if (first_on_device(seen)) {
+  if (auto first = first_on_device(seen)) {
     cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTcSmemMax - 64);
-    if (rc != cudaSuccess) return (int)rc;
+    if (first.take((int)rc)) return (int)rc;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);

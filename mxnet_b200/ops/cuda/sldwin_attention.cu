@@ -211,11 +211,12 @@ static size_t sw_smem(int D) { return (size_t)(2 * 32 * (D + 1) + 2 * kSwWarps *
 template <typename T>
 static int sw_general(const SwParams& p, int pass, cudaStream_t st) {
   static unsigned long long seen = 0;
-  if (first_on_device(&seen)) {
+  if (auto first = first_on_device(&seen)) {
     const int most = (int)sw_smem(kSwMaxD);
-    cudaFuncSetAttribute(sw_row_kernel<T, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    cudaFuncSetAttribute(sw_row_kernel<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    cudaFuncSetAttribute(sw_key_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    int code = first.take(allow_smem(sw_row_kernel<T, 0>, most));
+    if (!code) code = first.take(allow_smem(sw_row_kernel<T, 1>, most));
+    if (!code) code = first.take(allow_smem(sw_key_kernel<T>, most));
+    if (code) return code;
   }
   const int64_t tiles = (p.T + kSwWarps - 1) / kSwWarps;
   const int64_t gq = tiles * p.B * p.Hq, gk = tiles * p.B * p.Hk;

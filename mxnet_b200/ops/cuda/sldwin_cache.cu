@@ -358,7 +358,10 @@ static int step_tc(const StepParams& p, cudaStream_t st) {
   if (units * csize > 0x7fffffff) return -2;
   const size_t smem = (size_t)(nw + 1) * 8 * (D + 2) * sizeof(float);
   static unsigned long long seen = 0;
-  if (first_on_device(&seen)) cudaFuncSetAttribute(step_tc_kernel<T, D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (auto first = first_on_device(&seen)) {
+    const int code = first.take((int)cudaFuncSetAttribute(step_tc_kernel<T, D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (code) { cudaGetLastError(); return code; }
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(units * csize));
   cfg.blockDim = dim3(nw * 32);

@@ -570,7 +570,8 @@ static int tc_forward_launch(const CUtensorMap& mq, const CUtensorMap& mk, const
   const int64_t grid = (t.qpair || kTiles == 1 ? tiles : (tiles + 1) / 2) * t.items;
   if (grid > 0x7fffffff) return -2;
   static unsigned long long seen = 0;
-  if (first_on_device(&seen)) cudaFuncSetAttribute(sw_fwd_tc_kernel<T, D, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::total);
+  if (auto first = first_on_device(&seen))
+    if (int code = first.take(allow_smem(sw_fwd_tc_kernel<T, D, kTiles>, L::total))) return code;
   sw_fwd_tc_kernel<T, D, kTiles><<<(unsigned)grid, L::threads, L::total, st>>>(mq, mk, mv, t, bf16);
   return (int)cudaGetLastError();
 }

@@ -776,7 +776,8 @@ static int dq_launch(const SwParams& p, const TcParams& t, unsigned grid, int bf
   if (!rc) rc = tc_map(&mg, p.dout, bf16, p.B, p.T, p.Hq, D, p.sdo);
   if (rc) return rc;
   static unsigned long long seen = 0;
-  if (first_on_device(&seen)) cudaFuncSetAttribute(sw_dq_tc_kernel<T, D, kKeys>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::total);
+  if (auto first = first_on_device(&seen))
+    if (int code = first.take(allow_smem(sw_dq_tc_kernel<T, D, kKeys>, L::total))) return code;
   sw_dq_tc_kernel<T, D, kKeys><<<grid, L::threads, L::total, st>>>(mq, mk, mv, mg, t, bf16);
   return (int)cudaGetLastError();
 }
@@ -791,7 +792,8 @@ static int dkv_launch(const SwParams& p, const TcParams& t, const DkvSplit& s, u
   if (!rc) rc = tc_map(&mg, p.dout, bf16, p.B, p.T, p.Hq, D, p.sdo, kQ);
   if (rc) return rc;
   static unsigned long long seen = 0;
-  if (first_on_device(&seen)) cudaFuncSetAttribute(sw_dkv_tc_kernel<T, D, kQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::total);
+  if (auto first = first_on_device(&seen))
+    if (int code = first.take(allow_smem(sw_dkv_tc_kernel<T, D, kQ>, L::total))) return code;
   sw_dkv_tc_kernel<T, D, kQ><<<grid, L::threads, L::total, st>>>(mq, mk, mv, mg, t, s, bf16);
   return (int)cudaGetLastError();
 }
