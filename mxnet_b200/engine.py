@@ -43,7 +43,24 @@ def push_async_error(exc):
         _pending.append(exc)
 
 
+_sync_checks = []
+
+
+def at_sync(check):
+    """``check()`` is called wherever the host has waited for device work (``wait_to_read``, ``asnumpy``, ``waitall``, at exit): it
+    raises what kernels have reported."""
+    with _pending_lock:
+        if check not in _sync_checks:
+            _sync_checks.append(check)
+
+
+def check_reports():
+    for check in _sync_checks:
+        check()
+
+
 def _rethrow_pending():
+    check_reports()
     if _pending:
         with _pending_lock:
             exc = _pending.pop(0) if _pending else None
@@ -91,6 +108,7 @@ def _check_fused_steps():
 def _at_exit():
     try:
         _check_fused_steps()
+        check_reports()
     except MXNetError as e:          # no caller is left to catch it: say it on stderr
         import sys
         sys.stderr.write('mxnet_b200: %s\n' % e)

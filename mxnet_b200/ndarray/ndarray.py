@@ -163,6 +163,7 @@ class NDArray(object):
             t = t.float()
         if t.is_cuda:
             t = t.cpu()
+            engine.check_reports()              # of the kernels that made it
         return t.numpy().copy() if t.dim() else _np.array(t.numpy())
 
     def asscalar(self):

@@ -11,6 +11,8 @@
 // This file holds the general kernels, which serve fp32 and head sizes that the tensor-core kernels do not take.  One
 // warp works on one query (or key) row and walks the other side in tiles of 32 rows in shared memory, one lane for each
 // row of the tile in the products over channels, one lane for each 32nd channel in the sums over rows.
+#include <mutex>
+
 #include "tcgen05.cuh"
 
 namespace mxb {
@@ -259,6 +261,25 @@ static SwParams sw_params(const int64_t* form, bool strides, float scale) {
 using namespace mxb;
 
 MXB_EXPORT int mxb_sldwin_max_dim(void) { return kSwMaxD; }
+
+// The word of host memory in which the kernels of every device report a wait that ran out (null: there is no memory).  It may be
+// asked for first inside a stream capture, which forbids allocations unless the thread says that this one is none of its own.
+MXB_EXPORT int* mxb_report_word(void) {
+  static std::mutex lock;
+  static int* word = nullptr;
+  std::lock_guard<std::mutex> guard(lock);
+  if (!word) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    void* at = nullptr;
+    if (cudaHostAlloc(&at, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
+      word = static_cast<int*>(at);
+      *word = 0;
+    } else cudaGetLastError();
+    cudaThreadExchangeStreamCaptureMode(&mode);
+  }
+  return word;
+}
 
 // lse: [B, Hq, T] floats (may be null when no backward pass follows).
 MXB_EXPORT int mxb_sldwin_forward(int dtype, const void* q, const void* k, const void* v, const int* valid, void* out, float* lse,

@@ -5,24 +5,33 @@ import ctypes as C
 import torch
 
 from . import lib, count_launch, check
+from ...base import MXNetError
 from ._util import DT, address, on_device, once, raw_stream
 
 _I13, _I16, _I18, _I19 = C.c_int64 * 13, C.c_int64 * 16, C.c_int64 * 18, C.c_int64 * 19      # sizes, then strides
 
 
-_report = []          # a word of pinned host memory that the kernels set when a wait inside them ran out, and its reader
+_report = []          # where kernels report a wait that ran out: the word of host memory, its address and its reader
 
 
 def _error_word():
+    """Address of the word; raises what an earlier call reported."""
     if not _report:
-        if torch.cuda.is_current_stream_capturing():
-            return 0                                              # a capture allows no allocation of host memory
-        word = torch.zeros(1, dtype=torch.int32).pin_memory()
-        _report.extend((word, word.data_ptr(), C.c_int.from_address(word.data_ptr())))
-    elif _report[2].value:
-        _report[2].value = 0
-        raise RuntimeError('an earlier call reported a barrier time-out inside its kernel: its results are not valid')
+        at = lib().mxb_report_word()
+        if not at:
+            raise RuntimeError('no host memory for the reports of kernels')
+        from ... import engine
+        word = C.c_int.from_address(at)
+        _report[:] = (word, at, word)
+        engine.at_sync(_raise_reported)
+    _raise_reported()
     return _report[1]
+
+
+def _raise_reported():
+    if _report[2].value:
+        _report[2].value = 0
+        raise MXNetError('an earlier call reported a barrier time-out inside its kernel: its results are not valid')
 
 
 def _rows(t):
