@@ -8,6 +8,7 @@ They stand beside the reference's transformer helpers (``src/operator/contrib/tr
 from __future__ import annotations
 
 import math
+import numbers
 
 import torch
 
@@ -49,8 +50,11 @@ def _same(name, first, **others):
 
 
 def _whole(name, what, v):
-    _need(isinstance(v, int) and not isinstance(v, bool) or (isinstance(v, float) and v.is_integer()), '%s: %s must be a whole number, got %r',
-          name, what, v)
+    """``v`` as an int: whole numbers of any type that is not a truth value, real ones without a fraction."""
+    if isinstance(v, numbers.Integral) and not isinstance(v, bool):
+        return int(v)
+    _need(isinstance(v, numbers.Real) and not isinstance(v, bool) and float(v).is_integer(), '%s: %s must be a whole number, got %r', name,
+          what, v)
     return int(v)
 
 
@@ -162,7 +166,7 @@ def rotary_embedding(data, positions=None, inv_freq=None, interleaved=False, sca
 # ------------------------------------------------------------------------------------------
 def _window_args(name, window, sinks, scale, D):
     if type(window) is not int or type(sinks) is not int:
-        window, sinks = _whole(name, 'window', window or 0), _whole(name, 'sinks', sinks or 0)
+        window, sinks = _whole(name, 'window', 0 if window is None else window), _whole(name, 'sinks', 0 if sinks is None else sinks)
     if window < 0 or sinks < 0:
         _need(False, '%s: window and sinks must not be negative, got %d and %d', name, window, sinks)
     return window, sinks, 1.0 / math.sqrt(D) if scale is None else float(scale)
@@ -304,7 +308,7 @@ def sldwin_cache_fill(key, value=None, key_cache=None, value_cache=None, valid_l
     _need(key.dim() == 4 and value.shape == key.shape, '%s: key and value must be (B, T, H, D), got %s and %s', name, tuple(key.shape),
           tuple(value.shape))
     B, T, Hk, D = key.shape
-    sinks = _whole(name, 'sinks', sinks or 0)
+    sinks = _whole(name, 'sinks', 0 if sinks is None else sinks)
     _need(sinks >= 0, '%s: sinks must not be negative, got %d', name, sinks)
     _same(name, key, value=value)
     _cache_args(name, key_cache, value_cache, B, Hk, D, sinks, key)
@@ -411,7 +415,7 @@ def token_log_probs(logits, tokens=None, topk=0, ignore_label=-1):
     name = 'token_log_probs'
     if tokens is None or type(topk) is not int or type(ignore_label) is not int:
         _need(tokens is not None, '%s: logits and tokens are required', name)
-        topk, ignore_label = _whole(name, 'topk', topk or 0), _whole(name, 'ignore_label', ignore_label)
+        topk, ignore_label = _whole(name, 'topk', 0 if topk is None else topk), _whole(name, 'ignore_label', ignore_label)
     k, ignore = topk, ignore_label
     shape = logits.shape
     if not (len(shape) >= 1 and logits.is_floating_point() and tokens.shape == shape[:-1] and shape[-1] >= 1 and
