@@ -25,6 +25,7 @@ _amp_initialized = False
 _amp_loss_scale_initialized = False
 _target = None
 _sets = None
+_rules = ({}, {})        # inputs that are not cast, inputs that take another one's type
 _ORDER = [torch.float16, torch.bfloat16, torch.float32, torch.float64]
 
 
@@ -45,7 +46,46 @@ def _expand(names):
     return out
 
 
+def _kept(names, lists):
+    """Operator name -> indexes of the inputs that no list casts."""
+    from ..ops import registry as reg
+    out = {}
+    for n in names:
+        if reg.has(n):
+            op = reg.get(n)
+            keep = op.mutate + lists.KEEP_INPUTS.get(op.name, ())
+            if keep:
+                out[op.name] = frozenset(i for i, name in enumerate(op.inputs) if name in keep)
+    return out
+
+
+def _like(lists):
+    """Operator name -> (index of the input that gives the type, indexes of those that take it)."""
+    from ..ops import registry as reg
+    out = {}
+    for n, (giver, takers) in lists.LIKE_INPUTS.items():
+        names = reg.get(n).inputs
+        out[n] = names.index(giver), frozenset(names.index(t) for t in takers)
+    return out
+
+
 def _hook(opname, tensors):
+    like = _rules[1].get(opname)
+    if like is not None:
+        giver = tensors[like[0]] if like[0] < len(tensors) else None
+        if not isinstance(giver, torch.Tensor) or not giver.is_floating_point():
+            return tensors
+        return [t.to(giver.dtype) if i in like[1] and isinstance(t, torch.Tensor) and t.is_floating_point() else t
+                for i, t in enumerate(tensors)]
+    keep = _rules[0].get(opname)
+    if keep is None:
+        return _cast(opname, tensors)
+    rest = _cast(opname, [t for i, t in enumerate(tensors) if i not in keep])
+    at = iter(rest)
+    return [t if i in keep else next(at) for i, t in enumerate(tensors)]
+
+
+def _cast(opname, tensors):
     lp, fp32, widest = _sets
     if opname in lp:
         return [t.to(_target) if isinstance(t, torch.Tensor) and t.is_floating_point() and t.dtype != _target else t
@@ -66,7 +106,7 @@ from ..base import bfloat16   # noqa: E402,F401  (the dtype name scripts import 
 
 def init(target_dtype='float16', target_precision_ops=None, conditional_fp32_ops=None, fp32_ops=None, layout_optimization=False):
     """Turn on AMP for all subsequently executed operators."""
-    global _amp_initialized, _target, _sets
+    global _amp_initialized, _target, _sets, _rules
     td = to_torch_dtype(target_dtype)
     assert td in (torch.float16, torch.bfloat16), 'AMP currently supports only float16 or bfloat16 as a target_dtype'
     if _amp_initialized:
@@ -77,6 +117,7 @@ def init(target_dtype='float16', target_precision_ops=None, conditional_fp32_ops
     f32 = list(fp32_ops) if fp32_ops is not None else list(lists.FP32_FUNCS)
     _target = td
     _sets = (_expand(lp), _expand(f32), _expand(lists.WIDEST_TYPE_CASTS))
+    _rules = (_kept(set().union(*_sets), lists), _like(lists))
     _state.amp_hook = _hook
     _amp_initialized = True
     if layout_optimization:
@@ -170,7 +211,8 @@ def convert_symbol(sym, input_dtypes=None, param_dtypes=None, target_dtype='floa
     lp = target_dtype_ops if target_dtype_ops is not None else (lists.BF16_FUNCS if td == torch.bfloat16 else lists.FP16_FUNCS)
     f32 = fp32_ops if fp32_ops is not None else lists.FP32_FUNCS
     return passes.convert_precision(sym, 'bfloat16' if td == torch.bfloat16 else 'float16', _expand(lp), _expand(f32),
-                                    _expand(lists.WIDEST_TYPE_CASTS), cast_optional_params, set(excluded_sym_names or ()))
+                                    _expand(lists.WIDEST_TYPE_CASTS), cast_optional_params, set(excluded_sym_names or ()),
+                                    _kept(_expand(list(lp) + list(f32)), lists))
 
 
 def convert_model(sym, arg_params, aux_params, input_dtypes=None, target_dtype='float16', target_dtype_ops=None,

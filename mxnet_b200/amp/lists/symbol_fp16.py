@@ -7,8 +7,16 @@ FP16_FUNCS = [
     'Convolution', 'Deconvolution', 'FullyConnected', 'RNN', 'dot', 'batch_dot', '_npi_matmul', '_npi_dot',
     '_npi_einsum', '_npi_tensordot', '_contrib_interleaved_matmul_selfatt_qk', '_contrib_interleaved_matmul_selfatt_valatt',
     '_contrib_interleaved_matmul_encdec_qk', '_contrib_interleaved_matmul_encdec_valatt', '_contrib_fused_self_attention',
-    '_linalg_gemm', '_linalg_gemm2',
+    '_contrib_sldwin_attention', '_linalg_gemm', '_linalg_gemm2',
 ]
+# Inputs that keep their type whatever list their operator is in: numbers of tokens, which half types do not hold.  (What an operator
+# updates in place keeps its type as well: the update would go to a copy.)
+KEEP_INPUTS = {'_contrib_sldwin_attention': ('valid_length',)}
+# Inputs that take the type of another one: of a cache, which the program has laid out in the type that it wants.
+LIKE_INPUTS = {
+    '_contrib_sldwin_cache_fill': ('key_cache', ('key', 'value')),
+    '_contrib_sldwin_attention_step': ('key_cache', ('query', 'key', 'value')),
+}
 # softmax, log_softmax and the fused softmax cross-entropy are NOT forced to fp32 inputs here (the reference lists them
 # under FP32_FUNCS): their kernels read half-precision rows and do the exponentials, sums and the loss in fp32
 # registers, so casting a [tokens, vocabulary] score matrix to fp32 first would only add a pass over HBM.
@@ -27,7 +35,7 @@ FP16_FP32_FUNCS = [
     'abs', 'sign', 'sqrt', 'square', 'negative', 'LeakyReLU', 'expand_dims', 'squeeze', 'tile', 'repeat', 'reverse',
     'broadcast_to', 'broadcast_like', 'zeros_like', 'ones_like', 'Cast', 'identity', 'BlockGrad', 'SequenceMask',
     'SequenceLast', 'SequenceReverse', 'where', 'max', 'min', 'argmax', 'argmin', 'sort', 'argsort', 'UpSampling', 'Pad',
-    'SwapAxis', 'gather_nd', 'scatter_nd',
+    'SwapAxis', 'gather_nd', 'scatter_nd', '_contrib_rotary_embedding', '_contrib_token_log_probs',
 ]
 WIDEST_TYPE_CASTS = [
     'broadcast_add', 'broadcast_sub', 'broadcast_mul', 'broadcast_div', 'broadcast_mod', 'broadcast_power',

@@ -73,8 +73,9 @@ def eliminate_common_expr(sym):
 
 
 def convert_precision(sym, target_dtype, fp16_ops, fp32_ops, widest_ops, cast_optional_params=False,
-                      excluded_names=()):
-    """``ReducePrecision`` pass: insert ``amp_cast`` before operators according to the lists."""
+                      excluded_names=(), kept=None):
+    """``ReducePrecision`` pass: insert ``amp_cast`` before operators according to the lists.  ``kept``: operator name -> indexes
+    of the inputs that are left as they are."""
     cast = _reg.get('amp_cast')
     multicast = _reg.get('amp_multicast')
     counter = [0]
@@ -89,11 +90,11 @@ def convert_precision(sym, target_dtype, fp16_ops, fp32_ops, widest_ops, cast_op
             return None
         name = n.op.name
         names = [name] + list(n.op.aliases)
+        keep = (kept or {}).get(name, ())
         if any(x in fp16_ops for x in names):
-            new_ins = [casted(e, target_dtype) if (e[0].op is not None or cast_optional_params or j == 0 or True) else e
-                       for j, e in enumerate(ins)]
+            new_ins = [e if j in keep else casted(e, target_dtype) for j, e in enumerate(ins)]
         elif any(x in fp32_ops for x in names):
-            new_ins = [casted(e, 'float32') for e in ins]
+            new_ins = [e if j in keep else casted(e, 'float32') for j, e in enumerate(ins)]
         elif any(x in widest_ops for x in names) and len(ins) > 1:
             counter[0] += 1
             mc = _Node(multicast, 'amp_multicast_%d' % counter[0], {'num_outputs': len(ins)}, list(ins), len(ins))
