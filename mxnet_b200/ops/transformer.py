@@ -11,6 +11,7 @@ import math
 import numbers
 
 import torch
+from torch.autograd import forward_ad
 
 from .registry import register
 from .cuda import logprob_ops, rotary_ops, sldwin_ops
@@ -27,7 +28,8 @@ def _need(ok, what, *args):
 
 
 def _kernels(t):
-    return t.is_cuda and t.dtype in _KERNEL_TYPES and t.numel() > 0 and env.get('MXNET_B200_KERNELS')
+    # forward-mode differentiation runs through the tensor library: the kernels know no tangents
+    return t.is_cuda and t.dtype in _KERNEL_TYPES and t.numel() > 0 and env.get('MXNET_B200_KERNELS') and forward_ad._current_level < 0
 
 
 def _alike(first, second, third):
@@ -285,6 +287,9 @@ def _no_gradient(name, *arrays):
     if torch.is_grad_enabled():
         _need(not any(a.requires_grad for a in arrays), '%s updates its caches in place and has no gradient: call it '
               'outside of autograd.record(), or on detached arrays', name)
+    if forward_ad._current_level >= 0:
+        _need(all(forward_ad.unpack_dual(a).tangent is None for a in arrays), '%s updates its caches in place and has no gradient in '
+              'forward mode either', name)
 
 
 def _written(*arrays):
