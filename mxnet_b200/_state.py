@@ -15,6 +15,7 @@ class _State(threading.local):
         self.np_shape = False
         self.np_array = False
         self.np_default_dtype = False
+        self.crossed = False        # a copy between devices was recorded since the last gradient pass
         self.opt_constraints = 0      # HybridBlock.OptConstraint flags (bit 0: AMP casts off)
         self.tracer = None          # active deferred-compute tracer (symbol/_trace.py) or None
         self.writes = None          # list that collects the tensors operators update in place (gluon/cached_op.py) or None

@@ -205,9 +205,11 @@ _here = threading.local()           # .devices: those whose passes this thread r
 def _calling_thread(tensors):
     """Scope of a gradient pass whose heads lie on one device: it runs on the thread that asked for it.  The tensor library's
     worker of that device would do the same work in the same order after two thread switches (30 to 200 us, as the machine
-    schedules them); heads on several devices keep their workers, which run side by side."""
+    schedules them); heads on several devices, and graphs with a copy between devices, keep their workers, which run side by
+    side."""
     first = tensors[0].device if tensors else None
-    if first is not None and first.type == 'cuda' and all(t.device == first for t in tensors[1:]):
+    crossed, _state.state.crossed = _state.state.crossed, False
+    if first is not None and first.type == 'cuda' and not crossed and all(t.device == first for t in tensors[1:]):
         try:
             _here.devices.add(first.index)
         except AttributeError:

@@ -207,6 +207,7 @@ class NDArray(object):
             return other
         if isinstance(other, Device):
             t = self._data.to(other.torch_device, copy=True)
+            _note_crossing(self._data, t)
             return self.__class__._from_tensor(t, other)
         raise TypeError('copyto does not support type ' + str(type(other)))
 
@@ -221,6 +222,7 @@ class NDArray(object):
             return r
         if _state.state.recording and self._data.requires_grad:
             t = self._data.to(context.torch_device)
+            _note_crossing(self._data, t)
         elif context.torch_device.type == 'cuda' and not self._data.is_cuda:
             from .. import engine
             engine.wait_for(self)
@@ -327,6 +329,7 @@ class NDArray(object):
             v = value._data
             if v.device != self._data.device:
                 v = v.to(self._data.device)
+                _note_crossing(value._data, v)
         elif isinstance(value, (_np.ndarray, list, tuple)):
             v = torch.as_tensor(_np.asarray(value), device=self._data.device).to(self._data.dtype)
         else:
@@ -616,6 +619,12 @@ for _n in ('abs', 'sign', 'sqrt', 'rsqrt', 'cbrt', 'rcbrt', 'square', 'reciproca
         setattr(NDArray, _n, _unary_method(_n))
 
 _reg._set_array_class('nd', NDArray)
+
+
+def _note_crossing(src, dst):
+    """A recorded copy between devices: the graph that it belongs to lies on several (``autograd.backward``)."""
+    if dst.requires_grad and src.device != dst.device:
+        _state.state.crossed = True
 
 
 def _identity_copy(t):

@@ -558,6 +558,8 @@ class Symbol(object):
                     copies += 1                            # a _CrossDeviceCopy of the reference
                     if t.device != dev:
                         t = t.to(dev)
+                        if t.requires_grad:
+                            _state.state.crossed = True
                 ins.append(t)
             hook = _state.amp_hook
             if hook is not None and not _state.state.opt_constraints & 1:

@@ -2,9 +2,11 @@
 import threading
 from types import SimpleNamespace
 
+import pytest
 import torch
 
-from mxnet_b200 import autograd
+import mxnet_b200 as mx
+from mxnet_b200 import _state, autograd, nd
 
 
 def on(*indexes):
@@ -54,3 +56,42 @@ def test_the_setting_is_put_back_after_a_pass_that_raises():
         except ValueError:
             pass
         assert torch._C._is_multithreading_enabled()
+
+
+def test_a_graph_over_several_devices_keeps_its_workers(monkeypatch):
+    fresh(monkeypatch)
+    assert stays(autograd._calling_thread(on(0)))
+    _state.state.crossed = True
+    assert not stays(autograd._calling_thread(on(0)))
+    assert stays(autograd._calling_thread(on(0)))                   # the next graph is another one
+    nd.ones((2,)).as_in_context(mx.cpu(1))
+    with autograd.record():
+        nd.ones((2,)).as_in_context(mx.cpu(1))                      # one device by two names
+    assert not _state.state.crossed
+
+
+@pytest.mark.gpu
+def test_a_recorded_copy_between_devices_is_seen():
+    seen = []
+
+    class Spy(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            seen.append(threading.get_ident())
+            return g * 2
+    x = nd.ones((3,), ctx=mx.gpu(0))
+    x.attach_grad()
+    spied = lambda a: nd.NDArray(Spy.apply(a._data))                # noqa: E731
+    for move in (lambda a: a, lambda a: a.as_in_context(mx.cpu()).as_in_context(mx.gpu(0)), lambda a: a.copyto(mx.cpu()).copyto(mx.gpu(0)),
+                 lambda a: a):
+        with autograd.record():
+            with torch.enable_grad():
+                y = move(spied(x)) * 3
+        y.backward()
+        assert x.grad._data.tolist() == [6.] * 3
+    here = threading.get_ident()
+    assert [s == here for s in seen] == [True, False, False, True]
