@@ -260,8 +260,6 @@ static SwParams sw_params(const int64_t* form, bool strides, float scale) {
 
 using namespace mxb;
 
-MXB_EXPORT int mxb_sldwin_max_dim(void) { return kSwMaxD; }
-
 // The word of host memory in which the kernels of every device report a wait that ran out (null: there is no memory).  It may be
 // asked for first inside a stream capture, which forbids allocations unless the thread says that this one is none of its own.
 MXB_EXPORT int* mxb_report_word(void) {

@@ -24,7 +24,8 @@ def _error_word():
         word = C.c_int.from_address(at)
         _report[:] = (word, at, word)
         engine.at_sync(_raise_reported)
-    _raise_reported()
+    if _report[2].value:
+        _raise_reported()
     return _report[1]
 
 

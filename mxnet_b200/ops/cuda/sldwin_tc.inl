@@ -310,108 +310,104 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   if (warp == L::tma) {
     // ---------------------------------------------------------------- loads
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::other_regs));
-    if (ntiles > 0) {
+    if (lane == 0) {
+      for (int s = 0; s < kTiles; ++s) {
+        if ((s ? r1 : r0).count() == 0) continue;
+        mbar_expect_tx(&q_full[s], L::tile);
+        tc_load_tile<D>(smem + L::q + s * L::tile, &map_q, h0 + s * hstep, qa + s * qstep, b, &q_full[s]);
+      }
+    }
+    bool ok = true;
+    int nk = 0, nv = 0;                                         // tiles asked for
+    for (int j = 0; j < ntiles; ++j) {
+      const int st = j % kFwdStages, kt = key_tile(j);
+      const uint32_t ph = (uint32_t)(j / kFwdStages + 1) & 1u;
+      if (j >= kFwdStages && !(ok = mbar_wait_warp(&k_empty[st], ph))) break;
       if (lane == 0) {
-        for (int s = 0; s < kTiles; ++s) {
-          if ((s ? r1 : r0).count() == 0) continue;
-          mbar_expect_tx(&q_full[s], L::tile);
-          tc_load_tile<D>(smem + L::q + s * L::tile, &map_q, h0 + s * hstep, qa + s * qstep, b, &q_full[s]);
-        }
+        mbar_expect_tx(&k_full[st], L::tile);
+        tc_load_tile<D>(smem + L::k + st * L::tile, &map_k, hk, kt * kTcRows, b, &k_full[st]);
       }
-      bool ok = true;
-      int nk = 0, nv = 0;                                         // tiles asked for
-      for (int j = 0; j < ntiles; ++j) {
-        const int st = j % kFwdStages, kt = key_tile(j);
-        const uint32_t ph = (uint32_t)(j / kFwdStages + 1) & 1u;
-        if (j >= kFwdStages && !(ok = mbar_wait_warp(&k_empty[st], ph))) break;
-        if (lane == 0) {
-          mbar_expect_tx(&k_full[st], L::tile);
-          tc_load_tile<D>(smem + L::k + st * L::tile, &map_k, hk, kt * kTcRows, b, &k_full[st]);
-        }
-        nk = j + 1;
-        if (j >= kFwdStages && !(ok = mbar_wait_warp(&v_empty[st], ph))) break;
-        const bool ends = (kt + 1) * kTcRows > n && n < p.T;      // the sequence ends inside this tile
-        uint8_t* tile = smem + L::v + st * L::tile;
-        if (lane == 0) {
-          uint64_t* bar = ends ? patch : &v_full[st];
-          mbar_expect_tx(bar, L::tile);
-          tc_load_tile<D>(tile, &map_v, hk, kt * kTcRows, b, bar);
-        }
-        nv = ends ? j : j + 1;
-        if (ends) {                                               // the last tile of the sequence: at most once
-          if (!(ok = mbar_wait_warp(patch, 0))) break;
-          tc_clear_rows<D>(tile, n - kt * kTcRows);
-          if (lane == 0) mbar_arrive(&v_full[st]);
-        }
+      nk = j + 1;
+      if (j >= kFwdStages && !(ok = mbar_wait_warp(&v_empty[st], ph))) break;
+      const bool ends = (kt + 1) * kTcRows > n && n < p.T;      // the sequence ends inside this tile
+      uint8_t* tile = smem + L::v + st * L::tile;
+      if (lane == 0) {
+        uint64_t* bar = ends ? patch : &v_full[st];
+        mbar_expect_tx(bar, L::tile);
+        tc_load_tile<D>(tile, &map_v, hk, kt * kTcRows, b, bar);
       }
-      if (!ok) {
-        *abort_flag = 1;
-        if (lane == 0) {
-          // no copy may still be under way when the CTA's shared memory is given back
-          for (int s = 0; s < 2; ++s) {
-            if (s < kTiles && (s ? r1 : r0).count()) mbar_wait(&q_full[s], 0);
-            if (nk > s) mbar_wait(&k_full[s], (uint32_t)((nk - 1 - s) / kFwdStages) & 1u);
-            if (nv > s) mbar_wait(&v_full[s], (uint32_t)((nv - 1 - s) / kFwdStages) & 1u);
-          }
+      nv = ends ? j : j + 1;
+      if (ends) {                                               // the last tile of the sequence: at most once
+        if (!(ok = mbar_wait_warp(patch, 0))) break;
+        tc_clear_rows<D>(tile, n - kt * kTcRows);
+        if (lane == 0) mbar_arrive(&v_full[st]);
+      }
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      if (lane == 0) {
+        // no copy may still be under way when the CTA's shared memory is given back
+        for (int s = 0; s < 2; ++s) {
+          if (s < kTiles && (s ? r1 : r0).count()) mbar_wait(&q_full[s], 0);
+          if (nk > s) mbar_wait(&k_full[s], (uint32_t)((nk - 1 - s) / kFwdStages) & 1u);
+          if (nv > s) mbar_wait(&v_full[s], (uint32_t)((nv - 1 - s) / kFwdStages) & 1u);
         }
       }
     }
   } else if (warp == L::mma) {
     // ---------------------------------------------------------------- products
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::other_regs));
-    if (ntiles > 0) {
-      const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
-      const uint64_t dq = make_desc(smem_u32(smem + L::q)), dk = make_desc(smem_u32(smem + L::k)),
-                     dv = make_desc_mn(smem_u32(smem + L::v), kTcHalf);
-      constexpr uint64_t step = L::tile >> 4;
-      bool ok = true;
-      uint32_t pphase = 0, started = 0;                           // bit s: of query tile s
-      for (int s = 0; s < kTiles && ok; ++s) {
-        const KeyRange& r = s ? r1 : r0;
-        if (r.count() == 0) continue;
-        ok = mbar_wait_warp(&q_full[s], 0);
-        if (ok && r.has(key_tile(0))) {
-          ok = mbar_wait_warp(&k_full[0], 0);
-          tc_fence_after();
-          if (ok && elect_one()) { tc_scores<D>(tmem + 128 * s, dq + s * step, dk, id_s); umma_commit(&s_full[s]); }
-        }
+    const uint32_t id_s = make_idesc(bf16, 128, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
+    const uint64_t dq = make_desc(smem_u32(smem + L::q)), dk = make_desc(smem_u32(smem + L::k)),
+                   dv = make_desc_mn(smem_u32(smem + L::v), kTcHalf);
+    constexpr uint64_t step = L::tile >> 4;
+    bool ok = true;
+    uint32_t pphase = 0, started = 0;                           // bit s: of query tile s
+    for (int s = 0; s < kTiles && ok; ++s) {
+      const KeyRange& r = s ? r1 : r0;
+      if (r.count() == 0) continue;
+      ok = mbar_wait_warp(&q_full[s], 0);
+      if (ok && r.has(key_tile(0))) {
+        ok = mbar_wait_warp(&k_full[0], 0);
+        tc_fence_after();
+        if (ok && elect_one()) { tc_scores<D>(tmem + 128 * s, dq + s * step, dk, id_s); umma_commit(&s_full[s]); }
       }
-      if (elect_one()) umma_commit(&k_empty[0]);
-      for (int j = 0; j < ntiles && ok; ++j) {
-        const int kt = key_tile(j), next = j + 1 < ntiles ? key_tile(j + 1) : -1;
-        const int st = j % kFwdStages, sn = (j + 1) % kFwdStages;
-        const uint32_t ph = (uint32_t)(j / kFwdStages) & 1u, pn = (uint32_t)((j + 1) / kFwdStages) & 1u;
-        ok = mbar_wait_warp(&v_full[st], ph);
-#pragma unroll
-        for (int s = 0; s < kTiles; ++s) {
-          const KeyRange& r = s ? r1 : r0;
-          if (ok && r.has(kt)) {
-            ok = mbar_wait_warp(&p_half[s], pphase >> s & 1u);
-            tc_fence_after();
-            if (ok && elect_one()) tc_accumulate<8, 0, 4>(tmem + L::tmem_o + D * s, tmem + 128 * s, dv + st * step, id_o, started >> s & 1u);
-            ok = ok && mbar_wait_warp(&p_full[s], pphase >> s & 1u);
-            pphase ^= 1u << s;
-            tc_fence_after();
-            if (ok && elect_one()) tc_accumulate<8, 4, 8>(tmem + L::tmem_o + D * s, tmem + 128 * s, dv + st * step, id_o, 1u);
-            started |= 1u << s;
-          }
-          if (ok && next >= 0 && r.has(next)) {
-            if (s == 0 || !r0.has(next)) ok = mbar_wait_warp(&k_full[sn], pn);
-            tc_fence_after();
-            if (ok && elect_one()) {
-              tc_scores<D>(tmem + 128 * s, dq + s * step, dk + sn * step, id_s);
-              umma_commit(&s_full[s]);                            // complete only after P V of this tile, issued before it
-            }
-          }
-        }
-        if (ok && elect_one()) {
-          umma_commit(&v_empty[st]);
-          if (next >= 0) umma_commit(&k_empty[sn]);
-        }
-      }
-      if (elect_one()) umma_commit(ok ? o_full : drain);
-      if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
     }
+    if (elect_one()) umma_commit(&k_empty[0]);
+    for (int j = 0; j < ntiles && ok; ++j) {
+      const int kt = key_tile(j), next = j + 1 < ntiles ? key_tile(j + 1) : -1;
+      const int st = j % kFwdStages, sn = (j + 1) % kFwdStages;
+      const uint32_t ph = (uint32_t)(j / kFwdStages) & 1u, pn = (uint32_t)((j + 1) / kFwdStages) & 1u;
+      ok = mbar_wait_warp(&v_full[st], ph);
+#pragma unroll
+      for (int s = 0; s < kTiles; ++s) {
+        const KeyRange& r = s ? r1 : r0;
+        if (ok && r.has(kt)) {
+          ok = mbar_wait_warp(&p_half[s], pphase >> s & 1u);
+          tc_fence_after();
+          if (ok && elect_one()) tc_accumulate<8, 0, 4>(tmem + L::tmem_o + D * s, tmem + 128 * s, dv + st * step, id_o, started >> s & 1u);
+          ok = ok && mbar_wait_warp(&p_full[s], pphase >> s & 1u);
+          pphase ^= 1u << s;
+          tc_fence_after();
+          if (ok && elect_one()) tc_accumulate<8, 4, 8>(tmem + L::tmem_o + D * s, tmem + 128 * s, dv + st * step, id_o, 1u);
+          started |= 1u << s;
+        }
+        if (ok && next >= 0 && r.has(next)) {
+          if (s == 0 || !r0.has(next)) ok = mbar_wait_warp(&k_full[sn], pn);
+          tc_fence_after();
+          if (ok && elect_one()) {
+            tc_scores<D>(tmem + 128 * s, dq + s * step, dk + sn * step, id_s);
+            umma_commit(&s_full[s]);                            // complete only after P V of this tile, issued before it
+          }
+        }
+      }
+      if (ok && elect_one()) {
+        umma_commit(&v_empty[st]);
+        if (next >= 0) umma_commit(&k_empty[sn]);
+      }
+    }
+    if (elect_one()) umma_commit(ok ? o_full : drain);
+    if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
   } else if (warp > L::tma) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::other_regs));
   } else {
@@ -492,7 +488,7 @@ sw_fwd_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       unpack_f2(add_f2(part[0], part[1]), l0, l1);
       l += l0 + l1;
     }
-    if (ok && ntiles > 0) ok = mbar_wait_warp(o_full, 0);
+    if (ok) ok = mbar_wait_warp(o_full, 0);
     if (!ok) *abort_flag = 1;
     tc_fence_after();
     if (ok) {

@@ -160,90 +160,86 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   } else tmem = tc_start<L::threads, L::tmem_cols>(tmem_slot, warp == L::mma);
 
   if (warp == L::tma) {
-    if (ntiles > 0) {
+    if (lane == 0) {
+      mbar_expect_tx(qg_full, 2 * L::tile);
+      tc_load_tile<D>(smem + L::q, &map_q, h, q0, b, qg_full);
+      tc_load_tile<D>(smem + L::g, &map_g, h, q0, b, qg_full);
+    }
+    bool ok = true;
+    int nk = 0, nv = 0;
+    uint32_t patched = 0;
+    for (int j = 0; j < nit; ++j) {
+      const int sk = j % L::kst, sv = j % L::vst, kt = key_tile(j);
+      if (j >= L::kst && !(ok = mbar_wait_warp(&k_empty[sk], (uint32_t)(j / L::kst + 1) & 1u))) break;
+      const bool ends = (kt + 1) * kKeys > n && n < p.T;      // the sequence ends inside this tile: dS K must not meet what follows
+      uint8_t* tile = smem + L::k + sk * L::ktile;
       if (lane == 0) {
-        mbar_expect_tx(qg_full, 2 * L::tile);
-        tc_load_tile<D>(smem + L::q, &map_q, h, q0, b, qg_full);
-        tc_load_tile<D>(smem + L::g, &map_g, h, q0, b, qg_full);
+        uint64_t* bar = ends ? patch : &k_full[sk];
+        mbar_expect_tx(bar, L::ktile);
+        tc_load_tile<D>(tile, &map_k, hk, kt * kKeys, b, bar);
       }
-      bool ok = true;
-      int nk = 0, nv = 0;
-      uint32_t patched = 0;
-      for (int j = 0; j < nit; ++j) {
-        const int sk = j % L::kst, sv = j % L::vst, kt = key_tile(j);
-        if (j >= L::kst && !(ok = mbar_wait_warp(&k_empty[sk], (uint32_t)(j / L::kst + 1) & 1u))) break;
-        const bool ends = (kt + 1) * kKeys > n && n < p.T;      // the sequence ends inside this tile: dS K must not meet what follows
-        uint8_t* tile = smem + L::k + sk * L::ktile;
-        if (lane == 0) {
-          uint64_t* bar = ends ? patch : &k_full[sk];
-          mbar_expect_tx(bar, L::ktile);
-          tc_load_tile<D>(tile, &map_k, hk, kt * kKeys, b, bar);
-        }
-        nk = ends ? j : j + 1;
-        if (ends) {
-          if (!(ok = mbar_wait_warp(patch, patched++ & 1u))) break;
-          tc_clear_rows<D, kKeys>(tile, n - kt * kKeys);
-          if (lane == 0) mbar_arrive(&k_full[sk]);
-        }
-        if (j >= L::vst && !(ok = mbar_wait_warp(&v_empty[sv], (uint32_t)(j / L::vst + 1) & 1u))) break;
-        if (lane == 0) {
-          mbar_expect_tx(&v_full[sv], L::ktile);
-          tc_load_tile<D>(smem + L::v + sv * L::ktile, &map_v, hk, kt * kKeys, b, &v_full[sv]);
-        }
-        nv = j + 1;
+      nk = ends ? j : j + 1;
+      if (ends) {
+        if (!(ok = mbar_wait_warp(patch, patched++ & 1u))) break;
+        tc_clear_rows<D, kKeys>(tile, n - kt * kKeys);
+        if (lane == 0) mbar_arrive(&k_full[sk]);
       }
-      if (!ok) {
-        *abort_flag = 1;
-        if (lane == 0) {                                          // no copy may still be under way at the end
-          mbar_wait(qg_full, 0);
-          for (int s = 0; s < L::kst; ++s) if (nk > s) mbar_wait(&k_full[s], (uint32_t)((nk - 1 - s) / L::kst) & 1u);
-          for (int s = 0; s < L::vst; ++s) if (nv > s) mbar_wait(&v_full[s], (uint32_t)((nv - 1 - s) / L::vst) & 1u);
-        }
+      if (j >= L::vst && !(ok = mbar_wait_warp(&v_empty[sv], (uint32_t)(j / L::vst + 1) & 1u))) break;
+      if (lane == 0) {
+        mbar_expect_tx(&v_full[sv], L::ktile);
+        tc_load_tile<D>(smem + L::v + sv * L::ktile, &map_v, hk, kt * kKeys, b, &v_full[sv]);
+      }
+      nv = j + 1;
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      if (lane == 0) {                                          // no copy may still be under way at the end
+        mbar_wait(qg_full, 0);
+        for (int s = 0; s < L::kst; ++s) if (nk > s) mbar_wait(&k_full[s], (uint32_t)((nk - 1 - s) / L::kst) & 1u);
+        for (int s = 0; s < L::vst; ++s) if (nv > s) mbar_wait(&v_full[s], (uint32_t)((nv - 1 - s) / L::vst) & 1u);
       }
     }
   } else if (warp == L::mma) {
-    if (ntiles > 0) {
-      const uint32_t id_s = make_idesc(bf16, kKeys, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
-      const uint64_t dq = make_desc(smem_u32(smem + L::q)), dg = make_desc(smem_u32(smem + L::g)), dk = make_desc(smem_u32(smem + L::k)),
-                     dv = make_desc(smem_u32(smem + L::v)), dkm = make_desc_mn(smem_u32(smem + L::k), kTcHalf);
-      constexpr uint64_t step = L::ktile >> 4;
-      bool ok = mbar_wait_warp(qg_full, 0);
-      auto scores = [&](int j) {
-        ok = mbar_wait_warp(&k_full[j % L::kst], (uint32_t)(j / L::kst) & 1u);
-        tc_fence_after();
-        if (ok && elect_one()) tc_scores<D>(tmem + kKeys * (j & 1), dq, dk + (j % L::kst) * step, id_s);
-      };
-      auto dprobs = [&](int j) {
-        ok = mbar_wait_warp(&v_full[j % L::vst], (uint32_t)(j / L::vst) & 1u);
-        tc_fence_after();
-        if (ok && elect_one()) {
-          tc_scores<D>(tmem + L::tmem_dp, dg, dv + (j % L::vst) * step, id_s);
-          umma_commit(sd_full);
-          umma_commit(&v_empty[j % L::vst]);
-        }
-      };
-      if (ok) scores(0);
-      if (ok) dprobs(0);
-      if (ok && nit > 1) scores(1);
-      for (int j = 0; j < nit && ok; ++j) {
-        if (j + 1 < nit) {
-          ok = mbar_wait_warp(dp_empty, (uint32_t)j & 1u);        // dP of this tile is in registers
-          if (ok) dprobs(j + 1);
-          if (!ok) break;
-        }
-        ok = mbar_wait_warp(&ds_full[j & 1], (uint32_t)(j >> 1) & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          if (j >= ahead)
-            tc_accumulate<2, 0, kKeys / 16>(tmem + L::tmem_dq, tmem + kKeys * (j & 1), dkm + (j % L::kst) * step, id_o, j > ahead ? 1u : 0u);
-          umma_commit(&k_empty[j % L::kst]);
-        }
-        if (j + 2 < nit) scores(j + 2);                        // over S and dS of this tile, read by the product before it
+    const uint32_t id_s = make_idesc(bf16, kKeys, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
+    const uint64_t dq = make_desc(smem_u32(smem + L::q)), dg = make_desc(smem_u32(smem + L::g)), dk = make_desc(smem_u32(smem + L::k)),
+                   dv = make_desc(smem_u32(smem + L::v)), dkm = make_desc_mn(smem_u32(smem + L::k), kTcHalf);
+    constexpr uint64_t step = L::ktile >> 4;
+    bool ok = mbar_wait_warp(qg_full, 0);
+    auto scores = [&](int j) {
+      ok = mbar_wait_warp(&k_full[j % L::kst], (uint32_t)(j / L::kst) & 1u);
+      tc_fence_after();
+      if (ok && elect_one()) tc_scores<D>(tmem + kKeys * (j & 1), dq, dk + (j % L::kst) * step, id_s);
+    };
+    auto dprobs = [&](int j) {
+      ok = mbar_wait_warp(&v_full[j % L::vst], (uint32_t)(j / L::vst) & 1u);
+      tc_fence_after();
+      if (ok && elect_one()) {
+        tc_scores<D>(tmem + L::tmem_dp, dg, dv + (j % L::vst) * step, id_s);
+        umma_commit(sd_full);
+        umma_commit(&v_empty[j % L::vst]);
       }
-      if (elect_one()) umma_commit(ok ? done : drain);
-      if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
+    };
+    if (ok) scores(0);
+    if (ok) dprobs(0);
+    if (ok && nit > 1) scores(1);
+    for (int j = 0; j < nit && ok; ++j) {
+      if (j + 1 < nit) {
+        ok = mbar_wait_warp(dp_empty, (uint32_t)j & 1u);        // dP of this tile is in registers
+        if (ok) dprobs(j + 1);
+        if (!ok) break;
+      }
+      ok = mbar_wait_warp(&ds_full[j & 1], (uint32_t)(j >> 1) & 1u);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        if (j >= ahead)
+          tc_accumulate<2, 0, kKeys / 16>(tmem + L::tmem_dq, tmem + kKeys * (j & 1), dkm + (j % L::kst) * step, id_o, j > ahead ? 1u : 0u);
+        umma_commit(&k_empty[j % L::kst]);
+      }
+      if (j + 2 < nit) scores(j + 2);                        // over S and dS of this tile, read by the product before it
     }
+    if (elect_one()) umma_commit(ok ? done : drain);
+    if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
   } else {
     const int part = warp >> 2, quad = warp & 3;
     const int row = quad * 32 + lane, i = q0 + row;
@@ -359,13 +355,14 @@ sw_dq_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       __syncwarp();
       if (lane == 0) mbar_arrive(&ds_full[j & 1]);
     }
-    if (ok && ntiles > 0) ok = mbar_wait_warp(done, 0);
+    if (ok) ok = mbar_wait_warp(done, 0);
     if (!ok) *abort_flag = 1;
     tc_fence_after();
     if (ok && 32 * part < D) {
       T* dst = static_cast<T*>(p.dq) + (((int64_t)b * p.T + i) * p.Hq + h) * D + 32 * part;
       uint32_t o[32];
-      if (ntiles > 0) { tmem_ld32(tmem + L::tmem_dq + 32 * part + lane_off, o); tmem_wait_ld32(o); }
+      tmem_ld32(tmem + L::tmem_dq + 32 * part + lane_off, o);
+      tmem_wait_ld32(o);
       if (i < p.T) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
@@ -481,48 +478,46 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   } else tmem = tc_start<L::threads, L::tmem_cols>(tmem_slot, warp == L::mma);
 
   if (warp == L::tma) {
-    if (nit > 0) {
+    if (lane == 0) {
+      mbar_expect_tx(kv_full, 2 * L::tile);
+      tc_load_tile<D>(smem + L::k, &map_k, hk, k0, b, kv_full);
+      tc_load_tile<D>(smem + L::v, &map_v, hk, k0, b, kv_full);
+    }
+    bool ok = true;
+    int nq = 0, ng = 0;
+    uint32_t patched = 0;
+    for (int it = 0; it < nit && ok; ++it) {
+      const int h = h_first + it / per_head, q0 = (qlo + it % per_head) * kQ;
+      const int sq = it % L::qst, sg = it % L::gst;
+      const bool ends = q0 + kQ > n && n < p.T;            // the sequence ends inside this tile
+      uint8_t *tq = smem + L::q + sq * L::qtile, *tg = smem + L::g + sg * L::qtile;
+      if (it >= L::qst && !(ok = mbar_wait_warp(&q_empty[sq], (uint32_t)(it / L::qst + 1) & 1u))) break;
       if (lane == 0) {
-        mbar_expect_tx(kv_full, 2 * L::tile);
-        tc_load_tile<D>(smem + L::k, &map_k, hk, k0, b, kv_full);
-        tc_load_tile<D>(smem + L::v, &map_v, hk, k0, b, kv_full);
+        uint64_t* bar = ends ? patch : &q_full[sq];
+        mbar_expect_tx(bar, ends ? 2 * L::qtile : L::qtile);
+        tc_load_tile<D>(tq, &map_q, h, q0, b, bar);
       }
-      bool ok = true;
-      int nq = 0, ng = 0;
-      uint32_t patched = 0;
-      for (int it = 0; it < nit && ok; ++it) {
-        const int h = h_first + it / per_head, q0 = (qlo + it % per_head) * kQ;
-        const int sq = it % L::qst, sg = it % L::gst;
-        const bool ends = q0 + kQ > n && n < p.T;            // the sequence ends inside this tile
-        uint8_t *tq = smem + L::q + sq * L::qtile, *tg = smem + L::g + sg * L::qtile;
-        if (it >= L::qst && !(ok = mbar_wait_warp(&q_empty[sq], (uint32_t)(it / L::qst + 1) & 1u))) break;
-        if (lane == 0) {
-          uint64_t* bar = ends ? patch : &q_full[sq];
-          mbar_expect_tx(bar, ends ? 2 * L::qtile : L::qtile);
-          tc_load_tile<D>(tq, &map_q, h, q0, b, bar);
-        }
-        nq = ends ? it : it + 1;
-        if (it >= L::gst && !(ok = mbar_wait_warp(&g_empty[sg], (uint32_t)(it / L::gst + 1) & 1u))) break;
-        if (lane == 0) {
-          uint64_t* bar = ends ? patch : &g_full[sg];
-          if (!ends) mbar_expect_tx(bar, L::qtile);
-          tc_load_tile<D>(tg, &map_g, h, q0, b, bar);
-        }
-        ng = ends ? it : it + 1;
-        if (ends) {
-          if (!(ok = mbar_wait_warp(patch, patched++ & 1u))) break;
-          tc_clear_rows<D, kQ>(tq, n - q0);
-          tc_clear_rows<D, kQ>(tg, n - q0);
-          if (lane == 0) { mbar_arrive(&q_full[sq]); mbar_arrive(&g_full[sg]); }
-        }
+      nq = ends ? it : it + 1;
+      if (it >= L::gst && !(ok = mbar_wait_warp(&g_empty[sg], (uint32_t)(it / L::gst + 1) & 1u))) break;
+      if (lane == 0) {
+        uint64_t* bar = ends ? patch : &g_full[sg];
+        if (!ends) mbar_expect_tx(bar, L::qtile);
+        tc_load_tile<D>(tg, &map_g, h, q0, b, bar);
       }
-      if (!ok) {
-        *abort_flag = 1;
-        if (lane == 0) {                                          // no copy may still be under way at the end
-          mbar_wait(kv_full, 0);
-          for (int s = 0; s < L::qst; ++s) if (nq > s) mbar_wait(&q_full[s], (uint32_t)((nq - 1 - s) / L::qst) & 1u);
-          for (int s = 0; s < L::gst; ++s) if (ng > s) mbar_wait(&g_full[s], (uint32_t)((ng - 1 - s) / L::gst) & 1u);
-        }
+      ng = ends ? it : it + 1;
+      if (ends) {
+        if (!(ok = mbar_wait_warp(patch, patched++ & 1u))) break;
+        tc_clear_rows<D, kQ>(tq, n - q0);
+        tc_clear_rows<D, kQ>(tg, n - q0);
+        if (lane == 0) { mbar_arrive(&q_full[sq]); mbar_arrive(&g_full[sg]); }
+      }
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      if (lane == 0) {                                          // no copy may still be under way at the end
+        mbar_wait(kv_full, 0);
+        for (int s = 0; s < L::qst; ++s) if (nq > s) mbar_wait(&q_full[s], (uint32_t)((nq - 1 - s) / L::qst) & 1u);
+        for (int s = 0; s < L::gst; ++s) if (ng > s) mbar_wait(&g_full[s], (uint32_t)((ng - 1 - s) / L::gst) & 1u);
       }
     }
   } else if (warp == L::stats) {
@@ -553,47 +548,45 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
     if (!ok) *abort_flag = 1;
   } else if (warp == L::mma) {
-    if (nit > 0) {
-      const uint32_t id_s = make_idesc(bf16, kQ, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
-      const uint64_t dk = make_desc(smem_u32(smem + L::k)), dv = make_desc(smem_u32(smem + L::v)), dq = make_desc(smem_u32(smem + L::q)),
-                     dg = make_desc(smem_u32(smem + L::g)), dqm = make_desc_mn(smem_u32(smem + L::q), kTcHalf),
-                     dgm = make_desc_mn(smem_u32(smem + L::g), kTcHalf);
-      constexpr uint64_t step = L::qtile >> 4;
-      bool ok = mbar_wait_warp(kv_full, 0);
-      auto scores = [&](int it) {
-        ok = mbar_wait_warp(&q_full[it % L::qst], (uint32_t)(it / L::qst) & 1u);
-        tc_fence_after();
-        if (ok && elect_one()) { tc_scores<D>(tmem, dk, dq + (it % L::qst) * step, id_s); umma_commit(s_full); }
-      };
-      auto dprobs = [&](int it) {
-        ok = mbar_wait_warp(&g_full[it % L::gst], (uint32_t)(it / L::gst) & 1u);
-        tc_fence_after();
-        if (ok && elect_one()) { tc_scores<D>(tmem + L::tmem_dp, dv, dg + (it % L::gst) * step, id_s); umma_commit(dp_full); }
-      };
-      if (ok) scores(0);
-      if (ok) dprobs(0);
-      for (int it = 0; it < nit && ok; ++it) {
-        ok = mbar_wait_warp(p_ready, (uint32_t)it & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          tc_accumulate<2, 0, kQ / 16>(tmem + L::tmem_dv, tmem, dgm + (it % L::gst) * step, id_o, it > 0 ? 1u : 0u);
-          umma_commit(&g_empty[it % L::gst]);                     // dP of this tile was issued before: dO is done with
-        }
-        if (it + 1 < nit) scores(it + 1);
-        if (!ok) break;
-        ok = mbar_wait_warp(ds_ready, (uint32_t)it & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          tc_accumulate<2, 0, kQ / 16>(tmem + L::tmem_dk, tmem + L::tmem_dp, dqm + (it % L::qst) * step, id_o, it > 0 ? 1u : 0u);
-          umma_commit(&q_empty[it % L::qst]);
-        }
-        if (it + 1 < nit) dprobs(it + 1);
+    const uint32_t id_s = make_idesc(bf16, kQ, 0, 0), id_o = make_idesc(bf16, D, 0, 1);
+    const uint64_t dk = make_desc(smem_u32(smem + L::k)), dv = make_desc(smem_u32(smem + L::v)), dq = make_desc(smem_u32(smem + L::q)),
+                   dg = make_desc(smem_u32(smem + L::g)), dqm = make_desc_mn(smem_u32(smem + L::q), kTcHalf),
+                   dgm = make_desc_mn(smem_u32(smem + L::g), kTcHalf);
+    constexpr uint64_t step = L::qtile >> 4;
+    bool ok = mbar_wait_warp(kv_full, 0);
+    auto scores = [&](int it) {
+      ok = mbar_wait_warp(&q_full[it % L::qst], (uint32_t)(it / L::qst) & 1u);
+      tc_fence_after();
+      if (ok && elect_one()) { tc_scores<D>(tmem, dk, dq + (it % L::qst) * step, id_s); umma_commit(s_full); }
+    };
+    auto dprobs = [&](int it) {
+      ok = mbar_wait_warp(&g_full[it % L::gst], (uint32_t)(it / L::gst) & 1u);
+      tc_fence_after();
+      if (ok && elect_one()) { tc_scores<D>(tmem + L::tmem_dp, dv, dg + (it % L::gst) * step, id_s); umma_commit(dp_full); }
+    };
+    if (ok) scores(0);
+    if (ok) dprobs(0);
+    for (int it = 0; it < nit && ok; ++it) {
+      ok = mbar_wait_warp(p_ready, (uint32_t)it & 1u);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        tc_accumulate<2, 0, kQ / 16>(tmem + L::tmem_dv, tmem, dgm + (it % L::gst) * step, id_o, it > 0 ? 1u : 0u);
+        umma_commit(&g_empty[it % L::gst]);                     // dP of this tile was issued before: dO is done with
       }
-      if (elect_one()) umma_commit(ok ? done : drain);
-      if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
+      if (it + 1 < nit) scores(it + 1);
+      if (!ok) break;
+      ok = mbar_wait_warp(ds_ready, (uint32_t)it & 1u);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        tc_accumulate<2, 0, kQ / 16>(tmem + L::tmem_dk, tmem + L::tmem_dp, dqm + (it % L::qst) * step, id_o, it > 0 ? 1u : 0u);
+        umma_commit(&q_empty[it % L::qst]);
+      }
+      if (it + 1 < nit) dprobs(it + 1);
     }
+    if (elect_one()) umma_commit(ok ? done : drain);
+    if (!ok) { *abort_flag = 1; mbar_wait_warp(drain, 0); }
   } else {
     const int part = warp >> 2, quad = warp & 3;
     const int row = quad * 32 + lane, j = k0 + row;
@@ -653,7 +646,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       __syncwarp();
       if (lane == 0) { mbar_arrive(ds_ready); mbar_arrive(&st_empty[it & 1]); }
     }
-    if (ok && nit > 0) ok = mbar_wait_warp(done, 0);
+    if (ok) ok = mbar_wait_warp(done, 0);
     if (!ok) *abort_flag = 1;
     tc_fence_after();
     if (ok) {
@@ -663,7 +656,7 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const float mul = which == 0 ? p.scale / f : BwdRange<T>::unshift;
       const uint32_t acc = tmem + (which == 0 ? L::tmem_dk : L::tmem_dv) + from + lane_off;
       const bool parts = kt < sp.part_tiles;
-      const bool live = j < n && nit > 0;
+      const bool live = j < n;
       float* sum = nullptr;
       if (parts) {
         sum = far ? dkv_far_part(sp, (int64_t)p.B * p.Hk, hs, chunk, bh, kt, D) : dkv_near_part(sp, (int64_t)p.B * p.Hk, hs, bh, kt, D);
@@ -673,7 +666,8 @@ sw_dkv_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll 1
       for (int c0 = 0; c0 < kWide; c0 += 32) {
         uint32_t o[32];
-        if (nit > 0) { tmem_ld32(acc + c0, o); tmem_wait_ld32(o); }
+        tmem_ld32(acc + c0, o);
+        tmem_wait_ld32(o);
         if (parts) {
 #pragma unroll
           for (int v = 0; v < 8; ++v) {
