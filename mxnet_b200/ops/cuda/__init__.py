@@ -7,12 +7,14 @@ paths are these kernels.
 """
 import ctypes
 import os
+import threading
 
 import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libmxb200_kernels.so')
 _lib = None
+_lock = threading.Lock()
 _checked = False
 
 
@@ -20,12 +22,15 @@ def lib():
     """The loaded kernel library (raises if it is missing or fails to load)."""
     global _lib
     if _lib is None:
-        if not os.path.exists(LIB_PATH):
-            raise RuntimeError('sm_100a kernel library not built: run `python -m mxnet_b200.ops.cuda.build` '
-                               '(expected %s)' % LIB_PATH)
-        _lib = ctypes.CDLL(LIB_PATH)
-        from . import _signatures
-        _signatures.declare(_lib)
+        with _lock:
+            if _lib is None:
+                if not os.path.exists(LIB_PATH):
+                    raise RuntimeError('sm_100a kernel library not built: run `python -m mxnet_b200.ops.cuda.build` '
+                                       '(expected %s)' % LIB_PATH)
+                loaded = ctypes.CDLL(LIB_PATH)
+                from . import _signatures
+                _signatures.declare(loaded)
+                _lib = loaded            # only now: without its prototypes a call would cut addresses to 32 bits
     return _lib
 
 

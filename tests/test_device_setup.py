@@ -66,6 +66,39 @@ def test_no_thread_launches_before_the_setup(tmp_path, flags):
     assert 'WARNING: ThreadSanitizer' not in r.stderr
 
 
+def test_no_thread_gets_the_library_before_its_prototypes(monkeypatch):
+    import threading
+    import time
+    import types
+    from mxnet_b200.ops import cuda
+    from mxnet_b200.ops.cuda import _signatures
+
+    def declare(library):
+        time.sleep(0.05)
+        library.declared = True
+    made, seen, start = [], [], threading.Barrier(6)
+
+    def load(path):
+        made.append(types.SimpleNamespace(declared=False))
+        return made[-1]
+    monkeypatch.setattr(cuda, '_lib', None)
+    monkeypatch.setattr(cuda, 'LIB_PATH', __file__)
+    monkeypatch.setattr(cuda.ctypes, 'CDLL', load)
+    monkeypatch.setattr(_signatures, 'declare', declare)
+
+    def call():
+        start.wait()
+        seen.append(cuda.lib().declared)
+        time.sleep(0.01)
+        seen.append(cuda.lib().declared)
+    threads = [threading.Thread(target=call) for _ in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert seen == [True] * 12 and len(made) == 1
+
+
 FIRST_CALLS = """
 import threading
 import torch
