@@ -221,7 +221,11 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
 inline void ensure_context() {
   static thread_local bool bound = false;
   if (!bound) {
+    // a capture of this thread, or of any other in the strict mode, would end at a call like this one
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     cudaFree(nullptr);
+    cudaThreadExchangeStreamCaptureMode(&mode);
     bound = true;
   }
 }

@@ -126,3 +126,51 @@ def test_a_block_that_cannot_be_captured_runs_eagerly(where):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     run = subprocess.run([sys.executable, '-c', FAIL, where], cwd=root, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and 'carried on' in run.stdout and 'capture failed' in run.stderr, run.stdout + run.stderr[-3000:]
+
+FIRST = """
+import sys
+import torch
+import mxnet_b200 as mx
+
+op = lambda name: mx.ops.get('_contrib_' + name).fn
+D = int(sys.argv[2])
+dtype = getattr(torch, sys.argv[3])
+draw = lambda *shape: torch.randn(*shape, device='cuda').to(dtype)
+q, k, g = draw(2, 200, 4, D), draw(2, 200, 2, D), draw(2, 200, 4, D)
+one, few, caches = draw(2, 4, D), draw(2, 2, D), [draw(2, 50, 2, D) for _ in range(2)]
+at, tok, freq = torch.tensor([7, 300], device='cuda'), torch.arange(8, device='cuda'), torch.rand(D // 2, device='cuda')
+logits, places = draw(8, 1000), torch.arange(200, device='cuda')
+
+
+def attention():
+    a = q.detach().requires_grad_(True)
+    with torch.autograd.set_multithreading_enabled(False):
+        y = op('sldwin_attention')(a, k, k, window=60, sinks=2)
+        return y.detach(), torch.autograd.grad(y, a, g)[0]
+
+
+calls = {'attention': attention,
+         'step': lambda: (op('sldwin_attention_step')(one, few, few, *caches, at, sinks=2),) + tuple(c.clone() for c in caches),
+         'fill': lambda: tuple(c.clone() for c in op('sldwin_cache_fill')(k, k, *caches, sinks=2)),
+         'rotary': lambda: (op('rotary_embedding')(q, places, freq),),
+         'logprobs': lambda: op('token_log_probs')(logits, tok, topk=4)}
+call = calls[sys.argv[1]]
+before = [c.clone() for c in caches]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = call()
+graph.replay()
+got = [t.clone() for t in got]
+for c, b in zip(caches, before):
+    c.copy_(b)
+assert all(torch.equal(a, b) for a, b in zip(got, call()))
+print('captured')
+"""
+
+
+@pytest.mark.parametrize('what,D,dtype', [('attention', 64, 'float16'), ('attention', 128, 'bfloat16'), ('attention', 40, 'float32'),
+                                          ('step', 64, 'float16'), ('logprobs', 64, 'bfloat16')])
+def test_a_first_call_inside_a_capture(what, D, dtype):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, '-c', FIRST, what, str(D), dtype], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and 'captured' in run.stdout, run.stdout + run.stderr[-3000:]
