@@ -17,6 +17,7 @@ asynchronous work are stored and rethrown at the next synchronisation point
 from __future__ import annotations
 
 import contextlib
+import os
 import threading
 import weakref
 
@@ -57,6 +58,10 @@ def at_sync(check):
 def check_reports():
     for check in _sync_checks:
         check()
+
+
+# a forked child has none of the host memory that a device writes to
+os.register_at_fork(after_in_child=_sync_checks.clear)
 
 
 def _rethrow_pending():

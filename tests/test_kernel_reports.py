@@ -51,6 +51,28 @@ def test_the_word_is_there_inside_a_capture(library, monkeypatch):
     assert sldwin_ops._error_word() == ctypes.addressof(library.word)
 
 
+def test_a_forked_child_does_not_look_at_the_devices_memory():
+    run = subprocess.run([sys.executable, '-c', """
+import os
+from mxnet_b200 import engine, nd
+
+
+def check():
+    os.kill(os.getpid(), 9)                 # what reading memory would do that the child does not have
+
+
+engine.at_sync(check)
+pid = os.fork()
+if pid == 0:
+    nd.zeros((2,)).wait_to_read()
+    nd.waitall()
+    os._exit(0)
+print('child', os.waitpid(pid, 0)[1], len(engine._sync_checks))
+engine._sync_checks.clear()
+"""], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and 'child 0 1' in run.stdout, run.stdout + run.stderr[-2000:]
+
+
 CAPTURED = """
 import torch
 import mxnet_b200 as mx
