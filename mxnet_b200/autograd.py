@@ -215,6 +215,8 @@ def _calling_thread(tensors):
         except AttributeError:
             _here.devices = {first.index}
         return torch.autograd.set_multithreading_enabled(False)
+    if crossed or (first is not None and first.type != 'cuda' and torch.cuda.is_initialized()):
+        _worked.update(range(torch.cuda.device_count()))           # some of them; which ones only the graph knows
     _worked.update(t.device.index for t in tensors if t.device.type == 'cuda')
     return _HERE
 

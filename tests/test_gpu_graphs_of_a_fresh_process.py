@@ -27,6 +27,8 @@ def train(static, ask):
     for _ in range(6):
         with autograd.record():
             y = net(x).square().mean()
+            if ask == 'host':
+                y = y.as_in_context(mx.cpu())
         if ask == 'grad':
             ws = [p.data(ctx) for p in net.collect_params().values() if p.grad_req != 'null']
             autograd.grad(y, ws)
@@ -49,7 +51,7 @@ else:
 
 
 @pytest.mark.parametrize('how', [('static', 'backward', 'main'), ('plain', 'backward', 'main'), ('static', 'grad', 'main'),
-                                 ('static', 'backward', 'thread')])
+                                 ('static', 'host', 'main'), ('static', 'backward', 'thread')])
 def test_a_training_block_is_captured(how):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     run = subprocess.run([sys.executable, '-c', TRAIN, *how], cwd=root, capture_output=True, text=True, timeout=300)

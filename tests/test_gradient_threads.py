@@ -70,6 +70,18 @@ def test_a_graph_over_several_devices_keeps_its_workers(monkeypatch):
     assert not _state.state.crossed
 
 
+def test_a_pass_from_a_host_head_may_have_run_on_any_devices_worker(monkeypatch):
+    fresh(monkeypatch)
+    host = [SimpleNamespace(device=torch.device('cpu'))]
+    assert not stays(autograd._calling_thread(on(0, 0) + host)) and stays(autograd.captured_pass(torch.device('cuda', 1)))
+    assert stays(autograd._calling_thread(host)) is False and stays(autograd.captured_pass(torch.device('cuda', 1)))
+    monkeypatch.setattr(torch.cuda, 'is_initialized', lambda: True)
+    monkeypatch.setattr(torch.cuda, 'device_count', lambda: 2)
+    autograd._calling_thread(host)
+    assert not stays(autograd.captured_pass(torch.device('cuda', 1)))
+    assert stays(autograd._calling_thread(on(1))) and stays(autograd.captured_pass(torch.device('cuda', 1)))
+
+
 @pytest.mark.gpu
 def test_a_recorded_copy_between_devices_is_seen():
     seen = []
