@@ -400,7 +400,10 @@ class CachedOp(object):
             return eager(*args)
         except Exception as e:  # pylint: disable=broad-except
             self._disabled = True
-            _after_failed_capture(arrays[0]._data.device)
+            try:
+                _after_failed_capture(arrays[0]._data.device)
+            except RuntimeError:
+                _log.warning('the device takes no captures any more')      # the eager call says what is wrong with it
             _log.warning('CUDA graph capture failed (%s); block %s runs eagerly', e, type(self.block).__name__,
                          exc_info=bool(env.get('MXNET_CUDA_GRAPHS_VERBOSE')))
             return eager(*args)
